@@ -609,9 +609,8 @@ __global__ __launch_bounds__(256) void token_gemm_f32(const float *__restrict__ 
                 for (int j = 0; j < TN; ++j) { f.b[j][e] = lo4.b[j][e]; f.b[j][4 + e] = hi4.b[j][e]; }
             }
         };
-        // Written on PAIRS of values (two-element vectors): the conversions become one v_cvt_pk_bf16_f32 per pair and the residuals one
-        // v_pk_add_f32 per pair.  The scalar form left that pairing to the SLP vectoriser, which packed 40 of the 128 subtractions of a
-        // k-step and emitted 128 instead of 96 conversions (383 vector instructions per k-step against 48 MFMAs).  Same operations, same bits.
+        // Written on PAIRS of values (two-element vectors): the conversions become one v_cvt_pk_bf16_f32 per pair.  The scalar form left that
+        // pairing to the SLP vectoriser, which emitted 128 instead of 96 conversions per k-step (against 48 MFMAs).  Same operations, same bits.
         auto split8 = [&](const float (&x)[8], bf16x8 &h, bf16x8 &m, bf16x8 &l) {
 #pragma unroll
             for (int e = 0; e < 8; e += 2) {

@@ -17,6 +17,7 @@ import sys
 import tempfile
 
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+NOPK = ['-Xclang', '-target-feature', '-Xclang', '-packed-fp32-ops']          # as csrc/Makefile builds them
 CSRC = os.path.join(ROOT, 'segdistill_amd', 'csrc')
 REG = re.compile(r'\b([va])(\d+)\b|\b([va])\[(\d+):(\d+)\]')
 
@@ -90,7 +91,7 @@ def main():
             if not re.search(r'asm volatile\("[^"]*(global_load|buffer_load)', open(f).read()):
                 continue
             s = os.path.join(tmp, os.path.basename(f) + '.s')
-            subprocess.run(['/opt/rocm/bin/hipcc', '-O3', '-std=c++17', '--offload-arch=gfx950', '-I' + os.path.join(ROOT, 'include'), '-S',
+            subprocess.run(['/opt/rocm/bin/hipcc', '-O3', '-std=c++17', '--offload-arch=gfx950', *NOPK, '-I' + os.path.join(ROOT, 'include'), '-S',
                             '--cuda-device-only', f, '-o', s], check=True, stderr=subprocess.DEVNULL)
             found = audit(s)
             per = {}

@@ -12,6 +12,7 @@ import sys
 import tempfile
 
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+NOPK = ['-Xclang', '-target-feature', '-Xclang', '-packed-fp32-ops']          # as csrc/Makefile builds them
 CSRC = os.path.join(ROOT, 'segdistill_amd', 'csrc')
 SREG = re.compile(r'\bs(\d+)\b|\bs\[(\d+):(\d+)\]')
 
@@ -69,7 +70,7 @@ def main():
             if not re.search(r'asm volatile\("[^"]*(global_load|buffer_load)', src):
                 continue
             s = os.path.join(tmp, os.path.basename(f) + '.s')
-            subprocess.run(['/opt/rocm/bin/hipcc', '-O3', '-std=c++17', '--offload-arch=gfx950', '-I' + os.path.join(ROOT, 'include'), '-S',
+            subprocess.run(['/opt/rocm/bin/hipcc', '-O3', '-std=c++17', '--offload-arch=gfx950', *NOPK, '-I' + os.path.join(ROOT, 'include'), '-S',
                             '--cuda-device-only', f, '-o', s], check=True, stderr=subprocess.DEVNULL)
             found = scan(s)
             print(f'{os.path.basename(f)}: {len(found)} asm vector-memory instruction(s) reading an SGPR a VALU instruction wrote < 5 wait states earlier')
