@@ -292,7 +292,7 @@ int sd_ppm_pool_bwd(void *const *d_pooled, int dtype, long planes, int h, int w,
  *   qkv    [windows, N, 3, heads, D]  the qkv Linear's output as it stands (swin_transformer.py:128-129 before the permute)
  *   out    [windows, N, heads*D]  = (attn @ v).transpose(1, 2).reshape(B_, N, C)   (:148)
  * Bias and mask come PACKED in the accumulator layout of the kernel, sd_window_attn_packed_floats() (= 64 * 64) floats per table:
- * sd_window_attn_pack converts `count` tables [49][49] in the reference's orientation ([query][key]: relative_position_bias[head] of :133-135,
+ * sd_window_attn_pack converts `count` tables [N][N] (N <= 64; the training entry points below read the same layout) in the reference's orientation ([query][key]: relative_position_bias[head] of :133-135,
  * mask[window] of :138; window b uses mask b % mask_windows, :140) and fills padded keys with pad_key_value (-INFINITY for the bias, 0 for the
  * mask); flags[count] (optional) receives 1 for a table with a nonzero entry -- the kernel skips the mask read of windows whose mask is all
  * zero (all but 37 of a 19 x 19 shifted partition).  mask_packed NULL: no mask (mask_flags ignored).
@@ -304,6 +304,66 @@ int sd_window_attn_pack(const float *tables, float *packed, int32_t *flags /* or
                         void *stream);
 int sd_window_attn_fwd_packed(const void *qkv, const float *bias_packed, const float *mask_packed, const int32_t *mask_flags, void *out, int dtype,
                               long windows, int mask_windows, int heads, int tokens_per_window, int head_dim, float scale, void *stream);
+
+/* ---------------------------------------------------------------------------
+ * The same attention with an autograd graph (a Swin student's blocks; csrc/window_train.hip): swin_transformer.py:119-153 and its backward.
+ *   qkv [windows, N, 3, heads, D], out / dout [windows, N, heads*D], dqkv like qkv, storage SD_F32 | SD_BF16; dbias [heads][N][N] fp32
+ *   bias_packed / mask_packed / mask_flags from sd_window_attn_pack (pad -INFINITY for the bias, 0 for the mask).
+ * Softmax, its gradient and the bias gradient are fp32 for both storage types.  A row that bias + mask leave at -inf everywhere has output 0 and no
+ * gradient.  The backward recomputes the probabilities: nothing but the operands is kept.  dbias sums the windows in a fixed order (per-wave slabs in
+ * `workspace`, 16-byte aligned, sd_window_attn_train_workspace_bytes; no atomics).
+ * _supported(): 1 <= N <= 64, D == 32, else SD_E_UNSUPPORTED.  All operands 16-byte aligned.
+ */
+int sd_window_attn_train_supported(int tokens_per_window, int head_dim);
+int sd_window_attn_train_fwd(const void *qkv, const float *bias_packed, const float *mask_packed, const int32_t *mask_flags, void *out, int dtype,
+                             long windows, int mask_windows, int heads, int tokens_per_window, int head_dim, float scale, void *stream);
+size_t sd_window_attn_train_workspace_bytes(long windows, int heads, int tokens_per_window);
+int sd_window_attn_train_bwd(const void *qkv, const float *bias_packed, const float *mask_packed, const int32_t *mask_flags, const void *dout,
+                             void *dqkv, float *dbias, int dtype, long windows, int mask_windows, int heads, int tokens_per_window, int head_dim,
+                             float scale, void *workspace, size_t workspace_bytes, void *stream);
+
+/* ---------------------------------------------------------------------------
+ * A learned position bias by buckets and its gradient (csrc/rel_bias.hip): relative_position_bias_table[relative_position_index] of
+ * swin_transformer.py:133-135 and its autograd (index_put with accumulation), for any bucket map.
+ *   forward   out[h][p] = table[index[p]][h], p < pairs = Nq * Nk; table [buckets][heads], out [heads][pairs], SD_F32 | SD_BF16; every index[p] in
+ *             [0, buckets) (the caller's plan has checked it)
+ *   backward  dtable[b][h] = sum_{index[p] = b} dbias[h][p]: `order` lists the pairs bucket by bucket; chunk i is order[chunk_start[i] ..
+ *             chunk_start[i + 1]) with at most sd_bucket_bias_chunk() pairs of ONE bucket; bucket b owns the chunks [bucket_chunk[b],
+ *             bucket_chunk[b + 1]), at least one (an empty bucket: an empty one).  fp32 sums in a fixed order, the chunks of a bucket in fp64.
+ *             workspace: sd_bucket_bias_workspace_bytes (0 when every bucket is one chunk).
+ */
+int sd_bucket_bias_chunk(void);
+size_t sd_bucket_bias_workspace_bytes(int buckets, int chunks, int heads);
+int sd_bucket_bias_fwd(const void *table, const int32_t *index, void *out, int dtype, int buckets, int heads, long pairs, void *stream);
+int sd_bucket_bias_bwd(const void *dbias, const int32_t *order, const int32_t *chunk_start, const int32_t *bucket_chunk, void *dtable, int dtype,
+                       int buckets, int chunks, int heads, long pairs, void *workspace, size_t workspace_bytes, void *stream);
+
+/* ---------------------------------------------------------------------------
+ * Distillation from a teacher's top logits (csrc/topk_select.hip, csrc/topk_kl.hip): the teacher's part of the pixel-wise criterion
+ * (losses.py:47-49,108-112) as k logits, their classes and one logit for all others.
+ * Layout: [B][C][P] with the class axis in the middle (class planes, P = H*W), P == 1: contiguous rows of C classes.
+ *   sd_topk_select  values [B][k][P] (storage type of x) descending, index [B][k][P]; equal values by ascending class, NaN above everything;
+ *                   rest [B][P] fp32 = tau * log sum_{c not chosen} exp(x_c / tau), -INFINITY when k == C.
+ *   sd_topk_kl_fwd  p = softmax([values, rest] / tau) (rest == NULL: of the values alone), q = softmax(S / tau):
+ *                   loss = alpha / n * sum_rows [ sum_j p_j (log p_j - log q_index_j) + p_rest (log p_rest - log sum_{c not listed} q_c) ],
+ *                   n = rows with valid != 0 (valid == NULL: all; n = 0: loss 0).  An index outside [0, C) is no entry; a row without entries and
+ *                   rest has no loss; a class listed twice gets both entries' probability.  stats [B*P][4] (16-byte aligned) and inv_rows [1] go to
+ *                   the backward.  Rows with valid == 0 are not read.
+ *   sd_topk_kl_bwd  dS (storage type of S), upstream [1] on the device.
+ * k <= sd_topk_max_entries(), C <= sd_topk_max_classes(); class planes keep a bit and an entry column per pixel in LDS: sd_topk_kl_supported().
+ * values may be SD_F32 or SD_BF16 whatever S is.  Deterministic: every sum is taken in a fixed order.
+ */
+int sd_topk_max_entries(void);
+int sd_topk_max_classes(void);
+int sd_topk_select(const void *x, void *values, int32_t *index, float *rest, int dtype, long B, int C, long P, int k, float tau, void *stream);
+int sd_topk_kl_supported(long B, int C, long P, int k);
+size_t sd_topk_kl_workspace_bytes(long B, int C, long P, int k);
+int sd_topk_kl_fwd(const void *S, const void *values, const int32_t *index, const float *rest, const uint8_t *valid, int dtype, int values_dtype,
+                   long B, int C, long P, int k, float tau, float alpha, float *stats, float *inv_rows, float *loss, void *workspace,
+                   size_t workspace_bytes, void *stream);
+int sd_topk_kl_bwd(const void *S, const void *values, const int32_t *index, const float *rest, const uint8_t *valid, int dtype, int values_dtype,
+                   long B, int C, long P, int k, float tau, float alpha, const float *stats, const float *inv_rows, const float *upstream, void *dS,
+                   void *stream);
 
 /* ---------------------------------------------------------------------------
  * CGD / CD criterion on TOKEN-MAJOR operands S, T [B][P][C] (C contiguous; P = h*w pixels): the decoder features of a SegFormer head

@@ -56,6 +56,21 @@ SIGNATURES = {
     'sd_window_attn_packed_floats': (_sz, []),
     'sd_window_attn_pack': (_i, [_vp, _vp, _vp, _i, _i, _f, _vp]),
     'sd_window_attn_fwd_packed': (_i, [_vp, _vp, _vp, _vp, _vp, _i, C.c_long, _i, _i, _i, _i, _f, _vp]),
+    'sd_window_attn_train_supported': (_i, [_i, _i]),
+    'sd_window_attn_train_fwd': (_i, [_vp, _vp, _vp, _vp, _vp, _i, C.c_long, _i, _i, _i, _i, _f, _vp]),
+    'sd_window_attn_train_workspace_bytes': (_sz, [C.c_long, _i, _i]),
+    'sd_window_attn_train_bwd': (_i, [_vp] * 7 + [_i, C.c_long, _i, _i, _i, _i, _f, _vp, _sz, _vp]),
+    'sd_bucket_bias_chunk': (_i, []),
+    'sd_bucket_bias_workspace_bytes': (_sz, [_i, _i, _i]),
+    'sd_bucket_bias_fwd': (_i, [_vp, _vp, _vp, _i, _i, _i, C.c_long, _vp]),
+    'sd_bucket_bias_bwd': (_i, [_vp] * 5 + [_i, _i, _i, _i, C.c_long, _vp, _sz, _vp]),
+    'sd_topk_max_entries': (_i, []),
+    'sd_topk_max_classes': (_i, []),
+    'sd_topk_select': (_i, [_vp, _vp, _vp, _vp, _i, C.c_long, _i, C.c_long, _i, _f, _vp]),
+    'sd_topk_kl_supported': (_i, [C.c_long, _i, C.c_long, _i]),
+    'sd_topk_kl_workspace_bytes': (_sz, [C.c_long, _i, C.c_long, _i]),
+    'sd_topk_kl_fwd': (_i, [_vp] * 5 + [_i, _i, C.c_long, _i, C.c_long, _i, _f, _f, _vp, _vp, _vp, _vp, _sz, _vp]),
+    'sd_topk_kl_bwd': (_i, [_vp] * 5 + [_i, _i, C.c_long, _i, C.c_long, _i, _f, _f, _vp, _vp, _vp, _vp, _vp]),
     'sd_cgd_kl_tok_workspace_bytes': (_sz, [_i, _i, C.c_long]),
     'sd_cgd_kl_tok_fwd': (_i, [_vp, _vp, _i, _i, _i, C.c_long, _i, _f, _f, _vp, _vp, _vp, _vp, _vp, _sz, _vp]),
     'sd_cgd_kl_tok_bwd': (_i, [_vp, _vp, _i, _i, _i, C.c_long, _i, _f, _f, _vp, _vp, _vp, _vp, _vp]),

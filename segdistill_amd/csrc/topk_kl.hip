@@ -1,0 +1,530 @@
+// topk_kl.hip -- distillation from a teacher's top logits: the criterion and its gradient, gfx950.
+//
+// A row holds the student's logits z_c and k entries (i_j, v_j) of the teacher, with `rest` (optional) the one logit that stands for every
+// other class (topk_select.hip).  With p = softmax([v, rest] / tau), q = softmax(z / tau), A the set of the row's entry classes:
+//   KL   = sum_j p_j (log p_j - log q_{i_j}) + p_r (log p_r - log q_r),     q_r = sum_{c not in A} q_c
+//   dKL/dz_c * tau = q_c - sum_{j: i_j = c} p_j   (c in A),    (q_r - p_r) u_c   (c not in A),   u = softmax of z / tau over the classes not in A
+// and without `rest` the same with p_r = 0 ((q_r - 0) u_c = q_c).  The streaming pass therefore takes the softmax of the classes OUTSIDE A --
+// excluded one by one, not subtracted afterwards: a student that agrees with the teacher leaves q_r small -- and the entries join at the end.
+//
+// Each row keeps (m_r, w, m, 1/s): its gradient is w 2^{(z_c - m_r) c2} outside A, with w = (q_r - p_r) / s_r.
+// Memory bound: the forward reads z, the backward reads z and writes dz; nothing of the size of z is kept between them.
+#include <hip/hip_runtime.h>
+#include <math.h>
+
+#include "topk_device.h"
+
+namespace sd {
+namespace {
+
+struct Entries {          // one row's teacher entries lie at j * stride
+    const void *values;
+    const int *index;
+    const float *rest;               // NULL: the entries are all the teacher says
+    const unsigned char *valid;      // NULL: every row counts
+    int values_bf16, k;
+};
+__device__ __forceinline__ float entry_value(const Entries &e, size_t at) {
+    return e.values_bf16 ? VecIO<bf16_t>::load1(static_cast<const bf16_t *>(e.values) + at) : static_cast<const float *>(e.values)[at];
+}
+
+// p log(p / q) with 0 log 0 = 0, from p and the logarithms
+__device__ __forceinline__ float kl_term(float p, float logp, float logq) { return p > 0.f || p != p ? p * (logp - logq) : 0.f; }
+
+// The workgroup's sum of row losses and its number of counted rows -> part[2 * block], part[2 * block + 1].
+template <int NT>
+__device__ __forceinline__ void write_partial(double kl, double n, double *__restrict__ part) {
+    __shared__ double acc[2 * NT / 64];
+#pragma unroll
+    for (int d = 32; d > 0; d >>= 1) kl += __shfl_xor(kl, d, 64), n += __shfl_xor(n, d, 64);
+    if ((threadIdx.x & 63) == 0) acc[threadIdx.x >> 6] = kl, acc[NT / 64 + (threadIdx.x >> 6)] = n;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        double a = 0, b = 0;
+        for (int w = 0; w < NT / 64; ++w) a += acc[w], b += acc[NT / 64 + w];
+        part[2 * (size_t)blockIdx.x] = a;
+        part[2 * (size_t)blockIdx.x + 1] = b;
+    }
+}
+
+__global__ __launch_bounds__(256) void topk_kl_finish(const double *__restrict__ part, int n, float alpha, float *__restrict__ loss, float *__restrict__ inv_n) {
+    double kl = 0, rows = 0;
+    for (int i = threadIdx.x; i < n; i += 256) kl += part[2 * i], rows += part[2 * i + 1];
+    __shared__ double acc[8];
+#pragma unroll
+    for (int d = 32; d > 0; d >>= 1) kl += __shfl_xor(kl, d, 64), rows += __shfl_xor(rows, d, 64);
+    if ((threadIdx.x & 63) == 0) acc[threadIdx.x >> 6] = kl, acc[4 + (threadIdx.x >> 6)] = rows;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        kl = acc[0] + acc[1] + acc[2] + acc[3], rows = acc[4] + acc[5] + acc[6] + acc[7];
+        const double inv = rows > 0 ? 1.0 / rows : 0.0;              // no row left: the loss and every gradient are 0
+        loss[0] = (float)(kl * inv * (double)alpha);
+        inv_n[0] = (float)inv;
+    }
+}
+
+// ---- class planes [B, C, P]: one thread per pixel ------------------------------------------------------------------------------------------------
+// The pixel's set A is a bit mask in LDS, a column per thread: words[w][thread].  Classes come by in ascending order, so the entries are met in
+// ascending order too, and the rank of an entry -- the bits below it -- is its place in a second column: no search, no sort, and a class that
+// appears twice has one place.
+template <int BT>
+struct Columns {
+    unsigned *words, *ranks;
+    float *vals;
+    __device__ Columns(unsigned char *lds, int nwords) {
+        words = reinterpret_cast<unsigned *>(lds) + threadIdx.x;
+        ranks = words + (size_t)nwords * BT;
+        vals = reinterpret_cast<float *>(ranks + (size_t)nwords * BT);
+    }
+    __device__ int rank(int c) const { return (int)ranks[(c >> 5) * BT] + __popc(words[(c >> 5) * BT] & ((1u << (c & 31)) - 1)); }
+};
+template <int BT>
+__device__ __forceinline__ int mark_entries(const Columns<BT> &col, int nwords, const Entries &e, size_t at, long P, int C) {
+    for (int w = 0; w < nwords; ++w) col.words[w * BT] = 0;
+    for (int j = 0; j < e.k; ++j) {
+        const int c = e.index[at + (size_t)j * P];
+        if ((unsigned)c < (unsigned)C) col.words[(c >> 5) * BT] |= 1u << (c & 31);
+    }
+    int n = 0;
+    for (int w = 0; w < nwords; ++w) col.ranks[w * BT] = n, n += __popc(col.words[w * BT]);
+    return n;
+}
+// The teacher's maximum and normaliser over its live entries and the rest.
+__device__ __forceinline__ Online teacher(const Entries &e, size_t at, long stride, size_t row, int C, float c2) {
+    Online t = {-INFINITY, 0.f};
+    for (int j = 0; j < e.k; ++j) {
+        const int c = e.index[at + (size_t)j * stride];
+        const float v[1] = {(unsigned)c < (unsigned)C ? entry_value(e, at + (size_t)j * stride) : -INFINITY};
+        online_fold(t, v, c2);
+    }
+    if (e.rest) {
+        const float v[1] = {e.rest[row]};
+        online_fold(t, v, c2);
+    }
+    return t;
+}
+
+template <typename T, int BT>
+__global__ __launch_bounds__(BT) void topk_kl_planes_fwd(const T *__restrict__ S, Entries e, float4 *__restrict__ stats, double *__restrict__ part, int C, long P,
+                                                         int blocks_per_image, int nwords, float c2) {
+    extern __shared__ __attribute__((aligned(16))) unsigned char lds[];
+    constexpr int U = 8;
+    const Columns<BT> col(lds, nwords);
+    const long b = blockIdx.x / blocks_per_image;
+    const long p = (long)(blockIdx.x - b * blocks_per_image) * BT + threadIdx.x;
+    const size_t row = (size_t)b * P + p;
+    double kl = 0, counted = 0;
+    if (p < P && (!e.valid || e.valid[row])) {
+        counted = 1;
+        const size_t at = (size_t)b * e.k * P + p;
+        const int members = mark_entries<BT>(col, nwords, e, at, P, C);
+        const T *ps = S + (size_t)b * C * P + p;
+        Online low = {-INFINITY, 0.f};
+        int next = 0;
+        unsigned word = 0;
+        for (int c0 = 0; c0 < C; c0 += U) {
+            float z[U];
+#pragma unroll
+            for (int u = 0; u < U; ++u) z[u] = c0 + u < C ? VecIO<T>::load1(ps + (size_t)(c0 + u) * P) : -INFINITY;
+            if ((c0 & 31) == 0) word = col.words[(c0 >> 5) * BT];
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                if (word & 1) {
+                    col.vals[next * BT] = z[u];
+                    ++next;
+                    z[u] = -INFINITY;
+                }
+                word >>= 1;
+            }
+            online_fold(low, z, c2);
+        }
+        float m = low.m;
+        for (int j = 0; j < members; ++j) m = fmaxf(m, col.vals[j * BT]);
+        const float r = finite_ref(m);
+        const float qr_num = low.s * ex2((low.m - r) * c2);
+        float s = qr_num;
+        for (int j = 0; j < members; ++j) s += ex2((col.vals[j * BT] - r) * c2);
+        const float inv_s = 1.f / s, log_s = logf(s), tau_inv = c2 * kLn2;
+        const Online t = teacher(e, at, P, row, C, c2);
+        const float tr = finite_ref(t.m), inv_t = 1.f / t.s, log_t = logf(t.s);
+        float pr = 0.f, w = 0.f, k = 0.f;
+        if (t.s > 0.f || t.s != t.s) {
+            for (int j = 0; j < e.k; ++j) {
+                const int c = e.index[at + (size_t)j * P];
+                if ((unsigned)c >= (unsigned)C) continue;
+                const float v = entry_value(e, at + (size_t)j * P) - tr, zq = col.vals[col.rank(c) * BT] - r;
+                k += kl_term(ex2(v * c2) * inv_t, v * tau_inv - log_t, zq * tau_inv - log_s);
+            }
+            if (e.rest) {
+                const float v = e.rest[row] - tr;
+                pr = ex2(v * c2) * inv_t;
+                k += kl_term(pr, v * tau_inv - log_t, (low.m - r) * tau_inv + logf(low.s) - log_s);
+            }
+            w = low.s > 0.f || low.s != low.s ? (qr_num * inv_s - pr) / low.s : 0.f;
+            kl = (double)k;
+        }
+        // a row whose teacher says nothing (no live entry, no rest) has no loss and no gradient: 1 / s = 0 and w = 0 say so to the backward
+        stats[row] = t.s > 0.f || t.s != t.s ? make_float4(finite_ref(low.m), w, r, inv_s) : make_float4(0.f, 0.f, r, 0.f);
+    }
+    write_partial<BT>(kl, counted, part);
+}
+
+template <typename T, int BT>
+__global__ __launch_bounds__(BT) void topk_kl_planes_bwd(const T *__restrict__ S, Entries e, const float4 *__restrict__ stats, const float *__restrict__ inv_n,
+                                                         const float *__restrict__ upstream, T *__restrict__ dS, int C, long P, int blocks_per_image, int nwords,
+                                                         float c2, float coef) {
+    extern __shared__ __attribute__((aligned(16))) unsigned char lds[];
+    constexpr int U = 8;
+    const Columns<BT> col(lds, nwords);
+    const long b = blockIdx.x / blocks_per_image;
+    const long p = (long)(blockIdx.x - b * blocks_per_image) * BT + threadIdx.x;
+    const size_t row = (size_t)b * P + p;
+    if (p >= P) return;
+    T *pd = dS + (size_t)b * C * P + p;
+    const float4 st = !e.valid || e.valid[row] ? stats[row] : make_float4(0.f, 0.f, 0.f, 0.f);
+    if (st.y == 0.f && st.w == 0.f) {
+        for (int c = 0; c < C; ++c) VecIO<T>::store1(pd + (size_t)c * P, 0.f);
+        return;
+    }
+    const float g = coef * inv_n[0] * upstream[0];
+    const size_t at = (size_t)b * e.k * P + p;
+    const int members = mark_entries<BT>(col, nwords, e, at, P, C);
+    const Online t = teacher(e, at, P, row, C, c2);
+    const float tr = finite_ref(t.m), inv_t = 1.f / t.s;
+    for (int j = 0; j < members; ++j) col.vals[j * BT] = 0.f;
+    for (int j = 0; j < e.k; ++j) {
+        const int c = e.index[at + (size_t)j * P];
+        if ((unsigned)c < (unsigned)C) col.vals[col.rank(c) * BT] += ex2((entry_value(e, at + (size_t)j * P) - tr) * c2) * inv_t;
+    }
+    const T *ps = S + (size_t)b * C * P + p;
+    const float w = st.y * g, inv_s = st.w;
+    int next = 0;
+    unsigned word = 0;
+    for (int c0 = 0; c0 < C; c0 += U) {
+        float z[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) z[u] = c0 + u < C ? VecIO<T>::load1(ps + (size_t)(c0 + u) * P) : 0.f;
+        if ((c0 & 31) == 0) word = col.words[(c0 >> 5) * BT];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            float d = ex2((z[u] - st.x) * c2) * w;
+            if (word & 1) {
+                d = (ex2((z[u] - st.z) * c2) * inv_s - col.vals[next * BT]) * g;
+                ++next;
+            }
+            word >>= 1;
+            if (c0 + u < C) VecIO<T>::store1(pd + (size_t)(c0 + u) * P, d);
+        }
+    }
+}
+
+// ---- contiguous rows [B, C]: NT threads per row ----------------------------------------------------------------------------------------------------
+// A is a bit mask of the row in LDS, shifted so that an aligned 16-byte vector of logits has its bits in one byte (bf16) or half a byte (fp32).
+// Every wave takes the entries by itself, two per lane: their statistics need no exchange.
+struct RowEntries {
+    int c[2];
+    float v[2];
+    bool first[2];     // no earlier entry names the same class
+    float tr, ts;      // the teacher's finite reference and normaliser
+};
+__device__ __forceinline__ RowEntries load_entries(const Entries &e, size_t row, int C, float c2) {
+    RowEntries x;
+    const int lane = threadIdx.x & 63;
+    Online t = {-INFINITY, 0.f};
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        const int j = lane + 64 * h;
+        x.c[h] = j < e.k ? e.index[row * e.k + j] : -1;
+        if ((unsigned)x.c[h] >= (unsigned)C) x.c[h] = -1;
+        x.v[h] = x.c[h] >= 0 ? entry_value(e, row * e.k + j) : -INFINITY;
+        x.first[h] = x.c[h] >= 0;
+    }
+    online_fold(t, x.v, c2);
+    t = online_group<64>(t, nullptr, 0, c2);
+    if (e.rest) {
+        const float v[1] = {e.rest[row]};
+        online_fold(t, v, c2);
+    }
+    x.tr = finite_ref(t.m);
+    x.ts = t.s;
+    for (int j = 0; j < e.k && j < 64; ++j) {
+        const int c = __builtin_amdgcn_readlane(x.c[0], j);
+        if (c == x.c[0] && j < lane) x.first[0] = false;
+        if (c == x.c[1]) x.first[1] = false;
+    }
+    for (int j = 64; j < e.k; ++j) {
+        const int c = __builtin_amdgcn_readlane(x.c[1], j - 64);
+        if (c == x.c[1] && j - 64 < lane) x.first[1] = false;
+    }
+    return x;
+}
+
+__host__ __device__ inline int row_words(int C) { return (C + 7 + 31) / 32; }      // up to 7 bits of shift in front
+
+template <typename T, int NT>
+__global__ __launch_bounds__(NT == 64 ? 256 : NT) void topk_kl_rows_fwd(const T *__restrict__ S, Entries e, float4 *__restrict__ stats, double *__restrict__ part,
+                                                                        long rows, int C, float c2) {
+    extern __shared__ __attribute__((aligned(16))) unsigned char lds[];
+    constexpr int G = NT == 64 ? 4 : 1, N = VecIO<T>::N;
+    __shared__ Online tmp[NT / 64 + 1];
+    const int nwords = row_words(C);
+    const int grp = NT == 64 ? threadIdx.x >> 6 : 0, tid = NT == 64 ? threadIdx.x & 63 : threadIdx.x;
+    unsigned *bits = reinterpret_cast<unsigned *>(lds) + (size_t)grp * nwords;
+    const float tau_inv = c2 * kLn2;
+    double kl = 0, counted = 0;
+    for (int w = tid; w < nwords; w += NT) bits[w] = 0;
+    for (long row = (long)blockIdx.x * G + grp; row < rows; row += (long)gridDim.x * G) {
+        if (e.valid && !e.valid[row]) continue;                       // the same answer in all threads of the group
+        const T *z = S + (size_t)row * C;
+        const int head = row_head(z, C), shift = (8 - (head & 7)) & 7, nvec = (C - head) / N;
+        const RowEntries x = load_entries(e, row, C, c2);
+        group_sync<NT>();                                              // the mask is clear
+        if (tid < 64) {
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+                if (x.first[h]) atomicOr(&bits[(x.c[h] + shift) >> 5], 1u << ((x.c[h] + shift) & 31));
+        }
+        group_sync<NT>();
+        Online low = {-INFINITY, 0.f};
+        auto outside = [&](int c) { return ((bits[(c + shift) >> 5] >> ((c + shift) & 31)) & 1) == 0; };
+        if (tid < head && outside(tid)) {
+            const float one[1] = {VecIO<T>::load1(z + tid)};
+            online_fold(low, one, c2);
+        }
+        for (int i = tid; i < nvec; i += NT) {
+            float a[N];
+            VecIO<T>::load(z + head + (size_t)i * N, a);
+            const int at = head + shift + i * N;
+            unsigned m = bits[at >> 5] >> (at & 31);
+            if (m & ((1u << N) - 1)) {
+#pragma unroll
+                for (int q = 0; q < N; ++q)
+                    if ((m >> q) & 1) a[q] = -INFINITY;
+            }
+            online_fold(low, a, c2);
+        }
+        const int t = head + nvec * N + tid;
+        if (t < C && outside(t)) {
+            const float one[1] = {VecIO<T>::load1(z + t)};
+            online_fold(low, one, c2);
+        }
+        low = online_group<NT>(low, tmp, tid, c2);
+        if (tid < 64) {
+            float zj[2], m = low.m;
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                zj[h] = x.c[h] >= 0 ? VecIO<T>::load1(z + x.c[h]) : -INFINITY;
+                m = fmaxf(m, zj[h]);
+            }
+            m = wave_max(m);
+            const float r = finite_ref(m), qr_num = low.s * ex2((low.m - r) * c2);
+            float s = 0.f;
+#pragma unroll
+            for (int h = 0; h < 2; ++h) s += x.first[h] ? ex2((zj[h] - r) * c2) : 0.f;
+            s = wave_sum(s) + qr_num;
+            const float inv_s = 1.f / s, log_s = logf(s), inv_t = 1.f / x.ts, log_t = logf(x.ts);
+            float k = 0.f;
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+                if (x.c[h] >= 0) {
+                    const float v = x.v[h] - x.tr;
+                    k += kl_term(ex2(v * c2) * inv_t, v * tau_inv - log_t, (zj[h] - r) * tau_inv - log_s);
+                }
+            k = wave_sum(k);
+            const bool says = x.ts > 0.f || x.ts != x.ts;
+            float pr = 0.f;
+            if (e.rest) {
+                const float v = e.rest[row] - x.tr;
+                pr = ex2(v * c2) * inv_t;
+                k += kl_term(pr, v * tau_inv - log_t, (low.m - r) * tau_inv + logf(low.s) - log_s);
+            }
+            if (tid == 0) {
+                const float w = low.s > 0.f || low.s != low.s ? (qr_num * inv_s - pr) / low.s : 0.f;
+                stats[row] = says ? make_float4(finite_ref(low.m), w, r, inv_s) : make_float4(0.f, 0.f, r, 0.f);
+                kl += says ? (double)k : 0.0;
+                counted += 1;
+            }
+#pragma unroll
+            for (int h = 0; h < 2; ++h)                                // every vector of this row has been read (online_group waits for all)
+                if (x.first[h]) bits[(x.c[h] + shift) >> 5] = 0;
+        }
+    }
+    write_partial<NT == 64 ? 256 : NT>(kl, counted, part);
+}
+
+template <typename T, int NT>
+__global__ __launch_bounds__(NT == 64 ? 256 : NT) void topk_kl_rows_bwd(const T *__restrict__ S, Entries e, const float4 *__restrict__ stats,
+                                                                        const float *__restrict__ inv_n, const float *__restrict__ upstream, T *__restrict__ dS,
+                                                                        long rows, int C, float c2, float coef) {
+    constexpr int G = NT == 64 ? 4 : 1, N = VecIO<T>::N;
+    const int grp = NT == 64 ? threadIdx.x >> 6 : 0, tid = NT == 64 ? threadIdx.x & 63 : threadIdx.x;
+    const long row = (long)blockIdx.x * G + grp;
+    if (row >= rows) return;
+    const T *z = S + (size_t)row * C;
+    T *d = dS + (size_t)row * C;
+    const int head = row_head(z, C), nvec = (C - head) / N;
+    const bool aligned = row_head(d, C) == head;                       // dS starts where S does, modulo 16 bytes
+    const float4 st = !e.valid || e.valid[row] ? stats[row] : make_float4(0.f, 0.f, 0.f, 0.f);
+    const bool none = st.y == 0.f && st.w == 0.f;
+    const float g = none ? 0.f : coef * inv_n[0] * upstream[0], w = st.y * g;
+    auto grad = [&](float x) { return none ? 0.f : ex2((x - st.x) * c2) * w; };
+    if (tid < head) VecIO<T>::store1(d + tid, grad(none ? 0.f : VecIO<T>::load1(z + tid)));
+    for (int i = tid; i < nvec; i += NT) {
+        float a[N];
+        if (!none) VecIO<T>::load(z + head + (size_t)i * N, a);
+#pragma unroll
+        for (int q = 0; q < N; ++q) a[q] = grad(a[q]);
+        if (aligned) {
+            VecIO<T>::template store<false>(d + head + (size_t)i * N, a);
+        } else {
+#pragma unroll
+            for (int q = 0; q < N; ++q) VecIO<T>::store1(d + head + (size_t)i * N + q, a[q]);
+        }
+    }
+    const int t = head + nvec * N + tid;
+    if (t < C) VecIO<T>::store1(d + t, grad(none ? 0.f : VecIO<T>::load1(z + t)));
+    if (none) return;                                                   // the same answer in all threads of the group
+    // the entries' classes took the outside form above; they are written again once that pass is done
+    group_sync<NT>();
+    if (tid < 64) {
+        const RowEntries x = load_entries(e, row, C, c2);
+        const float inv_t = 1.f / x.ts;
+        float p[2], sum[2] = {0.f, 0.f};
+#pragma unroll
+        for (int h = 0; h < 2; ++h) p[h] = x.c[h] >= 0 ? ex2((x.v[h] - x.tr) * c2) * inv_t : 0.f;
+        for (int j = 0; j < e.k; ++j) {
+            const int c = j < 64 ? __builtin_amdgcn_readlane(x.c[0], j) : __builtin_amdgcn_readlane(x.c[1], j - 64);
+            const float pj = __int_as_float(j < 64 ? __builtin_amdgcn_readlane(__float_as_int(p[0]), j) : __builtin_amdgcn_readlane(__float_as_int(p[1]), j - 64));
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+                if (c == x.c[h]) sum[h] += pj;
+        }
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+            if (x.first[h]) VecIO<T>::store1(d + x.c[h], (ex2((VecIO<T>::load1(z + x.c[h]) - st.z) * c2) * st.w - sum[h]) * g);
+    }
+}
+
+// ---- launches ---------------------------------------------------------------------------------------------------------------------------------
+struct Plan {
+    int threads, blocks, nwords, lds;      // threads per row (P == 1) or per workgroup (planes)
+    long per;                              // workgroups per image (planes)
+};
+// false: not a shape these kernels launch
+bool plan(long B, int C, long P, int k, Plan *pl) {
+    if (P == 1) {
+        pl->nwords = row_words(C);
+        pl->threads = C <= 2048 ? 64 : 256;
+        const long wgs = pl->threads == 64 ? (B + 3) / 4 : B;
+        if (wgs > kMaxBlocks) return false;
+        pl->blocks = (int)(wgs < 4096 ? wgs : 4096);
+        pl->lds = pl->nwords * 4 * (pl->threads == 64 ? 4 : 1);
+        pl->per = wgs;
+        return true;
+    }
+    pl->nwords = (C + 31) / 32;
+    const long column = 4L * (2 * pl->nwords + k);                      // bytes of LDS per pixel
+    pl->threads = column * 256 <= 32768 ? 256 : 64;
+    if (column * 64 > 64512) return false;                              // 64 KB less what the kernels hold besides
+    pl->lds = (int)column * pl->threads;
+    pl->per = (P + pl->threads - 1) / pl->threads;
+    if (pl->per > kMaxBlocks / B) return false;
+    pl->blocks = (int)(pl->per * B);
+    return true;
+}
+
+template <typename T>
+int fwd_launch(const void *S, const Entries &e, long B, int C, long P, const Plan &pl, float c2, float alpha, float4 *stats, float *inv_n, float *loss, double *part,
+               hipStream_t st) {
+    const T *s = static_cast<const T *>(S);
+    const dim3 grid((unsigned)pl.blocks);
+    if (P == 1) {
+        if (pl.threads == 64) hipLaunchKernelGGL((topk_kl_rows_fwd<T, 64>), grid, dim3(256), pl.lds, st, s, e, stats, part, B, C, c2);
+        else hipLaunchKernelGGL((topk_kl_rows_fwd<T, 256>), grid, dim3(256), pl.lds, st, s, e, stats, part, B, C, c2);
+    } else {
+        if (pl.threads == 64) hipLaunchKernelGGL((topk_kl_planes_fwd<T, 64>), grid, dim3(64), pl.lds, st, s, e, stats, part, C, P, (int)pl.per, pl.nwords, c2);
+        else hipLaunchKernelGGL((topk_kl_planes_fwd<T, 256>), grid, dim3(256), pl.lds, st, s, e, stats, part, C, P, (int)pl.per, pl.nwords, c2);
+    }
+    hipLaunchKernelGGL(topk_kl_finish, dim3(1), dim3(256), 0, st, part, pl.blocks, alpha, loss, inv_n);
+    return (int)hipGetLastError();
+}
+
+template <typename T>
+int bwd_launch(const void *S, const Entries &e, long B, int C, long P, const Plan &pl, float c2, float coef, const float4 *stats, const float *inv_n,
+               const float *upstream, void *dS, hipStream_t st) {
+    const T *s = static_cast<const T *>(S);
+    T *d = static_cast<T *>(dS);
+    if (P == 1) {
+        const dim3 grid((unsigned)pl.per);
+        if (pl.threads == 64) hipLaunchKernelGGL((topk_kl_rows_bwd<T, 64>), grid, dim3(256), 0, st, s, e, stats, inv_n, upstream, d, B, C, c2, coef);
+        else hipLaunchKernelGGL((topk_kl_rows_bwd<T, 256>), grid, dim3(256), 0, st, s, e, stats, inv_n, upstream, d, B, C, c2, coef);
+    } else {
+        const dim3 grid((unsigned)pl.blocks);
+        if (pl.threads == 64)
+            hipLaunchKernelGGL((topk_kl_planes_bwd<T, 64>), grid, dim3(64), pl.lds, st, s, e, stats, inv_n, upstream, d, C, P, (int)pl.per, pl.nwords, c2, coef);
+        else
+            hipLaunchKernelGGL((topk_kl_planes_bwd<T, 256>), grid, dim3(256), pl.lds, st, s, e, stats, inv_n, upstream, d, C, P, (int)pl.per, pl.nwords, c2, coef);
+    }
+    return (int)hipGetLastError();
+}
+
+int check_args(const void *S, const void *values, const int32_t *index, const float *rest, int dtype, int values_dtype, long B, int C, long P, int k, float tau,
+               Plan *pl) {
+    if (!S || !values || !index) return SD_E_NULL;
+    if ((dtype != SD_F32 && dtype != SD_BF16) || (values_dtype != SD_F32 && values_dtype != SD_BF16)) return SD_E_DTYPE;
+    if (B <= 0 || C <= 0 || P <= 0 || k <= 0 || B > 0x7fffffffL || P > 0x7fffffffL || !(tau > 0.f) || !isfinite(tau)) return SD_E_SHAPE;
+    if (k > kTopkMax || C > kTopkMaxClasses || !plan(B, C, P, k, pl)) return SD_E_UNSUPPORTED;
+    const uintptr_t es = dtype == SD_F32 ? 3 : 1, ev = values_dtype == SD_F32 ? 3 : 1;
+    if ((reinterpret_cast<uintptr_t>(S) & es) || (reinterpret_cast<uintptr_t>(values) & ev) ||
+        ((reinterpret_cast<uintptr_t>(index) | reinterpret_cast<uintptr_t>(rest)) & 3))
+        return SD_E_ALIGN;
+    return SD_OK;
+}
+
+}  // namespace
+}  // namespace sd
+
+extern "C" {
+
+int sd_topk_kl_supported(long B, int C, long P, int k) {
+    sd::Plan pl;
+    return B > 0 && C > 0 && P > 0 && k > 0 && B <= 0x7fffffffL && P <= 0x7fffffffL && k <= sd::kTopkMax && C <= sd::kTopkMaxClasses && sd::plan(B, C, P, k, &pl);
+}
+
+size_t sd_topk_kl_workspace_bytes(long B, int C, long P, int k) {
+    sd::Plan pl;
+    return sd_topk_kl_supported(B, C, P, k) && sd::plan(B, C, P, k, &pl) ? 2 * sizeof(double) * (size_t)pl.blocks : 0;
+}
+
+int sd_topk_kl_fwd(const void *S, const void *values, const int32_t *index, const float *rest, const uint8_t *valid, int dtype, int values_dtype, long B, int C,
+                   long P, int k, float tau, float alpha, float *stats, float *inv_rows, float *loss, void *workspace, size_t workspace_bytes, void *stream) {
+    sd::Plan pl;
+    const int rc = sd::check_args(S, values, index, rest, dtype, values_dtype, B, C, P, k, tau, &pl);
+    if (rc != SD_OK) return rc;
+    if (!stats || !inv_rows || !loss || !workspace) return SD_E_NULL;
+    if (workspace_bytes < 2 * sizeof(double) * (size_t)pl.blocks || (reinterpret_cast<uintptr_t>(workspace) & 7)) return SD_E_WORKSPACE;
+    if (reinterpret_cast<uintptr_t>(stats) & 15) return SD_E_ALIGN;
+    const sd::Entries e = {values, index, rest, valid, values_dtype == SD_BF16, k};
+    hipStream_t st = static_cast<hipStream_t>(stream);
+    float4 *sv = reinterpret_cast<float4 *>(stats);
+    const float c2 = sd::kLog2e / tau;
+    return dtype == SD_F32 ? sd::fwd_launch<float>(S, e, B, C, P, pl, c2, alpha, sv, inv_rows, loss, static_cast<double *>(workspace), st)
+                           : sd::fwd_launch<sd::bf16_t>(S, e, B, C, P, pl, c2, alpha, sv, inv_rows, loss, static_cast<double *>(workspace), st);
+}
+
+int sd_topk_kl_bwd(const void *S, const void *values, const int32_t *index, const float *rest, const uint8_t *valid, int dtype, int values_dtype, long B, int C,
+                   long P, int k, float tau, float alpha, const float *stats, const float *inv_rows, const float *upstream, void *dS, void *stream) {
+    sd::Plan pl;
+    const int rc = sd::check_args(S, values, index, rest, dtype, values_dtype, B, C, P, k, tau, &pl);
+    if (rc != SD_OK) return rc;
+    if (!stats || !inv_rows || !upstream || !dS) return SD_E_NULL;
+    if ((reinterpret_cast<uintptr_t>(stats) & 15) || (reinterpret_cast<uintptr_t>(dS) & (dtype == SD_F32 ? 3 : 1))) return SD_E_ALIGN;
+    const sd::Entries e = {values, index, rest, valid, values_dtype == SD_BF16, k};
+    hipStream_t st = static_cast<hipStream_t>(stream);
+    const float4 *sv = reinterpret_cast<const float4 *>(stats);
+    const float c2 = sd::kLog2e / tau, coef = alpha / tau;
+    return dtype == SD_F32 ? sd::bwd_launch<float>(S, e, B, C, P, pl, c2, coef, sv, inv_rows, upstream, dS, st)
+                           : sd::bwd_launch<sd::bf16_t>(S, e, B, C, P, pl, c2, coef, sv, inv_rows, upstream, dS, st);
+}
+
+}  // extern "C"

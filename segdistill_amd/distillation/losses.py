@@ -10,7 +10,7 @@ iteration :38) are taken here; everything per-pixel runs on the GPU:
 * 'channel' rows (CD / CGD): ``ops.cgd_kl`` -- grouped-channel online softmax + KL, the -1e9 pad
   of :55-58 is virtual, the channel shuffle of :39-41 is a permutation table read by the
   kernel (no gather copies);
-* 'pixel' rows (PD): ``ops.pix_kl``.
+* 'pixel' rows (PD): ``ops.pix_kl``; the same from the teacher's k best classes alone (TopKLoss): ``ops.topk_logits`` / ``ops.topk_kl``.
 
 On a CPU tensor the ops raise; the one exception is the explicit plumbing mode below, which is never a fallback.
 """
@@ -310,6 +310,38 @@ class CGDLossWS(KLDLoss):
                          transform_config={'loss_type': 'channel', 'group_size': 10},
                          warmup_config={'mode': 'linear', 'warmup_iters': 2000},
                          earlydecay_config={'mode': 'linear', 'earlydecay_start': 110000, 'earlydecay_end': 120000})
+
+
+@DISTILL_LOSSES.register_module()
+class TopKLoss(KLDLoss):
+    """Pixel-wise distillation from the teacher's k best classes: PDLoss (reference :115-128) with every class the teacher does not list folded into one
+    (``rest=True``), or with the k classes renormalised.  The teacher tap is reduced to k logits and one for the rest per pixel (``ops.topk_logits``, what a
+    stored teacher holds) and the student meets those (``ops.topk_kl``).  At the student tap's resolution: a teacher tap of another size is resized first;
+    ``resize_config`` resizes both as KLDLoss does.  ``ignore_index``: pixels with that label (nearest label of the tap's grid) take no part, and the mean is
+    over the others.  Schedules as KLDLoss."""
+
+    def __init__(self, k=10, alpha=1, tau=1, rest=True, ignore_index=None, resize_config=None, warmup_config=None, earlydecay_config=None):
+        super().__init__(alpha=alpha, tau=tau, resize_config=resize_config, warmup_config=warmup_config, earlydecay_config=earlydecay_config)
+        self.k, self.rest, self.ignore_index = k, rest, ignore_index
+
+    def fused_up_size(self, x_student, x_teacher, gt):
+        return None
+
+    def forward(self, x_student, x_teacher, gt, n_iter):
+        alpha, alpha_t, _ = self._prepare(x_student, x_student.shape[1], n_iter)
+        if self.resize_config:
+            size = tuple(int(v) for v in (x_teacher if self.resize_config.get('target', 'gt') == 'teacher' else gt).shape[2:])
+            from ..layers import resize
+            x_student, x_teacher = (resize(x, size=size, mode=self.resize_config['mode'], align_corners=self.resize_config['align_corners'], warning=False,
+                                           alias_ok=True) for x in (x_student, x_teacher))
+        elif x_teacher.shape[2:] != x_student.shape[2:]:
+            x_teacher = _bilinear(x_teacher, x_student.shape[2:])
+        valid = None
+        if self.ignore_index is not None:
+            valid = F.interpolate(gt.float(), size=x_student.shape[2:], mode='nearest')[:, 0] != self.ignore_index
+        values, index, rest = ops.topk_logits(x_teacher.detach(), min(self.k, x_teacher.shape[1]), tau=self.tau)
+        loss = ops.topk_kl(x_student, values, index, rest if self.rest else None, tau=self.tau, alpha=alpha, valid=valid)
+        return loss if alpha_t is None else loss * alpha_t
 
 
 @DISTILL_LOSSES.register_module()

@@ -1,10 +1,13 @@
 """torch.autograd bindings over the C ABI (device pointers + the current HIP stream)."""
 from __future__ import annotations
 
+import contextlib
 import ctypes as C
+import math
 import os
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from . import _lib
 
@@ -23,6 +26,11 @@ def _require_gpu(*tensors):
 
 def _ptr(t):
     return None if t is None else t.data_ptr()
+
+
+def _launch_on(device):
+    """Launches inside go to `device`, whichever device is current outside."""
+    return contextlib.nullcontext() if device.index == torch.cuda.current_device() else torch.cuda.device(device)
 
 
 class _CGDKLFunction(torch.autograd.Function):
@@ -641,6 +649,128 @@ class _IFVDFunction(torch.autograd.Function):
 def ifvd_term(S, T, cls, n_cls):
     """cls: integer class per pixel [B,H,W] (or [B,1,H,W]); values outside [0, n_cls) mean "no class"."""
     return _IFVDFunction.apply(S, T, cls, n_cls)
+
+
+# ---- distillation from a teacher's top logits (csrc/topk_select.hip, csrc/topk_kl.hip) -----------------------------------------------
+def _class_layout(x, what):
+    """(B, C, P) of a logit tensor: class planes [B, C, H, W], or rows [R, C] / [B, N, C] with the classes last (P = 1)."""
+    if x.dim() == 4:
+        return x.shape[0], x.shape[1], x.shape[2] * x.shape[3]
+    if x.dim() in (2, 3):
+        return math.prod(x.shape[:-1]), x.shape[-1], 1
+    raise ValueError(f'{what}: expected [B, C, H, W] or classes last ([R, C], [B, N, C]), got {tuple(x.shape)}')
+
+
+def _row_shape(x):
+    return (x.shape[0],) + tuple(x.shape[2:]) if x.dim() == 4 else tuple(x.shape[:-1])
+
+
+def _entry_shape(x, k):
+    return (x.shape[0], k) + tuple(x.shape[2:]) if x.dim() == 4 else tuple(x.shape[:-1]) + (k,)
+
+
+def _check_tau(tau):
+    tau = float(tau)
+    if not (tau > 0 and math.isfinite(tau)):
+        raise ValueError(f'tau must be a positive number, got {tau}')
+    return tau
+
+
+@torch.no_grad()
+def topk_logits(x, k, *, tau=1.0):
+    """The k largest logits of every row -> (values, index, rest): what a teacher says, without the classes it does not believe in.
+
+    x: class planes [B, C, H, W] (-> values, index [B, k, H, W], rest [B, H, W]) or rows with the classes last ([R, C], [B, N, C] -> [..., k],
+    [...]); fp32 or bf16.  values descend (equal ones by ascending class; NaN counts as the largest), index is int32, rest is fp32 and stands for
+    all other classes at this temperature: tau * log(sum of exp(x / tau) over them), -inf for k = C.  No gradient."""
+    _require_gpu(x)
+    B, Cc, P = _class_layout(x, 'topk_logits')
+    if x.dtype not in _DT:
+        raise TypeError(f'topk_logits: unsupported dtype {x.dtype}')
+    tau, k = _check_tau(tau), int(k)
+    L = _lib.lib()
+    if not 1 <= k <= min(Cc, L.sd_topk_max_entries()):
+        raise ValueError(f'topk_logits: k = {k} is not within 1 .. {min(Cc, L.sd_topk_max_entries())} ({Cc} classes)')
+    x = x.contiguous()
+    values = torch.empty(_entry_shape(x, k), dtype=x.dtype, device=x.device)
+    index = torch.empty(_entry_shape(x, k), dtype=torch.int32, device=x.device)
+    rest = torch.empty(_row_shape(x), dtype=torch.float32, device=x.device)
+    if x.numel():
+        with _launch_on(x.device):
+            _lib.check(L.sd_topk_select(x.data_ptr(), values.data_ptr(), index.data_ptr(), rest.data_ptr(), _DT[x.dtype], B, Cc, P, k, tau, _stream_ptr()),
+                       'sd_topk_select')
+    return values, index, rest
+
+
+class _TopKKLFunction(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, S, values, index, rest, valid, tau, alpha, B, Cc, P, k):
+        L = _lib.lib()
+        rows = B * P
+        ws_bytes = L.sd_topk_kl_workspace_bytes(B, Cc, P, k)
+        ws = torch.empty(ws_bytes, dtype=torch.uint8, device=S.device)
+        stats = torch.empty(rows, 4, dtype=torch.float32, device=S.device)
+        inv_rows = torch.empty((), dtype=torch.float32, device=S.device)
+        loss = torch.empty((), dtype=torch.float32, device=S.device)
+        with _launch_on(S.device):
+            rc = L.sd_topk_kl_fwd(S.data_ptr(), values.data_ptr(), index.data_ptr(), _ptr(rest), _ptr(valid), _DT[S.dtype], _DT[values.dtype], B, Cc, P, k,
+                                  tau, alpha, stats.data_ptr(), inv_rows.data_ptr(), loss.data_ptr(), ws.data_ptr(), ws_bytes, _stream_ptr())
+        _lib.check(rc, 'sd_topk_kl_fwd')
+        ctx.save_for_backward(S, values, index, rest, valid, stats, inv_rows)
+        ctx.meta = (tau, alpha, B, Cc, P, k)
+        return loss
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad_loss):
+        S, values, index, rest, valid, stats, inv_rows = ctx.saved_tensors
+        tau, alpha, B, Cc, P, k = ctx.meta
+        dS = torch.empty_like(S)
+        up = grad_loss.to(torch.float32).contiguous()
+        with _launch_on(S.device):
+            rc = _lib.lib().sd_topk_kl_bwd(S.data_ptr(), values.data_ptr(), index.data_ptr(), _ptr(rest), _ptr(valid), _DT[S.dtype], _DT[values.dtype], B, Cc,
+                                           P, k, tau, alpha, stats.data_ptr(), inv_rows.data_ptr(), up.data_ptr(), dS.data_ptr(), _stream_ptr())
+        _lib.check(rc, 'sd_topk_kl_bwd')
+        return (dS,) + (None,) * 10
+
+
+def topk_kl(S, values, index, rest=None, *, tau, alpha, valid=None):
+    """alpha * mean over rows of KL(teacher || softmax(S / tau)) from the teacher's top logits (topk_logits' values, index, rest; or a stored copy).
+
+    With `rest` (taken at the same tau) the teacher is softmax([values, rest] / tau) and the classes outside `index` meet it as one; without, it is
+    softmax(values / tau): the k classes renormalised.  S: [B, C, H, W] or classes last, fp32 or bf16; values fp32 or bf16; index int32 (int64 is
+    converted); an index outside [0, C) is no entry, a row without any has no loss.  `valid` (bool, one per row): rows to take part; the mean is over
+    them, the others are not read and get a zero gradient.  Gradient for S only."""
+    _require_gpu(S, values, index)
+    B, Cc, P = _class_layout(S, 'topk_kl')
+    if S.dtype not in _DT or values.dtype not in _DT:
+        raise TypeError(f'topk_kl: unsupported dtypes {S.dtype} / {values.dtype}')
+    if index.dtype not in (torch.int32, torch.int64):
+        raise TypeError(f'topk_kl: index must be int32 or int64, got {index.dtype}')
+    tau, alpha = _check_tau(tau), float(alpha)
+    if values.dim() != S.dim() or index.shape != values.shape:
+        raise ValueError(f'topk_kl: values {tuple(values.shape)} and index {tuple(index.shape)} do not fit logits {tuple(S.shape)}')
+    k = values.shape[1] if S.dim() == 4 else values.shape[-1]
+    if tuple(values.shape) != _entry_shape(S, k):
+        raise ValueError(f'topk_kl: values {tuple(values.shape)} do not fit logits {tuple(S.shape)}')
+    for name, t in (('rest', rest), ('valid', valid)):
+        if t is not None and tuple(t.shape) != _row_shape(S):
+            raise ValueError(f'topk_kl: {name} {tuple(t.shape)} must have one value per row {_row_shape(S)}')
+    if rest is not None and rest.dtype != torch.float32:
+        raise TypeError(f'topk_kl: rest must be float32, got {rest.dtype}')
+    if valid is not None and valid.dtype not in (torch.bool, torch.uint8):
+        raise TypeError(f'topk_kl: valid must be bool or uint8, got {valid.dtype}')
+    if any(t is not None and t.device != S.device for t in (values, index, rest, valid)):
+        raise ValueError('topk_kl: operands on different devices')
+    if S.numel() == 0:
+        return S.float().sum() * 0.0
+    if not _lib.lib().sd_topk_kl_supported(B, Cc, P, k):
+        raise ValueError(f'topk_kl: {k} entries of {Cc} classes are not supported (at most {_lib.lib().sd_topk_max_entries()} entries; class planes hold a '
+                         'bit per class and pixel in LDS)')
+    if index.dtype == torch.int64:
+        index = index.clamp(-1, 2 ** 31 - 1).to(torch.int32)
+    return _TopKKLFunction.apply(S.contiguous(), values.detach().contiguous(), index.contiguous(), None if rest is None else rest.detach().contiguous(),
+                                 None if valid is None else valid.contiguous().view(torch.uint8), tau, alpha, B, Cc, P, k)
 
 
 def align1x1(x, weight, bias=None):

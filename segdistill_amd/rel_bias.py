@@ -1,0 +1,85 @@
+"""A learned position bias by buckets and its gradient (csrc/rel_bias.hip; reference mmseg/models/backbones/swin_transformer.py:133-135, where the buckets
+are the (dy, dx) offsets of a window's tokens).  Autograd of `table[index]` scatters with atomics, in an order of its own each time; here the pairs are
+ordered by bucket once (`BucketPlan`) and the gradient is a sum over each bucket's pairs in that order."""
+from __future__ import annotations
+
+import torch
+import torch.nn as nn
+from torch.autograd.function import once_differentiable
+
+from . import _lib
+from .ops import _DT, _launch_on, _require_gpu, _stream_ptr
+
+
+class BucketPlan(nn.Module):
+    """The (query, key) pairs of `index` [Nq, Nk] (integers in [0, num_buckets)) in the order the gradient sums them.  Built once per index: it reads the
+    index on the host.  A module without parameters or state-dict entries, so that a model that holds one moves it along."""
+
+    def __init__(self, index, num_buckets):
+        super().__init__()
+        if index.dim() != 2 or index.is_floating_point() or index.is_complex() or index.dtype == torch.bool or index.numel() == 0:
+            raise ValueError(f'BucketPlan: index must be a non-empty integer [Nq, Nk], got {index.dtype} {tuple(index.shape)}')
+        nb = int(num_buckets)
+        if index.numel() > 2 ** 31 - 1:
+            raise ValueError('BucketPlan: more than 2^31 - 1 pairs')
+        flat = index.detach().reshape(-1).long()
+        lo, hi = torch.stack(torch.aminmax(flat)).tolist()
+        if lo < 0 or hi >= nb:
+            raise ValueError(f'BucketPlan: index holds {lo} .. {hi}, outside [0, {nb})')
+        chunk = _lib.lib().sd_bucket_bias_chunk()
+        order = torch.sort(flat, stable=True).indices
+        count = torch.bincount(flat, minlength=nb)
+        chunks = ((count + chunk - 1) // chunk).clamp(min=1)               # an empty bucket: one empty chunk
+        first = torch.cumsum(chunks, 0)
+        bucket_chunk = torch.cat([first.new_zeros(1), first])
+        owner = torch.repeat_interleave(torch.arange(nb, device=flat.device), chunks)
+        within = torch.arange(owner.numel(), device=flat.device) - bucket_chunk[owner]
+        start = (torch.cumsum(count, 0) - count)[owner] + within * chunk
+        self.num_buckets, self.shape = nb, tuple(index.shape)
+        self.register_buffer('index', flat.int().view(index.shape), persistent=False)
+        self.register_buffer('order', order.int(), persistent=False)
+        self.register_buffer('chunk_start', torch.cat([start, start.new_tensor([flat.numel()])]).int(), persistent=False)
+        self.register_buffer('bucket_chunk', bucket_chunk.int(), persistent=False)
+
+    def extra_repr(self):
+        return f'{self.shape[0]} x {self.shape[1]} pairs in {self.num_buckets} buckets'
+
+
+class _BucketBiasFunction(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, table, plan):
+        nb, heads = table.shape
+        out = torch.empty((heads,) + plan.shape, dtype=table.dtype, device=table.device)
+        with _launch_on(table.device):
+            rc = _lib.lib().sd_bucket_bias_fwd(table.data_ptr(), plan.index.data_ptr(), out.data_ptr(), _DT[table.dtype], nb, heads, plan.index.numel(), _stream_ptr())
+        _lib.check(rc, 'sd_bucket_bias_fwd')
+        ctx.plan = plan
+        return out
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad_out):
+        plan = ctx.plan
+        d = grad_out.contiguous()
+        heads, nb, chunks = d.shape[0], plan.num_buckets, plan.chunk_start.numel() - 1
+        L = _lib.lib()
+        dtable = torch.empty(nb, heads, dtype=d.dtype, device=d.device)
+        ws_bytes = L.sd_bucket_bias_workspace_bytes(nb, chunks, heads)
+        ws = torch.empty(ws_bytes, dtype=torch.uint8, device=d.device) if ws_bytes else None
+        with _launch_on(d.device):
+            rc = L.sd_bucket_bias_bwd(d.data_ptr(), plan.order.data_ptr(), plan.chunk_start.data_ptr(), plan.bucket_chunk.data_ptr(), dtable.data_ptr(),
+                                      _DT[d.dtype], nb, chunks, heads, plan.index.numel(), None if ws is None else ws.data_ptr(), ws_bytes, _stream_ptr())
+        _lib.check(rc, 'sd_bucket_bias_bwd')
+        return dtable, None
+
+
+def bucket_bias(table, plan):
+    """table [num_buckets, heads] (fp32 or bf16) -> bias [heads, Nq, Nk] = table[index].permute(2, 0, 1), with a deterministic gradient for the table."""
+    _require_gpu(table)
+    if table.dtype not in _DT:
+        raise TypeError(f'bucket_bias: unsupported dtype {table.dtype}')
+    if table.dim() != 2 or table.shape[0] != plan.num_buckets or table.shape[1] == 0:
+        raise ValueError(f'bucket_bias: table {tuple(table.shape)} does not fit a plan of {plan.num_buckets} buckets')
+    if plan.index.device != table.device:
+        raise ValueError(f'bucket_bias: the plan is on {plan.index.device}, the table on {table.device}')
+    return _BucketBiasFunction.apply(table.contiguous(), plan)

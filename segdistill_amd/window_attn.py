@@ -1,4 +1,4 @@
-"""Window attention of a Swin block without an autograd graph (the frozen teacher of BASELINE config 4) as ONE kernel over the qkv Linear's
+"""Window attention of a Swin block.  `attention`: with its gradients (csrc/window_train.hip; a Swin student).  The rest: without an autograd graph (the frozen teacher of BASELINE config 4) as ONE kernel over the qkv Linear's
 output (csrc/window_attn.hip; reference mmseg/models/backbones/swin_transformer.py:119-153): relative position bias and shift mask are read
 from small packed tables inside the kernel, q / k / v are not permuted and the output comes out token-major for the projection."""
 from __future__ import annotations
@@ -6,9 +6,10 @@ from __future__ import annotations
 import os
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from . import _lib
-from .ops import _DT, _stream_ptr
+from .ops import _DT, _launch_on, _ptr, _require_gpu, _stream_ptr
 
 ENABLED = os.environ.get('SEGDISTILL_WINDOW_ATTN', '1') == '1'       # A/B: 0 = F.scaled_dot_product_attention with a materialised additive tensor
 
@@ -20,15 +21,15 @@ def supported(qkv, n, heads, head_dim):
 
 
 def pack_tables(tables, pad_key=0.0, want_flags=False):
-    """[n, 49, 49] additive tables in the reference's orientation ([query, key]) -> ([n, 4096] in the MFMA kernel's accumulator layout,
+    """[n, N, N] additive tables, N <= 64, in the reference's orientation ([query, key]) -> ([n, 4096] in the MFMA kernel's accumulator layout,
     int32 flags [n] = table has a nonzero entry, or None)."""
     t = tables.detach().float().contiguous()
     n = t.shape[0]
-    assert t.shape[1:] == (49, 49)
+    assert t.dim() == 3 and t.shape[1] == t.shape[2] <= 64
     L = _lib.lib()
     packed = torch.empty(n, int(L.sd_window_attn_packed_floats()), dtype=torch.float32, device=t.device)
     flags = torch.empty(n, dtype=torch.int32, device=t.device) if want_flags else None
-    _lib.check(L.sd_window_attn_pack(t.data_ptr(), packed.data_ptr(), None if flags is None else flags.data_ptr(), n, 49, float(pad_key), _stream_ptr()),
+    _lib.check(L.sd_window_attn_pack(t.data_ptr(), packed.data_ptr(), None if flags is None else flags.data_ptr(), n, t.shape[1], float(pad_key), _stream_ptr()),
                'sd_window_attn_pack')
     return packed, flags
 
@@ -45,3 +46,78 @@ def forward_packed(qkv, bias_p, mask_p, mask_flags, heads, scale):
                                               0 if mask_p is None else mask_p.shape[0], heads, n, c // heads, float(scale), _stream_ptr())
     _lib.check(rc, 'sd_window_attn_fwd_packed')
     return out
+
+
+def train_supported(qkv, n, head_dim):
+    """The training kernels take this qkv Linear output [windows, N, 3*heads*head_dim]: fp32 or bf16, windows of up to 64 tokens, head_dim 32."""
+    return bool(ENABLED and qkv.is_cuda and qkv.dtype in _DT and qkv.dim() == 3 and _lib.lib().sd_window_attn_train_supported(int(n), int(head_dim)))
+
+
+class _WindowAttentionFunction(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, qkv, bias, mask, heads, scale):
+        bw, n, c3 = qkv.shape
+        c = c3 // 3
+        out = torch.empty(bw, n, c, dtype=qkv.dtype, device=qkv.device)
+        with _launch_on(qkv.device):
+            bias_p = pack_tables(bias, float('-inf'))[0]
+            mask_p, flags = pack_tables(mask, 0.0, True) if mask is not None else (None, None)
+            rc = _lib.lib().sd_window_attn_train_fwd(qkv.data_ptr(), bias_p.data_ptr(), _ptr(mask_p), _ptr(flags), out.data_ptr(), _DT[qkv.dtype], bw,
+                                                     0 if mask is None else mask.shape[0], heads, n, c // heads, scale, _stream_ptr())
+        _lib.check(rc, 'sd_window_attn_train_fwd')
+        ctx.save_for_backward(qkv, bias_p, mask_p, flags)
+        ctx.meta = (heads, scale, bias.dtype)
+        return out
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad_out):
+        qkv, bias_p, mask_p, flags = ctx.saved_tensors
+        heads, scale, bias_dtype = ctx.meta
+        bw, n, c3 = qkv.shape
+        L = _lib.lib()
+        go = grad_out.to(qkv.dtype).contiguous()
+        if go.data_ptr() % 16:
+            go = go.clone()
+        dqkv = torch.empty_like(qkv)
+        dbias = torch.empty(heads, n, n, dtype=torch.float32, device=qkv.device)
+        ws_bytes = L.sd_window_attn_train_workspace_bytes(bw, heads, n)
+        ws = torch.empty(ws_bytes, dtype=torch.uint8, device=qkv.device)
+        with _launch_on(qkv.device):
+            rc = L.sd_window_attn_train_bwd(qkv.data_ptr(), bias_p.data_ptr(), _ptr(mask_p), _ptr(flags), go.data_ptr(), dqkv.data_ptr(), dbias.data_ptr(),
+                                            _DT[qkv.dtype], bw, 0 if mask_p is None else mask_p.shape[0], heads, n, c3 // 3 // heads, scale, ws.data_ptr(),
+                                            ws_bytes, _stream_ptr())
+        _lib.check(rc, 'sd_window_attn_train_bwd')
+        return dqkv, dbias.to(bias_dtype), None, None, None
+
+
+def attention(qkv, bias, mask, heads, scale):
+    """softmax(scale * q k^T + bias[head] + mask[window % nW]) v for every window and head, with gradients for qkv and bias.
+
+    qkv [windows, N, 3*heads*32] (fp32 or bf16) as the qkv Linear leaves it, N <= 64; bias [heads, N, N]; mask [nW, N, N] additive, without a gradient
+    (windows of one image are contiguous and nW divides their number), or None -> [windows, N, heads*32].  A query row that bias + mask leave at -inf
+    everywhere has output 0 and no gradient."""
+    _require_gpu(qkv, bias)
+    heads = int(heads)
+    if qkv.dim() != 3 or heads <= 0 or qkv.shape[2] % (3 * heads):
+        raise ValueError(f'attention: qkv must be [windows, N, 3 * heads * head_dim], got {tuple(qkv.shape)} for {heads} heads')
+    bw, n, c3 = qkv.shape
+    if qkv.dtype not in _DT:
+        raise TypeError(f'attention: unsupported dtype {qkv.dtype}')
+    if not _lib.lib().sd_window_attn_train_supported(n, c3 // 3 // heads):
+        raise ValueError(f'attention: windows of {n} tokens with head_dim {c3 // 3 // heads} are not supported (1 .. 64 tokens, head_dim 32)')
+    if tuple(bias.shape) != (heads, n, n) or not bias.is_floating_point():
+        raise ValueError(f'attention: bias must be a floating [{heads}, {n}, {n}], got {bias.dtype} {tuple(bias.shape)}')
+    if mask is not None:
+        if mask.dim() != 3 or tuple(mask.shape[1:]) != (n, n) or mask.shape[0] == 0 or bw % mask.shape[0] or not mask.is_floating_point():
+            raise ValueError(f'attention: mask must be a floating [nW, {n}, {n}] with nW dividing {bw}, got {mask.dtype} {tuple(mask.shape)}')
+        if mask.requires_grad:
+            raise ValueError('attention: the mask has no gradient')
+    if any(t is not None and t.device != qkv.device for t in (bias, mask)):
+        raise ValueError('attention: operands on different devices')
+    if bw == 0:
+        return qkv[..., :c3 // 3] * bias.sum().to(qkv.dtype)           # empty, and so are its gradients
+    qkv = qkv.contiguous()
+    if qkv.data_ptr() % 16:
+        qkv = qkv.clone()
+    return _WindowAttentionFunction.apply(qkv, bias, mask, heads, float(scale))
