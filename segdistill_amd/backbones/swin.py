@@ -1,4 +1,4 @@
-"""Swin Transformer encoder (frozen teacher of BASELINE config 4) on PyTorch-ROCm.
+"""Swin Transformer encoder (frozen teacher of BASELINE config 4, or a student) on PyTorch-ROCm.
 
 Behavioural counterpart of reference mmseg/models/backbones/swin_transformer.py
 (WindowAttention :72-151, SwinTransformerBlock :154-260, PatchMerging :263-292, BasicLayer
@@ -9,8 +9,10 @@ relative_position_index, qkv, proj}, norm2, mlp.{fc1,fc2}}``, ``layers.i.downsam
 ``norm{i}``.
 
 MI355X notes: the shifted-window mask is built once per (padded size, device) and cached
-instead of being rebuilt by a Python double loop on every forward of every stage; the window
-attention adds (relative-position bias + mask) as one additive term of SDPA.
+instead of being rebuilt by a Python double loop on every forward of every stage.  The window
+attention of a frozen block and that of a trainable one are kernels over the qkv Linear's output
+(csrc/window_attn.hip, csrc/window_train.hip); the trainable bias table is gathered, and its
+gradient summed, bucket by bucket (csrc/rel_bias.hip).
 """
 from __future__ import annotations
 
@@ -22,11 +24,11 @@ import torch.nn.functional as F
 
 from ..builder import BACKBONES
 from ..layernorm import HipLayerNorm, layernorm_map, map_supported          # nn.LayerNorm subclass: same keys, HIP kernels on CUDA tokens (ATen's ran 3.9 ms of a config-4 step)
-from .. import window_attn
+from .. import rel_bias, window_attn
 from ..layers import DropPath, to_2tuple, trunc_normal_
 
 
-_GATHER_WINDOWS = True          # test hook: False = the literal pad / roll / window_partition chain (the path a trainable Swin takes)
+_GATHER_WINDOWS = True          # test hook: False = the literal pad / roll / window_partition chain (the path a trainable Swin takes around its attention)
 _FUSE_NORMS = os.environ.get('SEGDISTILL_SWIN_FUSE_NORMS', '1') == '1'      # A/B: 0 = LayerNorm, zero-row cat, index_select and add as separate kernels
 _TABLES = {}
 
@@ -89,12 +91,20 @@ class WindowAttention(nn.Module):
         rel = (coords[:, :, None] - coords[:, None, :]).permute(1, 2, 0)   # [N, N, 2]
         index = (rel[..., 0] + wh - 1) * (2 * ww - 1) + (rel[..., 1] + ww - 1)
         self.register_buffer('relative_position_index', index)
+        self.bias_plan = rel_bias.BucketPlan(index, self.relative_position_bias_table.shape[0])
+        self.register_load_state_dict_post_hook(WindowAttention._plan_of_loaded_index)
         self.qkv = nn.Linear(dim, dim * 3, bias=qkv_bias)
         self.attn_drop = nn.Dropout(attn_drop)
         self.proj = nn.Linear(dim, dim)
         self.proj_drop = nn.Dropout(proj_drop)
         trunc_normal_(self.relative_position_bias_table, std=.02)
         self.softmax = nn.Softmax(dim=-1)
+
+    @staticmethod
+    def _plan_of_loaded_index(self, _keys):
+        """a checkpoint brings its own relative_position_index"""
+        if not torch.equal(self.bias_plan.index, self.relative_position_index.to(torch.int32)):
+            self.bias_plan = rel_bias.BucketPlan(self.relative_position_index, self.relative_position_bias_table.shape[0])
 
     def _bias_packed(self, n, h):
         """relative position bias [h, N, N] in the attention kernel's accumulator layout (padded keys = -inf); cached for a frozen table."""
@@ -134,9 +144,16 @@ class WindowAttention(nn.Module):
             # (csrc/window_attn.hip) -- no [windows, heads, N, N] additive tensor, no permuted copies of q / k / v or of the output
             out = window_attn.forward_packed(qkv.contiguous(), self._bias_packed(n, h), *self._mask_packed(mask), h, self.scale)
             return self.proj_drop(self.proj(out))
+        if (torch.is_grad_enabled() and (qkv.requires_grad or tbl.requires_grad) and not (self.training and self.attn_drop.p > 0)
+                and window_attn.train_supported(qkv, n, c // h) and (mask is None or bw % mask.shape[0] == 0)):
+            # a graph to build (a Swin student): the same product with its gradients, one kernel each way (csrc/window_train.hip)
+            return self.proj_drop(self.proj(window_attn.attention(qkv, rel_bias.bucket_bias(tbl, self.bias_plan), mask, h, self.scale)))
         q, k, v = qkv.reshape(bw, n, 3, h, c // h).permute(2, 0, 3, 1, 4)
         def additive():
-            bias = self.relative_position_bias_table[self.relative_position_index.view(-1)].view(n, n, h).permute(2, 0, 1)  # [h,N,N]
+            if tbl.is_cuda and tbl.requires_grad:
+                bias = rel_bias.bucket_bias(tbl, self.bias_plan)                                        # [h,N,N]
+            else:
+                bias = tbl[self.relative_position_index.view(-1)].view(n, n, h).permute(2, 0, 1)
             add = bias.unsqueeze(0)
             if mask is not None:
                 nw = mask.shape[0]

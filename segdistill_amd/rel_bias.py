@@ -11,6 +11,9 @@ from . import _lib
 from .ops import _DT, _launch_on, _require_gpu, _stream_ptr
 
 
+CHUNK = 512          # sd_bucket_bias_chunk(): the pairs of one bucket that one wave sums (a plan is built without the library)
+
+
 class BucketPlan(nn.Module):
     """The (query, key) pairs of `index` [Nq, Nk] (integers in [0, num_buckets)) in the order the gradient sums them.  Built once per index: it reads the
     index on the host.  A module without parameters or state-dict entries, so that a model that holds one moves it along."""
@@ -26,15 +29,14 @@ class BucketPlan(nn.Module):
         lo, hi = torch.stack(torch.aminmax(flat)).tolist()
         if lo < 0 or hi >= nb:
             raise ValueError(f'BucketPlan: index holds {lo} .. {hi}, outside [0, {nb})')
-        chunk = _lib.lib().sd_bucket_bias_chunk()
         order = torch.sort(flat, stable=True).indices
         count = torch.bincount(flat, minlength=nb)
-        chunks = ((count + chunk - 1) // chunk).clamp(min=1)               # an empty bucket: one empty chunk
+        chunks = ((count + CHUNK - 1) // CHUNK).clamp(min=1)               # an empty bucket: one empty chunk
         first = torch.cumsum(chunks, 0)
         bucket_chunk = torch.cat([first.new_zeros(1), first])
         owner = torch.repeat_interleave(torch.arange(nb, device=flat.device), chunks)
         within = torch.arange(owner.numel(), device=flat.device) - bucket_chunk[owner]
-        start = (torch.cumsum(count, 0) - count)[owner] + within * chunk
+        start = (torch.cumsum(count, 0) - count)[owner] + within * CHUNK
         self.num_buckets, self.shape = nb, tuple(index.shape)
         self.register_buffer('index', flat.int().view(index.shape), persistent=False)
         self.register_buffer('order', order.int(), persistent=False)

@@ -56,7 +56,8 @@ def test_topk_kl_refusals(L):
 
 def test_bucket_bias_refusals(L):
     c = L.sd_bucket_bias_chunk()
-    assert c == 512 and L.sd_bucket_bias_workspace_bytes(7, 7, 3) == 0 and L.sd_bucket_bias_workspace_bytes(7, 9, 3) == 9 * 3 * 4
+    from segdistill_amd import rel_bias
+    assert c == rel_bias.CHUNK and L.sd_bucket_bias_workspace_bytes(7, 7, 3) == 0 and L.sd_bucket_bias_workspace_bytes(7, 9, 3) == 9 * 3 * 4
 
     def fwd(t=P, i=P, o=P, dt=0, nb=7, h=3, n=100):
         return L.sd_bucket_bias_fwd(t, i, o, dt, nb, h, n, NULL)

@@ -1,0 +1,147 @@
+"""A Swin student: the attention of a trainable block on csrc/window_train.hip with the bias table through csrc/rel_bias.hip, against the same modules in
+fp64 on the CPU, and a KD step of such a student against its teacher's top logits (TopKLoss), eager and as a replayed graph."""
+import copy
+import math
+import warnings
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+
+def _layer(ws, dim=96, heads=3):
+    from segdistill_amd.backbones.swin import BasicLayer
+    torch.manual_seed(3)
+    layer = BasicLayer(dim=dim, depth=2, num_heads=heads, window_size=ws)
+    for blk in layer.blocks:
+        torch.nn.init.normal_(blk.attn.relative_position_bias_table, std=0.5)
+    return layer.train()
+
+
+@pytest.mark.parametrize('ws,hw,amp', [(7, (28, 28), False), (7, (30, 26), False), (5, (12, 13), False), (8, (16, 24), False), (7, (30, 26), True), (9, (18, 20), False)])
+def test_trainable_stage_matches_the_modules_in_fp64(ws, hw, amp, monkeypatch):
+    """unshifted + shifted block, whole and padded windows, window sizes 5 / 7 / 8 on the kernel (9: 81 tokens, the library's attention with the bucketed
+    bias).  Two blocks with their Linears, norms and GELU: fp32 2e-5 of the largest value, bf16 autocast 4e-2."""
+    from segdistill_amd import rel_bias, window_attn
+    layer = _layer(ws)
+    ref = copy.deepcopy(layer).double()
+    layer = layer.cuda()
+    calls, gathers = [], []
+    real, bias = window_attn.attention, rel_bias.bucket_bias
+    monkeypatch.setattr(window_attn, 'attention', lambda *a: (calls.append(a[0].dtype), real(*a))[1])
+    monkeypatch.setattr(rel_bias, 'bucket_bias', lambda *a: (gathers.append(1), bias(*a))[1])
+    h, w = hw
+    x = torch.randn(2, h * w, 96)
+    d = torch.randn(2, h * w, 96)
+    xg = x.cuda().requires_grad_()
+    with torch.autocast('cuda', dtype=torch.bfloat16, enabled=amp):
+        y = layer(xg, h, w)[0]
+    y.backward(d.cuda().to(y.dtype))
+    assert calls == ([] if ws == 9 else [torch.bfloat16 if amp else torch.float32] * 2) and len(gathers) == 2
+    xr = x.double().requires_grad_()
+    yr = ref(xr, h, w)[0]
+    yr.backward(d.double())
+    tol = 4e-2 if amp else 2e-5
+    assert float((y.double().cpu() - yr).abs().max() / yr.abs().max()) < tol
+    assert float((xg.grad.double().cpu() - xr.grad).abs().max() / xr.grad.abs().max()) < tol
+    for (n, p), (_, q) in zip(layer.named_parameters(), ref.named_parameters()):
+        assert p.grad is not None, n
+        # key biases do not move a softmax: their third of the qkv bias gradient is rounding alone
+        a, b = p.grad.double().cpu(), q.grad
+        assert float((a - b).abs().max()) < tol * float(b.abs().max()), n
+
+
+def test_table_gradient_is_the_same_each_time_and_the_switch_still_works(monkeypatch):
+    from segdistill_amd import window_attn
+    layer = _layer(7).cuda()
+    x = torch.randn(2, 30 * 26, 96, device='cuda')
+
+    def grads():
+        layer.zero_grad()
+        layer(x, 30, 26)[0].square().sum().backward()
+        return [b.attn.relative_position_bias_table.grad.clone() for b in layer.blocks]
+    a, b = grads(), grads()
+    assert all(torch.equal(p, q) for p, q in zip(a, b))
+    monkeypatch.setattr(window_attn, 'ENABLED', False)
+    c = grads()
+    assert all(float((p - q).abs().max()) < 2e-5 * float(q.abs().max()) for p, q in zip(a, c))
+
+
+def test_a_loaded_index_gives_the_plan():
+    from segdistill_amd.backbones.swin import WindowAttention
+    att = WindowAttention(64, (4, 4), 2).cuda()
+    sd = att.state_dict()
+    assert set(sd) == {'relative_position_bias_table', 'relative_position_index', 'qkv.weight', 'qkv.bias', 'proj.weight', 'proj.bias'}
+    sd['relative_position_index'] = sd['relative_position_index'].flip(0)
+    att.load_state_dict(sd)
+    assert torch.equal(att.bias_plan.index.long(), sd['relative_position_index']) and att.bias_plan.index.is_cuda
+
+
+def _model():
+    import segdistill_amd
+    from segdistill_amd.builder import build_segmentor
+    from segdistill_amd.segmentors import sd_module
+    segdistill_amd.register_all()
+
+    def seg(depths):
+        return dict(type='EncoderDecoder', pretrained=None,
+                    backbone=dict(type='SwinTransformer', embed_dim=64, depths=depths, num_heads=[2, 4], window_size=7, drop_path_rate=0., out_indices=(0, 1)),
+                    decode_head=dict(type='FCNHead', in_channels=128, in_index=1, channels=128, num_convs=0, concat_input=False, dropout_ratio=1e-12, num_classes=19,
+                                     norm_cfg=dict(type='SyncBN', requires_grad=True), align_corners=False,
+                                     loss_decode=dict(type='CrossEntropyLoss', use_sigmoid=False, loss_weight=1.0)))
+    cfg = dict(type='SDModule', cfg_s=seg([2, 2]), cfg_t=seg([2, 4]),
+               distillation=[dict(student_layer='decode_head.conv_seg', teacher_layer='decode_head.conv_seg', loss_name='TopKLoss',
+                                  loss_config=dict(k=5, alpha=3, tau=2, ignore_index=255, warmup_config={'mode': 'linear', 'warmup_iters': 2}))],
+               t_pretrain=None, train_cfg=dict(), test_cfg=dict(mode='whole'))
+    sd_module.SYNTHETIC_WEIGHTS_OK = True
+    try:
+        with warnings.catch_warnings():
+            warnings.simplefilter('ignore')
+            torch.manual_seed(0)
+            m = build_segmentor(cfg)
+    finally:
+        sd_module.SYNTHETIC_WEIGHTS_OK = False
+    for p in m.teacher.decode_head.conv_seg.parameters():
+        p.data.mul_(30)                       # a teacher that has opinions
+    return m.cuda()
+
+
+def test_kd_step_of_a_swin_student_against_top_logits_eager_and_replayed():
+    from segdistill_amd.engine import KDTrainer, SyntheticADE
+    opt, sched = dict(type='AdamW', lr=6e-5, betas=(0.9, 0.999), weight_decay=0.01), dict(policy='poly', power=1.0, min_lr=0.0, by_epoch=False)
+    ref = _model()
+    gra = copy.deepcopy(ref)
+    taps = {}
+    inner = ref.distillation_loss.forward
+
+    def spy(sf, tf, gt, step, *rest):
+        taps.update(s=sf['decode_head.conv_seg'].detach().double().cpu(), t=tf['decode_head.conv_seg'].detach().double().cpu(), gt=gt.cpu())
+        return inner(sf, tf, gt, step, *rest)
+    ref.distillation_loss.forward = spy
+    te, tg = KDTrainer(ref, opt, sched), KDTrainer(gra, opt, sched)
+    de, dg = (SyntheticADE(2, size=(112, 120), num_classes=19, device='cuda:0', pool=3, seed=1) for _ in range(2))
+    assert tg.enable_graph(dict(img=dg._pool[0][0], img_metas=None, gt_semantic_seg=dg._pool[0][1])), getattr(tg, 'graph_error', None)
+    for it in range(4):
+        te.step(de.next())
+        torch.cuda.synchronize()
+        tg.step(dg.next())
+        ve, vg = te.log_values(), tg.log_values()
+        key = [k for k in ve if k.startswith('loss_')]
+        assert list(ve) == list(vg) and len(key) == 1
+        # the definition on the taps that the eager step saw
+        alpha = ref.distillation_loss.criteria[0].alpha
+        s, t = (x.permute(0, 2, 3, 1).reshape(-1, 19) / 2 for x in (taps['s'], taps['t']))
+        keep = torch.nn.functional.interpolate(taps['gt'].float(), size=taps['s'].shape[2:], mode='nearest').reshape(-1) != 255
+        lp, lq = torch.log_softmax(t, 1), torch.log_softmax(s, 1)
+        top = t.topk(5, 1).indices
+        low = torch.ones_like(t, dtype=torch.bool).scatter(1, top, False)
+        terms = (lp.exp() * (lp - lq)).gather(1, top).sum(1)
+        pr, qr = ((l.masked_fill(~low, -math.inf)).logsumexp(1) for l in (lp, lq))
+        want = float(alpha * (terms + pr.exp() * (pr - qr))[keep].mean())
+        assert want > 0 and ve[key[0]] == pytest.approx(want, rel=1e-4)
+        for k in ve:
+            if 'acc' not in k:
+                assert vg[k] == pytest.approx(ve[k], abs=3e-4 * max(1.0, abs(ve[k]))), (it, k)
+    tables = [b.attn.relative_position_bias_table for l in ref.student.backbone.layers for b in l.blocks]
+    assert all(p.grad is not None and float(p.grad.abs().sum()) > 0 for p in tables)
