@@ -292,7 +292,7 @@ int sd_ppm_pool_bwd(void *const *d_pooled, int dtype, long planes, int h, int w,
  *   qkv    [windows, N, 3, heads, D]  the qkv Linear's output as it stands (swin_transformer.py:128-129 before the permute)
  *   out    [windows, N, heads*D]  = (attn @ v).transpose(1, 2).reshape(B_, N, C)   (:148)
  * Bias and mask come PACKED in the accumulator layout of the kernel, sd_window_attn_packed_floats() (= 64 * 64) floats per table:
- * sd_window_attn_pack converts `count` tables [N][N] (N <= 64; the training entry points below read the same layout) in the reference's orientation ([query][key]: relative_position_bias[head] of :133-135,
+ * sd_window_attn_pack converts `count` tables [49][49] in the reference's orientation ([query][key]: relative_position_bias[head] of :133-135,
  * mask[window] of :138; window b uses mask b % mask_windows, :140) and fills padded keys with pad_key_value (-INFINITY for the bias, 0 for the
  * mask); flags[count] (optional) receives 1 for a table with a nonzero entry -- the kernel skips the mask read of windows whose mask is all
  * zero (all but 37 of a 19 x 19 shifted partition).  mask_packed NULL: no mask (mask_flags ignored).
@@ -307,20 +307,23 @@ int sd_window_attn_fwd_packed(const void *qkv, const float *bias_packed, const f
 
 /* ---------------------------------------------------------------------------
  * The same attention with an autograd graph (a Swin student's blocks; csrc/window_train.hip): swin_transformer.py:119-153 and its backward.
- *   qkv [windows, N, 3, heads, D], out / dout [windows, N, heads*D], dqkv like qkv, storage SD_F32 | SD_BF16; dbias [heads][N][N] fp32
- *   bias_packed / mask_packed / mask_flags from sd_window_attn_pack (pad -INFINITY for the bias, 0 for the mask).
+ *   qkv [windows, N, 3, heads, D], out / dout [windows, N, heads*D], dqkv like qkv, storage SD_F32 | SD_BF16
+ *   bias [heads][N][N], mask [mask_windows][N][N] fp32 ([query][key]; window b uses mask b % mask_windows; mask_windows = 0: no mask)
+ *   packed: scratch of _packed_floats(), 16-byte aligned, that the forward fills (both tables in the kernels' layout) and the backward reads
+ *   dbias [heads][N][N] fp32
  * Softmax, its gradient and the bias gradient are fp32 for both storage types.  A row that bias + mask leave at -inf everywhere has output 0 and no
- * gradient.  The backward recomputes the probabilities: nothing but the operands is kept.  dbias sums the windows in a fixed order (per-wave slabs in
- * `workspace`, 16-byte aligned, sd_window_attn_train_workspace_bytes; no atomics).
- * _supported(): 1 <= N <= 64, D == 32, else SD_E_UNSUPPORTED.  All operands 16-byte aligned.
+ * gradient.  The backward recomputes the probabilities: nothing but the operands and `packed` is kept.  dbias sums the windows in a fixed order
+ * (slabs in `workspace`, 16-byte aligned, _workspace_bytes; no atomics).
+ * _supported(): 1 <= N <= 64, D == 32, else SD_E_UNSUPPORTED.  qkv, out, dout, dqkv 16-byte aligned.
  */
 int sd_window_attn_train_supported(int tokens_per_window, int head_dim);
-int sd_window_attn_train_fwd(const void *qkv, const float *bias_packed, const float *mask_packed, const int32_t *mask_flags, void *out, int dtype,
+size_t sd_window_attn_train_packed_floats(int heads, int mask_windows, int tokens_per_window);
+int sd_window_attn_train_fwd(const void *qkv, const float *bias, const float *mask, float *packed, size_t packed_floats, void *out, int dtype,
                              long windows, int mask_windows, int heads, int tokens_per_window, int head_dim, float scale, void *stream);
-size_t sd_window_attn_train_workspace_bytes(long windows, int heads, int tokens_per_window);
-int sd_window_attn_train_bwd(const void *qkv, const float *bias_packed, const float *mask_packed, const int32_t *mask_flags, const void *dout,
-                             void *dqkv, float *dbias, int dtype, long windows, int mask_windows, int heads, int tokens_per_window, int head_dim,
-                             float scale, void *workspace, size_t workspace_bytes, void *stream);
+size_t sd_window_attn_train_workspace_bytes(int dtype, long windows, int heads, int tokens_per_window);
+int sd_window_attn_train_bwd(const void *qkv, const float *packed, size_t packed_floats, const void *dout, void *dqkv, float *dbias, int dtype,
+                             long windows, int mask_windows, int heads, int tokens_per_window, int head_dim, float scale, void *workspace,
+                             size_t workspace_bytes, void *stream);
 
 /* ---------------------------------------------------------------------------
  * A learned position bias by buckets and its gradient (csrc/rel_bias.hip): relative_position_bias_table[relative_position_index] of

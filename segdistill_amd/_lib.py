@@ -57,9 +57,10 @@ SIGNATURES = {
     'sd_window_attn_pack': (_i, [_vp, _vp, _vp, _i, _i, _f, _vp]),
     'sd_window_attn_fwd_packed': (_i, [_vp, _vp, _vp, _vp, _vp, _i, C.c_long, _i, _i, _i, _i, _f, _vp]),
     'sd_window_attn_train_supported': (_i, [_i, _i]),
-    'sd_window_attn_train_fwd': (_i, [_vp, _vp, _vp, _vp, _vp, _i, C.c_long, _i, _i, _i, _i, _f, _vp]),
-    'sd_window_attn_train_workspace_bytes': (_sz, [C.c_long, _i, _i]),
-    'sd_window_attn_train_bwd': (_i, [_vp] * 7 + [_i, C.c_long, _i, _i, _i, _i, _f, _vp, _sz, _vp]),
+    'sd_window_attn_train_packed_floats': (_sz, [_i, _i, _i]),
+    'sd_window_attn_train_fwd': (_i, [_vp, _vp, _vp, _vp, _sz, _vp, _i, C.c_long, _i, _i, _i, _i, _f, _vp]),
+    'sd_window_attn_train_workspace_bytes': (_sz, [_i, C.c_long, _i, _i]),
+    'sd_window_attn_train_bwd': (_i, [_vp, _vp, _sz, _vp, _vp, _vp, _i, C.c_long, _i, _i, _i, _i, _f, _vp, _sz, _vp]),
     'sd_bucket_bias_chunk': (_i, []),
     'sd_bucket_bias_workspace_bytes': (_sz, [_i, _i, _i]),
     'sd_bucket_bias_fwd': (_i, [_vp, _vp, _vp, _i, _i, _i, C.c_long, _vp]),

@@ -175,20 +175,20 @@ __global__ __launch_bounds__(256) void window_attn_zero_flags(int *__restrict__ 
     if (i < n) flags[i] = 0;
 }
 
-// tables [n][N][N], N <= 64, in the reference's orientation ([query i][key j]) -> [n][a][b][g][lane][c] as the accumulators hold them; padded positions
-// take `pad_key` (keys j >= N) or 0 (queries i >= N); flags[n] = 1 if the table has a nonzero entry (NULL: not wanted)
+// tables [n][49][49] in the reference's orientation ([query i][key j]) -> [n][a][b][g][lane][c] as the accumulators hold them; padded positions
+// take `pad_key` (keys j >= 49) or 0 (queries i >= 49); flags[n] = 1 if the table has a nonzero entry (NULL: not wanted)
 __global__ __launch_bounds__(256) void window_attn_pack(const float *__restrict__ table, float *__restrict__ packed, int *__restrict__ flags, int n,
-                                                         int N, float pad_key) {
+                                                         float pad_key) {
     const long idx = (long)blockIdx.x * 256 + threadIdx.x;
     if (idx >= (long)n * kPackFloats) return;
     const int t = (int)(idx / kPackFloats), rem = (int)(idx - (long)t * kPackFloats);
     const int c = rem & 3, lane = (rem >> 2) & 63, g = (rem >> 8) & 3, b = (rem >> 10) & 1, a = rem >> 11;
     const int j = 32 * a + 8 * g + c + 4 * (lane >> 5), i = 32 * b + (lane & 31);
     float v = 0.f;
-    if (j >= N) v = pad_key;
-    else if (i < N) v = table[((size_t)t * N + i) * N + j];
+    if (j >= 49) v = pad_key;
+    else if (i < 49) v = table[((size_t)t * 49 + i) * 49 + j];
     packed[idx] = v;
-    if (flags && j < N && i < N && v != 0.f) flags[t] = 1;           // benign race: every writer stores 1
+    if (flags && j < 49 && i < 49 && v != 0.f) flags[t] = 1;           // benign race: every writer stores 1
 }
 
 }  // namespace
@@ -202,7 +202,7 @@ size_t sd_window_attn_packed_floats(void) { return (size_t)sd::kPackFloats; }
 
 int sd_window_attn_pack(const float *tables, float *packed, int32_t *flags, int count, int tokens_per_window, float pad_key_value, void *stream) {
     if (!tables || !packed) return SD_E_NULL;
-    if (tokens_per_window < 1 || tokens_per_window > 64) return SD_E_UNSUPPORTED;
+    if (tokens_per_window != 49) return SD_E_UNSUPPORTED;
     if (count <= 0 || (long)count * sd::kPackFloats > 0x7fffffffL * 256L) return SD_E_SHAPE;
     if (reinterpret_cast<uintptr_t>(packed) & 15) return SD_E_ALIGN;
     hipStream_t st = static_cast<hipStream_t>(stream);
@@ -210,8 +210,7 @@ int sd_window_attn_pack(const float *tables, float *packed, int32_t *flags, int 
     // a memset node -- memset nodes of one graph are corruptible by a concurrent memset on another stream (engine/trainer.py::_issues_memsets)
     if (flags) hipLaunchKernelGGL(sd::window_attn_zero_flags, dim3((unsigned)((count + 255) / 256)), dim3(256), 0, st, (int *)flags, count);
     const long total = (long)count * sd::kPackFloats;
-    hipLaunchKernelGGL(sd::window_attn_pack, dim3((unsigned)((total + 255) / 256)), dim3(256), 0, st, tables, packed, (int *)flags, count, tokens_per_window,
-                       pad_key_value);
+    hipLaunchKernelGGL(sd::window_attn_pack, dim3((unsigned)((total + 255) / 256)), dim3(256), 0, st, tables, packed, (int *)flags, count, pad_key_value);
     return (int)hipGetLastError();
 }
 

@@ -1,13 +1,11 @@
 """torch.autograd bindings over the C ABI (device pointers + the current HIP stream)."""
 from __future__ import annotations
 
-import contextlib
 import ctypes as C
 import math
 import os
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from . import _lib
 
@@ -28,9 +26,30 @@ def _ptr(t):
     return None if t is None else t.data_ptr()
 
 
-def _launch_on(device):
-    """Launches inside go to `device`, whichever device is current outside."""
-    return contextlib.nullcontext() if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+class _launch_on:
+    """`with _launch_on(device) as stream`: the device's current stream (a raw hipStream_t); launches inside go to that device, whichever is current
+    outside."""
+
+    __slots__ = ('index', 'back')
+
+    def __init__(self, device):
+        self.index, self.back = device.index, -1
+
+    def __enter__(self):
+        if torch.cuda.current_device() != self.index:
+            self.back = torch.cuda._exchange_device(self.index)
+        return torch._C._cuda_getCurrentRawStream(self.index)
+
+    def __exit__(self, *exc):
+        if self.back >= 0:
+            torch.cuda._exchange_device(self.back)
+        return False
+
+
+def _no_double_backward(name):
+    """The gradients are kernels' outputs without a graph of their own; under create_graph they would be constants, silently."""
+    if torch.is_grad_enabled():
+        raise RuntimeError(f'{name} has no second derivative (backward was called with create_graph=True)')
 
 
 class _CGDKLFunction(torch.autograd.Function):
@@ -696,9 +715,9 @@ def topk_logits(x, k, *, tau=1.0):
     index = torch.empty(_entry_shape(x, k), dtype=torch.int32, device=x.device)
     rest = torch.empty(_row_shape(x), dtype=torch.float32, device=x.device)
     if x.numel():
-        with _launch_on(x.device):
-            _lib.check(L.sd_topk_select(x.data_ptr(), values.data_ptr(), index.data_ptr(), rest.data_ptr(), _DT[x.dtype], B, Cc, P, k, tau, _stream_ptr()),
-                       'sd_topk_select')
+        with _launch_on(x.device) as stream:
+            rc = L.sd_topk_select(x.data_ptr(), values.data_ptr(), index.data_ptr(), rest.data_ptr(), _DT[x.dtype], B, Cc, P, k, tau, stream)
+        _lib.check(rc, 'sd_topk_select')
     return values, index, rest
 
 
@@ -708,30 +727,31 @@ class _TopKKLFunction(torch.autograd.Function):
         L = _lib.lib()
         rows = B * P
         ws_bytes = L.sd_topk_kl_workspace_bytes(B, Cc, P, k)
-        ws = torch.empty(ws_bytes, dtype=torch.uint8, device=S.device)
-        stats = torch.empty(rows, 4, dtype=torch.float32, device=S.device)
-        inv_rows = torch.empty((), dtype=torch.float32, device=S.device)
+        # one allocation: four floats per row and 1 / n (padded to 16 bytes) for the backward, then the forward's workspace
+        keep = torch.empty(4 * rows + 4 + ws_bytes // 4, dtype=torch.float32, device=S.device)
         loss = torch.empty((), dtype=torch.float32, device=S.device)
-        with _launch_on(S.device):
+        at = keep.data_ptr()
+        with _launch_on(S.device) as stream:
             rc = L.sd_topk_kl_fwd(S.data_ptr(), values.data_ptr(), index.data_ptr(), _ptr(rest), _ptr(valid), _DT[S.dtype], _DT[values.dtype], B, Cc, P, k,
-                                  tau, alpha, stats.data_ptr(), inv_rows.data_ptr(), loss.data_ptr(), ws.data_ptr(), ws_bytes, _stream_ptr())
+                                  tau, alpha, at, at + 16 * rows, loss.data_ptr(), at + 16 * rows + 16, ws_bytes, stream)
         _lib.check(rc, 'sd_topk_kl_fwd')
-        ctx.save_for_backward(S, values, index, rest, valid, stats, inv_rows)
+        ctx.save_for_backward(S, values, index, rest, valid, keep)
         ctx.meta = (tau, alpha, B, Cc, P, k)
         return loss
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, grad_loss):
-        S, values, index, rest, valid, stats, inv_rows = ctx.saved_tensors
+        _no_double_backward('topk_kl')
+        S, values, index, rest, valid, keep = ctx.saved_tensors
         tau, alpha, B, Cc, P, k = ctx.meta
         dS = torch.empty_like(S)
-        up = grad_loss.to(torch.float32).contiguous()
-        with _launch_on(S.device):
+        up = grad_loss if grad_loss.dtype == torch.float32 else grad_loss.float()
+        at = keep.data_ptr()
+        with _launch_on(S.device) as stream:
             rc = _lib.lib().sd_topk_kl_bwd(S.data_ptr(), values.data_ptr(), index.data_ptr(), _ptr(rest), _ptr(valid), _DT[S.dtype], _DT[values.dtype], B, Cc,
-                                           P, k, tau, alpha, stats.data_ptr(), inv_rows.data_ptr(), up.data_ptr(), dS.data_ptr(), _stream_ptr())
+                                           P, k, tau, alpha, at, at + 16 * B * P, up.data_ptr(), dS.data_ptr(), stream)
         _lib.check(rc, 'sd_topk_kl_bwd')
-        return (dS,) + (None,) * 10
+        return dS, None, None, None, None, None, None, None, None, None, None
 
 
 def topk_kl(S, values, index, rest=None, *, tau, alpha, valid=None):

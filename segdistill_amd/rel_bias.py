@@ -5,10 +5,9 @@ from __future__ import annotations
 
 import torch
 import torch.nn as nn
-from torch.autograd.function import once_differentiable
 
 from . import _lib
-from .ops import _DT, _launch_on, _require_gpu, _stream_ptr
+from .ops import _DT, _launch_on, _no_double_backward, _ptr, _require_gpu
 
 
 CHUNK = 512          # sd_bucket_bias_chunk(): the pairs of one bucket that one wave sums (a plan is built without the library)
@@ -51,26 +50,28 @@ class _BucketBiasFunction(torch.autograd.Function):
     @staticmethod
     def forward(ctx, table, plan):
         nb, heads = table.shape
+        index = plan._buffers['index']
         out = torch.empty((heads,) + plan.shape, dtype=table.dtype, device=table.device)
-        with _launch_on(table.device):
-            rc = _lib.lib().sd_bucket_bias_fwd(table.data_ptr(), plan.index.data_ptr(), out.data_ptr(), _DT[table.dtype], nb, heads, plan.index.numel(), _stream_ptr())
+        with _launch_on(table.device) as stream:
+            rc = _lib.lib().sd_bucket_bias_fwd(table.data_ptr(), index.data_ptr(), out.data_ptr(), _DT[table.dtype], nb, heads, index.numel(), stream)
         _lib.check(rc, 'sd_bucket_bias_fwd')
         ctx.plan = plan
         return out
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, grad_out):
+        _no_double_backward('bucket_bias')
         plan = ctx.plan
+        order, start, bucket = plan._buffers['order'], plan._buffers['chunk_start'], plan._buffers['bucket_chunk']
         d = grad_out.contiguous()
-        heads, nb, chunks = d.shape[0], plan.num_buckets, plan.chunk_start.numel() - 1
+        heads, nb, chunks = d.shape[0], plan.num_buckets, start.numel() - 1
         L = _lib.lib()
         dtable = torch.empty(nb, heads, dtype=d.dtype, device=d.device)
         ws_bytes = L.sd_bucket_bias_workspace_bytes(nb, chunks, heads)
         ws = torch.empty(ws_bytes, dtype=torch.uint8, device=d.device) if ws_bytes else None
-        with _launch_on(d.device):
-            rc = L.sd_bucket_bias_bwd(d.data_ptr(), plan.order.data_ptr(), plan.chunk_start.data_ptr(), plan.bucket_chunk.data_ptr(), dtable.data_ptr(),
-                                      _DT[d.dtype], nb, chunks, heads, plan.index.numel(), None if ws is None else ws.data_ptr(), ws_bytes, _stream_ptr())
+        with _launch_on(d.device) as stream:
+            rc = L.sd_bucket_bias_bwd(d.data_ptr(), order.data_ptr(), start.data_ptr(), bucket.data_ptr(), dtable.data_ptr(), _DT[d.dtype], nb, chunks, heads,
+                                      order.numel(), _ptr(ws), ws_bytes, stream)
         _lib.check(rc, 'sd_bucket_bias_bwd')
         return dtable, None
 
@@ -82,6 +83,6 @@ def bucket_bias(table, plan):
         raise TypeError(f'bucket_bias: unsupported dtype {table.dtype}')
     if table.dim() != 2 or table.shape[0] != plan.num_buckets or table.shape[1] == 0:
         raise ValueError(f'bucket_bias: table {tuple(table.shape)} does not fit a plan of {plan.num_buckets} buckets')
-    if plan.index.device != table.device:
+    if plan._buffers['index'].device != table.device:
         raise ValueError(f'bucket_bias: the plan is on {plan.index.device}, the table on {table.device}')
     return _BucketBiasFunction.apply(table.contiguous(), plan)

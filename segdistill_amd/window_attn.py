@@ -6,10 +6,9 @@ from __future__ import annotations
 import os
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from . import _lib
-from .ops import _DT, _launch_on, _ptr, _require_gpu, _stream_ptr
+from .ops import _DT, _launch_on, _no_double_backward, _ptr, _require_gpu, _stream_ptr
 
 ENABLED = os.environ.get('SEGDISTILL_WINDOW_ATTN', '1') == '1'       # A/B: 0 = F.scaled_dot_product_attention with a materialised additive tensor
 
@@ -21,15 +20,15 @@ def supported(qkv, n, heads, head_dim):
 
 
 def pack_tables(tables, pad_key=0.0, want_flags=False):
-    """[n, N, N] additive tables, N <= 64, in the reference's orientation ([query, key]) -> ([n, 4096] in the MFMA kernel's accumulator layout,
+    """[n, 49, 49] additive tables in the reference's orientation ([query, key]) -> ([n, 4096] in the MFMA kernel's accumulator layout,
     int32 flags [n] = table has a nonzero entry, or None)."""
     t = tables.detach().float().contiguous()
     n = t.shape[0]
-    assert t.dim() == 3 and t.shape[1] == t.shape[2] <= 64
+    assert t.shape[1:] == (49, 49)
     L = _lib.lib()
     packed = torch.empty(n, int(L.sd_window_attn_packed_floats()), dtype=torch.float32, device=t.device)
     flags = torch.empty(n, dtype=torch.int32, device=t.device) if want_flags else None
-    _lib.check(L.sd_window_attn_pack(t.data_ptr(), packed.data_ptr(), None if flags is None else flags.data_ptr(), n, t.shape[1], float(pad_key), _stream_ptr()),
+    _lib.check(L.sd_window_attn_pack(t.data_ptr(), packed.data_ptr(), None if flags is None else flags.data_ptr(), n, 49, float(pad_key), _stream_ptr()),
                'sd_window_attn_pack')
     return packed, flags
 
@@ -57,36 +56,37 @@ class _WindowAttentionFunction(torch.autograd.Function):
     @staticmethod
     def forward(ctx, qkv, bias, mask, heads, scale):
         bw, n, c3 = qkv.shape
-        c = c3 // 3
-        out = torch.empty(bw, n, c, dtype=qkv.dtype, device=qkv.device)
-        with _launch_on(qkv.device):
-            bias_p = pack_tables(bias, float('-inf'))[0]
-            mask_p, flags = pack_tables(mask, 0.0, True) if mask is not None else (None, None)
-            rc = _lib.lib().sd_window_attn_train_fwd(qkv.data_ptr(), bias_p.data_ptr(), _ptr(mask_p), _ptr(flags), out.data_ptr(), _DT[qkv.dtype], bw,
-                                                     0 if mask is None else mask.shape[0], heads, n, c // heads, scale, _stream_ptr())
+        nw, dt, L = (0 if mask is None else mask.shape[0]), _DT[qkv.dtype], _lib.lib()
+        b = bias.detach().to(torch.float32).contiguous()
+        m = None if mask is None else mask.to(torch.float32).contiguous()
+        floats = L.sd_window_attn_train_packed_floats(heads, nw, n)
+        packed = torch.empty(floats, dtype=torch.float32, device=qkv.device)
+        out = torch.empty(bw, n, c3 // 3, dtype=qkv.dtype, device=qkv.device)
+        with _launch_on(qkv.device) as stream:
+            rc = L.sd_window_attn_train_fwd(qkv.data_ptr(), b.data_ptr(), _ptr(m), packed.data_ptr(), floats, out.data_ptr(), dt, bw, nw, heads, n,
+                                            c3 // 3 // heads, scale, stream)
         _lib.check(rc, 'sd_window_attn_train_fwd')
-        ctx.save_for_backward(qkv, bias_p, mask_p, flags)
-        ctx.meta = (heads, scale, bias.dtype)
+        ctx.save_for_backward(qkv, packed)
+        ctx.meta = (nw, heads, scale, bias.dtype)
         return out
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, grad_out):
-        qkv, bias_p, mask_p, flags = ctx.saved_tensors
-        heads, scale, bias_dtype = ctx.meta
+        _no_double_backward('window_attn.attention')
+        qkv, packed = ctx.saved_tensors
+        nw, heads, scale, bias_dtype = ctx.meta
         bw, n, c3 = qkv.shape
-        L = _lib.lib()
+        L, dt = _lib.lib(), _DT[qkv.dtype]
         go = grad_out.to(qkv.dtype).contiguous()
         if go.data_ptr() % 16:
             go = go.clone()
         dqkv = torch.empty_like(qkv)
         dbias = torch.empty(heads, n, n, dtype=torch.float32, device=qkv.device)
-        ws_bytes = L.sd_window_attn_train_workspace_bytes(bw, heads, n)
+        ws_bytes = L.sd_window_attn_train_workspace_bytes(dt, bw, heads, n)
         ws = torch.empty(ws_bytes, dtype=torch.uint8, device=qkv.device)
-        with _launch_on(qkv.device):
-            rc = L.sd_window_attn_train_bwd(qkv.data_ptr(), bias_p.data_ptr(), _ptr(mask_p), _ptr(flags), go.data_ptr(), dqkv.data_ptr(), dbias.data_ptr(),
-                                            _DT[qkv.dtype], bw, 0 if mask_p is None else mask_p.shape[0], heads, n, c3 // 3 // heads, scale, ws.data_ptr(),
-                                            ws_bytes, _stream_ptr())
+        with _launch_on(qkv.device) as stream:
+            rc = L.sd_window_attn_train_bwd(qkv.data_ptr(), packed.data_ptr(), packed.numel(), go.data_ptr(), dqkv.data_ptr(), dbias.data_ptr(), dt, bw, nw, heads,
+                                            n, c3 // 3 // heads, scale, ws.data_ptr(), ws_bytes, stream)
         _lib.check(rc, 'sd_window_attn_train_bwd')
         return dqkv, dbias.to(bias_dtype), None, None, None
 

@@ -74,22 +74,23 @@ def test_bucket_bias_refusals(L):
 def test_window_attention_refusals(L):
     ok = L.sd_window_attn_train_supported
     assert ok(1, 32) and ok(49, 32) and ok(64, 32) and not ok(0, 32) and not ok(65, 32) and not ok(49, 64)
-    ws = L.sd_window_attn_train_workspace_bytes(6, 3, 49)
-    assert ws > 0 and L.sd_window_attn_train_workspace_bytes(6, 3, 65) == 0 and L.sd_window_attn_train_workspace_bytes(0, 3, 49) == 0
+    ws, pk = L.sd_window_attn_train_workspace_bytes(0, 6, 3, 49), L.sd_window_attn_train_packed_floats(3, 2, 49)
+    assert ws > 0 and L.sd_window_attn_train_workspace_bytes(0, 6, 3, 65) == 0 and L.sd_window_attn_train_workspace_bytes(0, 0, 3, 49) == 0
+    assert L.sd_window_attn_train_workspace_bytes(2, 6, 3, 49) == 0 and pk == 5 * 4096 + 2 and L.sd_window_attn_train_packed_floats(3, -1, 49) == 0
 
-    def fwd(q=P, b=P, m=NULL, f=NULL, o=P, dt=0, w=6, nw=0, h=3, n=49, d=32):
-        return L.sd_window_attn_train_fwd(q, b, m, f, o, dt, w, nw, h, n, d, 1.0, NULL)
+    def fwd(q=P, b=P, m=NULL, k=P, kf=pk, o=P, dt=0, w=6, nw=0, h=3, n=49, d=32):
+        return L.sd_window_attn_train_fwd(q, b, m, k, kf, o, dt, w, nw, h, n, d, 1.0, NULL)
 
-    def bwd(q=P, b=P, m=NULL, f=NULL, g=P, dq=P, db=P, dt=0, w=6, nw=0, h=3, n=49, d=32, s=P, sb=ws):
-        return L.sd_window_attn_train_bwd(q, b, m, f, g, dq, db, dt, w, nw, h, n, d, 1.0, s, sb, NULL)
-    for f, names in ((fwd, 'qbo'), (bwd, ('q', 'b', 'g', 'dq', 'db'))):
+    def bwd(q=P, k=P, kf=pk, g=P, dq=P, db=P, dt=0, w=6, nw=0, h=3, n=49, d=32, s=P, sb=ws):
+        return L.sd_window_attn_train_bwd(q, k, kf, g, dq, db, dt, w, nw, h, n, d, 1.0, s, sb, NULL)
+    for f, names in ((fwd, 'qbko'), (bwd, ('q', 'k', 'g', 'dq', 'db'))):
         for a in names:
             assert f(**{a: NULL}) == E_NULL, a
         assert f(dt=2) == E_DTYPE and f(n=65) == E_UNSUP and f(n=0) == E_UNSUP and f(d=16) == E_UNSUP
-        assert f(w=0) == f(h=0) == f(w=2 ** 40) == E_SHAPE and f(m=P, f=P, nw=4) == E_SHAPE and f(m=P, nw=3) == E_SHAPE and f(m=P, f=P, nw=0) == E_SHAPE
-        assert f(q=P + 4) == E_ALIGN and f(m=P + 4, f=P, nw=3) == E_ALIGN
+        assert f(w=0) == f(h=0) == f(w=2 ** 40) == f(nw=4) == f(nw=-1) == E_SHAPE and f(kf=10) == E_WS and f(nw=3) == E_WS
+        assert f(q=P + 4) == E_ALIGN and f(k=P + 4) == E_ALIGN
+    assert fwd(nw=2) == E_NULL and fwd(nw=2, m=P + 2) == E_ALIGN and fwd(b=P + 2) == E_ALIGN
     assert bwd(s=NULL) == E_WS and bwd(sb=ws - 1) == E_WS and bwd(s=P + 8) == E_WS and bwd(g=P + 8) == E_ALIGN and fwd(o=P + 8) == E_ALIGN
-    assert L.sd_window_attn_pack(P, P, NULL, 1, 65, 0.0, NULL) == E_UNSUP and L.sd_window_attn_pack(P, P, NULL, 1, 0, 0.0, NULL) == E_UNSUP
 
 
 def test_bucket_plan_orders_every_pair_once_and_refuses_bad_maps():
