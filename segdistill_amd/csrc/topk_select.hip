@@ -82,96 +82,235 @@ __global__ __launch_bounds__(256) void topk_planes(const T *__restrict__ x, T *_
     rest[(size_t)b * P + p] = low.s > 0.f || low.s != low.s ? low.m + tau * logf(low.s) : -INFINITY;
 }
 
-// ---- contiguous rows --------------------------------------------------------------------------------------------------------------------------
-// NT threads per row.  1: every thread takes the maximum of its own elements; the k-th largest of these NT maxima is a lower bound of the row's
-// k-th largest value (k different elements reach it).  2: elements that reach the bound -- about k of them unless the row is adverse -- go to a
-// list in LDS, the others into the rest's running sum.  3: each list entry counts the entries that come before it: its rank is its place.  A
-// row with more than CAP elements at the bound (constant rows, many ties) takes the k-th key exactly, by four histograms of its bytes.
-template <typename T, int NT, typename F>
-__device__ __forceinline__ void scan_row(const T *__restrict__ row, int V, int tid, F f) {
-    constexpr int N = VecIO<T>::N;
-    const int head = row_head(row, V), nvec = (V - head) / N;
-    if (tid < head) {
-        const float one[1] = {VecIO<T>::load1(row + tid)};
-        f(one, tid);
+// The same with the pixels' classes parked in LDS (a column per lane, 64 pixels per wave) when they fit: the register list costs K steps per class; here
+// the maxima of groups of eight classes sit in registers, and each of the k rounds takes the largest of them and scans its group again -- ng + 8 steps per
+// entry instead of K per class.  A taken class is overwritten by kNoKey, so the sum of the rest is one more pass over the column with its maximum known.
+// The scans go up and compare strictly: the lowest class wins a tie.
+template <typename T, int NG>
+__global__ __launch_bounds__(64) void topk_planes_lds(const T *__restrict__ x, T *__restrict__ values, int *__restrict__ index, float *__restrict__ rest, int C,
+                                                      long P, int blocks_per_image, int k, float tau, float c2) {
+    extern __shared__ int column[];
+    int *mine = column + threadIdx.x;                 // class c at mine[64 c]; rows up to a multiple of eight
+    const long b = blockIdx.x / blocks_per_image;
+    const long p = (long)(blockIdx.x - b * blocks_per_image) * 64 + threadIdx.x;
+    const bool live = p < P;
+    const T *px = x + (size_t)b * C * P + (live ? p : P - 1);
+    // a wave's column leaves room for one wave per SIMD or two: all its loads go out before the first is used
+    float f[NG * 8];
+#pragma unroll
+    for (int g = 0; g < NG; g += 4)
+        if (g * 8 < C) {
+#pragma unroll
+            for (int u = 0; u < 32; ++u) f[g * 8 + u] = VecIO<T>::load1(px + (size_t)min(g * 8 + u, C - 1) * P);
+        }
+    int top[NG];
+#pragma unroll
+    for (int g = 0; g < NG; ++g) {
+        top[g] = kNoKey;
+        if (g * 8 < C) {                              // whole groups
+#pragma unroll
+            for (int u = 0; u < 8; ++u) {
+                const int c = g * 8 + u, n = c < C ? key_of(f[c]) : kNoKey;
+                mine[64 * c] = n;
+                top[g] = max(top[g], n);
+            }
+        }
     }
+    for (int j = 0; j < k; ++j) {
+        int best = top[0], bg = 0;
+#pragma unroll
+        for (int g = 1; g < NG; ++g) {
+            const bool gt = top[g] > best;
+            best = gt ? top[g] : best;
+            bg = gt ? g : bg;
+        }
+        int *group = mine + 512 * bg;
+        int at = -1, next = kNoKey;
+#pragma unroll
+        for (int u = 0; u < 8; ++u) {
+            const int n = group[64 * u];
+            const bool here = n == best && at < 0;
+            at = here ? u : at;
+            next = here ? next : max(next, n);
+        }
+        group[64 * at] = kNoKey;
+#pragma unroll
+        for (int g = 0; g < NG; ++g) top[g] = g == bg ? next : top[g];
+        if (live) {
+            const size_t o = ((size_t)b * k + j) * P + p;
+            VecIO<T>::store1(values + o, of_key(best));
+            index[o] = 8 * bg + at;
+        }
+    }
+    int m = kMinusInfKey;
+#pragma unroll
+    for (int g = 0; g < NG; ++g) m = max(m, top[g]);
+    const float ref = finite_ref(of_key(m));
+    float s = 0.f;
+    for (int c = 0; c < C; c += 8) {
+#pragma unroll
+        for (int u = 0; u < 8; ++u) {
+            const int n = mine[64 * (c + u)];
+            const float e = ex2((of_key(n) - ref) * c2);
+            s += n > kMinusInfKey ? e : 0.f;
+        }
+    }
+    if (live) rest[(size_t)b * P + p] = s > 0.f || s != s ? ref + tau * logf(s) : -INFINITY;
+}
+
+// ---- contiguous rows --------------------------------------------------------------------------------------------------------------------------
+// NT threads per row, the row in their registers: NV 16-byte vectors each (a longer row comes by in tiles, and is read a second time).
+// 1: group maxima -- each of up to 256 groups of threads takes the largest of its elements.  The k-th largest of these maxima bounds the row's k-th
+// largest value from below (k different elements reach it); one wave finds it by bisection of the ordered keys, 20 bits of them: a lower bound stays
+// one.  2: elements that reach the bound -- about k of them unless the row is adverse -- go to a list in LDS, the others into the rest's sum, taken
+// relative to the bound (they lie below it).  3: each list entry counts the entries before it: its rank is its place.
+// A row with more than CAP elements at the bound (constant rows, many ties) takes the k-th key exactly, by four histograms of its bytes; a rest that
+// lies so far below the bound that its sum loses digits is summed again relative to its own maximum.
+template <typename T, int NT, int NV>
+struct RowTile {
+    static constexpr int N = VecIO<T>::N;
     typedef typename VecIO<T>::raw_t raw_t;
-    const raw_t *v = reinterpret_cast<const raw_t *>(row + head);
-    for (int i = tid; i < nvec; i += NT) {
-        const raw_t r = v[i];
-        float a[N];
+    const T *row;
+    int V, head, nvec, tail;
+    raw_t reg[NV];
+
+    __device__ __forceinline__ RowTile(const T *r, int v) : row(r), V(v) {
+        head = row_head(r, v);
+        nvec = (v - head) / N;
+        tail = head + nvec * N;
+    }
+    __device__ __forceinline__ int tiles() const { return nvec > NT * NV ? (nvec + NT * NV - 1) / (NT * NV) : 1; }
+    __device__ __forceinline__ void load(int tile, int tid) {
+        const raw_t *v = reinterpret_cast<const raw_t *>(row + head) + (long)tile * NT * NV;
+        const int n = nvec - tile * NT * NV;
+#pragma unroll
+        for (int u = 0; u < NV; ++u)
+            if (tid + u * NT < n) reg[u] = __builtin_nontemporal_load(v + tid + u * NT);
+    }
+    __device__ __forceinline__ void unpack(int u, float (&a)[N]) const {
         if constexpr (N == 4) {
 #pragma unroll
-            for (int q = 0; q < 4; ++q) a[q] = r[q];
+            for (int q = 0; q < 4; ++q) a[q] = reg[u][q];
         } else {
 #pragma unroll
-            for (int q = 0; q < 4; ++q) a[2 * q] = __uint_as_float((unsigned)r[q] << 16), a[2 * q + 1] = __uint_as_float((unsigned)r[q] & 0xffff0000u);
+            for (int q = 0; q < 4; ++q) a[2 * q] = __uint_as_float((unsigned)reg[u][q] << 16), a[2 * q + 1] = __uint_as_float((unsigned)reg[u][q] & 0xffff0000u);
         }
-        f(a, head + i * N);
     }
-    const int t = head + nvec * N + tid;
-    if (t < V) {
-        const float one[1] = {VecIO<T>::load1(row + t)};
-        f(one, t);
+    // f(values, first index) for every element of the row that is this thread's; one tile: from the registers that hold it
+    template <typename F>
+    __device__ __forceinline__ void each(int tid, bool reload, F f) {
+        if (tid < head) {
+            const float one[1] = {VecIO<T>::load1(row + tid)};
+            f(one, tid);
+        }
+        const int nt = tiles();
+        for (int tile = 0; tile < nt; ++tile) {
+            if (reload || nt > 1) load(tile, tid);
+            const int n = nvec - tile * NT * NV, first = head + tile * NT * NV * N;
+#pragma unroll
+            for (int u = 0; u < NV; ++u) {
+                if (u * NT >= n) break;
+                if (tid + u * NT < n) {
+                    float a[N];
+                    unpack(u, a);
+                    f(a, first + (tid + u * NT) * N);
+                }
+            }
+        }
+        if (tail + tid < V) {
+            const float one[1] = {VecIO<T>::load1(row + tail + tid)};
+            f(one, tail + tid);
+        }
     }
-}
+};
 
 template <int NT>
 struct SelectShared {
-    static constexpr int CAP = NT == 64 ? 256 : 1024;
-    int max_key[NT];
-    int key[CAP], idx[CAP];
+    static constexpr int CAP = NT == 64 ? 256 : 1024, GROUPS = NT < 256 ? NT : 256;
+    float max_of[GROUPS];
+    unsigned long long entry[CAP];                    // key above, ~index below: descending keys, ascending indices
     float left[CAP];
     Online tmp[NT / 64];
     int hist[256];
-    int count, bound, bin, need, ties, wave_ties[NT / 64];
+    unsigned long long last;
+    int count, bin, need, ties, wave_ties[NT / 64];
+    float bound;
 };
 
-template <typename T, int NT>
+__device__ __forceinline__ unsigned long long entry_of(int key, int idx) { return ((unsigned long long)((unsigned)key ^ 0x80000000u) << 32) | (unsigned)~idx; }
+__device__ __forceinline__ int entry_key(unsigned long long e) { return (int)((unsigned)(e >> 32) ^ 0x80000000u); }
+__device__ __forceinline__ int entry_idx(unsigned long long e) { return (int)~(unsigned)e; }
+
+template <typename T, int NT, int NV>
 __global__ __launch_bounds__(NT == 64 ? 256 : NT) void topk_rows(const T *__restrict__ x, T *__restrict__ values, int *__restrict__ index,
                                                                  float *__restrict__ rest, long rows, int V, int k, float tau, float c2) {
-    constexpr int G = NT == 64 ? 4 : 1, CAP = SelectShared<NT>::CAP;
-    __shared__ SelectShared<NT> shared[G];
-    SelectShared<NT> &sh = shared[NT == 64 ? threadIdx.x >> 6 : 0];
+    typedef SelectShared<NT> Shared;
+    constexpr int G = NT == 64 ? 4 : 1, CAP = Shared::CAP, GROUPS = Shared::GROUPS;
+    __shared__ Shared shared[G];
+    Shared &sh = shared[NT == 64 ? threadIdx.x >> 6 : 0];
     const int tid = NT == 64 ? threadIdx.x & 63 : threadIdx.x;
     const long r = (long)blockIdx.x * G + (NT == 64 ? threadIdx.x >> 6 : 0);
     if (r >= rows) return;                            // whole waves (NT == 64) or never (one row per workgroup)
-    const T *row = x + (size_t)r * V;
+    RowTile<T, NT, NV> row(x + (size_t)r * V, V);
 
-    int mine = kNoKey;
-    scan_row<T, NT>(row, V, tid, [&](const auto &a, int) {
-        for (const float f : a) mine = max(mine, key_of(f));
+    float mine = -INFINITY;                           // NaN elements drop out here: the bound only gets lower
+    row.each(tid, true, [&](const auto &a, int) {
+        for (const float f : a) mine = fmaxf(mine, f);
     });
-    sh.max_key[tid] = mine;
+    if constexpr (NT / GROUPS > 1) {
+#pragma unroll
+        for (int d = 1; d < NT / GROUPS; d <<= 1) mine = fmaxf(mine, __shfl_xor(mine, d, 64));
+    }
+    if (tid % (NT / GROUPS) == 0) sh.max_of[tid / (NT / GROUPS)] = mine;
     if (tid == 0) sh.count = 0;
     group_sync<NT>();
-    int before = 0;
-    for (int u = 0; u < NT; ++u) {
-        const int o = sh.max_key[u];
-        before += o > mine || (o == mine && u < tid);
+    if (tid < 64) {
+        unsigned u[GROUPS / 64];
+#pragma unroll
+        for (int q = 0; q < GROUPS / 64; ++q) u[q] = (unsigned)key_of(sh.max_of[64 * q + tid]) ^ 0x80000000u;
+        unsigned low = 0;
+        for (int bit = 31; bit >= 12; --bit) {
+            const unsigned trial = low | (1u << bit);
+            int n = 0;
+#pragma unroll
+            for (int q = 0; q < GROUPS / 64; ++q) n += __popcll(__ballot(u[q] >= trial));
+            if (n >= k) low = trial;
+        }
+        if (tid == 0) sh.bound = of_key((int)(low ^ 0x80000000u));        // below -inf this is a NaN: then every element is taken
     }
-    if (before == k - 1) sh.bound = mine;
     group_sync<NT>();
-    int bound = sh.bound;
+    const float bound = sh.bound;
 
-    Online low = {-INFINITY, 0.f};
-    scan_row<T, NT>(row, V, tid, [&](const auto &a, int i0) {
+    // the sum of the elements below the bound, relative to it: 2^{x c2 - bound c2} in one rounding.  Where bound * c2 leaves the range there is no such sum;
+    // the last step below takes it then.
+    const float shift = bound * c2;
+    const bool fits = fabsf(shift) < 1e30f;
+    float sum = 0.f;
+    row.each(tid, false, [&](const auto &a, int i0) {
         constexpr int N = sizeof(a) / sizeof(float);
-        float out[N];
+        float e[N];
+        bool any = false;
 #pragma unroll
         for (int i = 0; i < N; ++i) {
-            const int n = key_of(a[i]);
-            out[i] = a[i];
-            if (n >= bound) {
-                out[i] = -INFINITY;
-                const int at = atomicAdd(&sh.count, 1);
-                if (at < CAP) sh.key[at] = n, sh.idx[at] = i0 + i;
-            }
+            any |= !(a[i] < bound);
+            e[i] = ex2(fmaf(a[i], c2, -shift));
         }
-        online_fold(low, out, c2);
+        if (any) {
+#pragma unroll
+            for (int i = 0; i < N; ++i)
+                if (!(a[i] < bound)) {
+                    e[i] = 0.f;
+                    const int at = atomicAdd(&sh.count, 1);
+                    if (at < CAP) sh.entry[at] = entry_of(key_of(a[i]), i0 + i);
+                }
+        }
+#pragma unroll
+        for (int i = 0; i < N; ++i) sum += e[i];
     });
+    if (!fits) sum = 0.f;
     group_sync<NT>();
     int count = sh.count;
+    Online low = {sum > 0.f ? bound : -INFINITY, sum};
 
     if (count > CAP) {
         // the k-th key by its bytes, most significant first; `need` counts down to the number of its ties that belong to the k
@@ -181,7 +320,7 @@ __global__ __launch_bounds__(NT == 64 ? 256 : NT) void topk_rows(const T *__rest
             for (int h = tid; h < 256; h += NT) sh.hist[h] = 0;
             group_sync<NT>();
             const unsigned high = shift == 24 ? 0u : ~0u << (shift + 8);
-            scan_row<T, NT>(row, V, tid, [&](const auto &a, int) {
+            row.each(tid, false, [&](const auto &a, int) {
                 for (const float f : a) {
                     const unsigned n = (unsigned)key_of(f) ^ 0x80000000u;
                     if ((n & high) == prefix) atomicAdd(&sh.hist[(n >> shift) & 255], 1);
@@ -190,16 +329,16 @@ __global__ __launch_bounds__(NT == 64 ? 256 : NT) void topk_rows(const T *__rest
             group_sync<NT>();
             if (tid < 64) {
                 // lane l holds bins 4 l .. 4 l + 3; `above` = elements in the bins of the lanes behind it
-                int h[4], sum = 0;
+                int h[4], all = 0;
 #pragma unroll
-                for (int q = 0; q < 4; ++q) h[q] = sh.hist[4 * tid + q], sum += h[q];
-                int above = 0, run = sum;
+                for (int q = 0; q < 4; ++q) h[q] = sh.hist[4 * tid + q], all += h[q];
+                int run = all;
 #pragma unroll
                 for (int d = 1; d < 64; d <<= 1) {
                     const int o = __shfl_down(run, d, 64);
                     if (tid + d < 64) run += o;
                 }
-                above = run - sum;
+                int above = run - all;
 #pragma unroll
                 for (int q = 3; q >= 0; --q) {
                     if (above < need && above + h[q] >= need) sh.bin = 4 * tid + q, sh.need = need - above, sh.ties = h[q];
@@ -211,28 +350,28 @@ __global__ __launch_bounds__(NT == 64 ? 256 : NT) void topk_rows(const T *__rest
             need = sh.need;
             group_sync<NT>();
         }
-        bound = (int)(prefix ^ 0x80000000u);
+        const int kth = (int)(prefix ^ 0x80000000u);
         const int ties = sh.ties;
         if (tid == 0) sh.count = 0;
         group_sync<NT>();
         low = {-INFINITY, 0.f};
-        scan_row<T, NT>(row, V, tid, [&](const auto &a, int i0) {
+        row.each(tid, false, [&](const auto &a, int i0) {
             constexpr int N = sizeof(a) / sizeof(float);
             float out[N];
 #pragma unroll
             for (int i = 0; i < N; ++i) {
                 const int n = key_of(a[i]);
-                out[i] = n < bound ? a[i] : -INFINITY;
-                if (n > bound) {
+                out[i] = n < kth ? a[i] : -INFINITY;
+                if (n > kth) {
                     const int at = atomicAdd(&sh.count, 1);          // k - need of them
-                    sh.key[at] = n, sh.idx[at] = i0 + i;
+                    sh.entry[at] = entry_of(n, i0 + i);
                 }
             }
             online_fold(low, out, c2);
         });
         for (int base = 0, taken = 0; taken < need; base += NT) {    // the first `need` ties in index order; there are that many
             const int i = base + tid;
-            const bool tie = i < V && key_of(VecIO<T>::load1(row + i)) == bound;
+            const bool tie = i < V && key_of(VecIO<T>::load1(row.row + i)) == kth;
             const unsigned long long vote = __ballot(tie);
             int at = taken + __popcll(vote & ((1ull << (tid & 63)) - 1)), all = __popcll(vote);
             if constexpr (NT > 64) {
@@ -245,11 +384,11 @@ __global__ __launch_bounds__(NT == 64 ? 256 : NT) void topk_rows(const T *__rest
                 }
                 __syncthreads();
             }
-            if (tie && at < need) sh.key[k - need + at] = bound, sh.idx[k - need + at] = i;
+            if (tie && at < need) sh.entry[k - need + at] = entry_of(kth, i);
             taken += all;
         }
         if (tid == 0 && ties > need) {
-            const Online t = {of_key(bound), (float)(ties - need)};
+            const Online t = {of_key(kth), (float)(ties - need)};
             low = online_merge(low, t, c2);
         }
         count = k;
@@ -257,23 +396,58 @@ __global__ __launch_bounds__(NT == 64 ? 256 : NT) void topk_rows(const T *__rest
     }
 
     for (int c = tid; c < count; c += NT) {
-        const int n = sh.key[c], i = sh.idx[c];
+        const unsigned long long e = sh.entry[c];
         int rank = 0;
-        for (int o = 0; o < count; ++o) rank += sh.key[o] > n || (sh.key[o] == n && sh.idx[o] < i);
+#pragma unroll 8
+        for (int o = 0; o < count; ++o) rank += sh.entry[o] > e;
+        const int n = entry_key(e);
         if (rank < k) {
             VecIO<T>::store1(values + (size_t)r * k + rank, of_key(n));
-            index[(size_t)r * k + rank] = i;
+            index[(size_t)r * k + rank] = entry_idx(e);
+            if (rank == k - 1) sh.last = e;           // the last one that is taken
         } else {
             sh.left[rank - k] = of_key(n);           // by rank: the order of the sum does not hang on the order of arrival
         }
     }
     group_sync<NT>();
+    const unsigned long long last = sh.last;
     for (int c = tid; c < count - k; c += NT) {
         const float left[1] = {sh.left[c]};
         online_fold(low, left, c2);
     }
     low = online_group<NT>(low, sh.tmp, tid, c2);
+    if (low.s < 0x1p-64f && k < V) {                  // what is left lies far below the bound (or is -inf): relative to its own maximum
+        low = {-INFINITY, 0.f};
+        row.each(tid, false, [&](const auto &a, int i0) {
+            constexpr int N = sizeof(a) / sizeof(float);
+            float out[N];
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                out[i] = entry_of(key_of(a[i]), i0 + i) < last ? a[i] : -INFINITY;
+            }
+            online_fold(low, out, c2);
+        });
+        low = online_group<NT>(low, sh.tmp, tid, c2);
+    }
     if (tid == 0) rest[r] = low.s > 0.f || low.s != low.s ? low.m + tau * logf(low.s) : -INFINITY;
+}
+
+// Threads and registers by the row's bytes: a wave per row up to 8 KB (its 64 group maxima serve k <= 32), else a workgroup whose registers hold the row.
+template <typename T>
+int rows_launch(const T *x, T *values, int32_t *index, float *rest, long rows, int V, int k, float tau, float c2, hipStream_t st) {
+    if (rows > kMaxBlocks / 4) return SD_E_SHAPE;     // workgroups of up to 1024 threads
+    const long bytes = (long)V * (long)sizeof(T);
+#define SD_ROWS(NT, NV)                                                                                                                          \
+    hipLaunchKernelGGL((topk_rows<T, NT, NV>), dim3((unsigned)(NT == 64 ? (rows + 3) / 4 : rows)), dim3(NT == 64 ? 256 : NT), 0, st, x, values, index, rest, rows, \
+                       V, k, tau, c2)
+    if (k <= 32 && bytes <= 2048) SD_ROWS(64, 2);
+    else if (k <= 32 && bytes <= 8192) SD_ROWS(64, 8);
+    else if (bytes <= 16384) SD_ROWS(256, 4);
+    else if (bytes <= 65536) SD_ROWS(256, 16);
+    else if (bytes <= 131072) SD_ROWS(512, 16);
+    else SD_ROWS(1024, 16);
+#undef SD_ROWS
+    return (int)hipGetLastError();
 }
 
 template <typename T>
@@ -281,17 +455,20 @@ int select_launch(const void *x, void *values, int32_t *index, float *rest, long
     const T *xi = static_cast<const T *>(x);
     T *vo = static_cast<T *>(values);
     const float c2 = kLog2e / tau;
-    if (P == 1) {
-        if (B > kMaxBlocks) return SD_E_SHAPE;
-        if (C <= 2048 && k <= 32) {
-            hipLaunchKernelGGL((topk_rows<T, 64>), dim3((unsigned)((B + 3) / 4)), dim3(256), 0, st, xi, vo, index, rest, B, C, k, tau, c2);
-        } else {
-            hipLaunchKernelGGL((topk_rows<T, 256>), dim3((unsigned)B), dim3(256), 0, st, xi, vo, index, rest, B, C, k, tau, c2);
-        }
-        return (int)hipGetLastError();
-    }
+    if (P == 1) return rows_launch<T>(xi, vo, index, rest, B, C, k, tau, c2, st);
     const long per = (P + 255) / 256;
     if (per > kMaxBlocks / B) return SD_E_SHAPE;
+    if (C <= 240 && (P + 63) / 64 <= kMaxBlocks / B) {                          // a column of at most 240 keys: 60 KB of LDS
+        const long waves = (P + 63) / 64;
+        const size_t lds = (size_t)((C + 7) / 8) * 8 * 256;
+#define SD_COLUMNS(NG) hipLaunchKernelGGL((topk_planes_lds<T, NG>), dim3((unsigned)(waves * B)), dim3(64), lds, st, xi, vo, index, rest, C, P, (int)waves, k, tau, c2)
+        if (C <= 32) SD_COLUMNS(4);
+        else if (C <= 64) SD_COLUMNS(8);
+        else if (C <= 160) SD_COLUMNS(20);
+        else SD_COLUMNS(32);
+#undef SD_COLUMNS
+        return (int)hipGetLastError();
+    }
     const dim3 grid((unsigned)(per * B)), block(256);
 #define SD_PLANES(K) hipLaunchKernelGGL((topk_planes<T, K>), grid, block, 0, st, xi, vo, index, rest, C, P, (int)per, k, tau, c2)
     if (k <= 4) SD_PLANES(4);
