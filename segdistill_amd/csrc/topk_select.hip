@@ -82,80 +82,112 @@ __global__ __launch_bounds__(256) void topk_planes(const T *__restrict__ x, T *_
     rest[(size_t)b * P + p] = low.s > 0.f || low.s != low.s ? low.m + tau * logf(low.s) : -INFINITY;
 }
 
-// The same with the pixels' classes parked in LDS (a column per lane, 64 pixels per wave) when they fit: the register list costs K steps per class; here
-// the maxima of groups of eight classes sit in registers, and each of the k rounds takes the largest of them and scans its group again -- ng + 8 steps per
-// entry instead of K per class.  A taken class is overwritten by kNoKey, so the sum of the rest is one more pass over the column with its maximum known.
-// The scans go up and compare strictly: the lowest class wins a tie.
+// The same with the pixels' classes parked in LDS when they fit: the register list costs K steps per class; here the maxima of groups of eight classes sit in
+// registers, and each of the k rounds takes the largest of them and scans its group again -- NG + 8 steps per entry instead of K per class.  Two lanes
+// share a pixel, each with half of its classes in a column of its own, and exchange their best: 64 pixels per column pair leave one wave per SIMD at 150
+// classes, 32 leave two (45 -> 37 us at [8, 150, 128, 128]; four lanes per pixel: 46 us, each lane scans a group per entry).  A taken class is
+// overwritten by kNoKey, so the sum of the rest is one more pass over the columns with its maximum known.  The scans go up and compare strictly, and the
+// lower half wins a tie: the lowest class does.
 template <typename T, int NG>
 __global__ __launch_bounds__(64) void topk_planes_lds(const T *__restrict__ x, T *__restrict__ values, int *__restrict__ index, float *__restrict__ rest, int C,
-                                                      long P, int blocks_per_image, int k, float tau, float c2) {
-    extern __shared__ int column[];
-    int *mine = column + threadIdx.x;                 // class c at mine[64 c]; rows up to a multiple of eight
-    const long b = blockIdx.x / blocks_per_image;
-    const long p = (long)(blockIdx.x - b * blocks_per_image) * 64 + threadIdx.x;
-    const bool live = p < P;
-    const T *px = x + (size_t)b * C * P + (live ? p : P - 1);
-    // a wave's column leaves room for one wave per SIMD or two: all its loads go out before the first is used
-    float f[NG * 8];
+                                                      long P, int per, long tiles, int k, float tau, float c2) {
+    constexpr int CL = 8 * NG;
+    __shared__ int column[64 * CL];
+    // half = classes per lane; for an odd count the upper half starts with the lower one's last class, which it leaves out
+    const int half = (C + 1) / 2, upper = threadIdx.x >> 5, first = upper ? C - half : 0;
+    const bool doubled = upper && (C & 1);
+    int *mine = column + threadIdx.x;                 // class first + c at mine[64 c]
+    float f[CL];
+    // the next tile's loads are on their way while this one is searched
+    auto fetch = [&](long tile) {
+        const long b = tile / per, p = (tile - b * per) * 32 + (threadIdx.x & 31);
+        const T *px = x + (size_t)b * C * P + (size_t)first * P + min(p, P - 1);
+        long step = P;
+        int n = half;
+        asm volatile("" : "+s"(step), "+s"(n));       // offsets kept over the loop would not fit the registers: formed anew
 #pragma unroll
-    for (int g = 0; g < NG; g += 4)
-        if (g * 8 < C) {
+        for (int g = 0; g < NG; ++g)
+            if (8 * g < n) {
 #pragma unroll
-            for (int u = 0; u < 32; ++u) f[g * 8 + u] = VecIO<T>::load1(px + (size_t)min(g * 8 + u, C - 1) * P);
-        }
-    int top[NG];
+                for (int u = 0; u < 8; ++u) {
+                    f[8 * g + u] = VecIO<T>::load1(px);
+                    px += 8 * g + u + 1 < n ? step : 0;
+                }
+            }
+    };
+    fetch(blockIdx.x);
+    for (long tile = blockIdx.x; tile < tiles; tile += gridDim.x) {
+        const long b = tile / per, p = (tile - b * per) * 32 + (threadIdx.x & 31);
+        const bool writes = !upper && p < P;
+        int top[NG];
 #pragma unroll
-    for (int g = 0; g < NG; ++g) {
-        top[g] = kNoKey;
-        if (g * 8 < C) {                              // whole groups
+        for (int g = 0; g < NG; ++g) {
+            top[g] = kNoKey;
+            if (8 * g < half) {
 #pragma unroll
-            for (int u = 0; u < 8; ++u) {
-                const int c = g * 8 + u, n = c < C ? key_of(f[c]) : kNoKey;
-                mine[64 * c] = n;
-                top[g] = max(top[g], n);
+                for (int u = 0; u < 8; ++u) {
+                    int n = key_of(f[8 * g + u]);
+                    if (8 * g + u >= half || (g + u == 0 && doubled)) n = kNoKey;
+                    mine[64 * (8 * g + u)] = n;
+                    top[g] = max(top[g], n);
+                }
             }
         }
+        if (tile + gridDim.x < tiles) fetch(tile + gridDim.x);
+        for (int j = 0; j < k; ++j) {
+            int best = top[0], bg = 0;
+#pragma unroll
+            for (int g = 1; g < NG; ++g) {
+                const bool gt = top[g] > best;
+                best = gt ? top[g] : best;
+                bg = gt ? g : bg;
+            }
+            int *group = mine + 512 * bg;
+            int at = 8, next = kNoKey;
+#pragma unroll
+            for (int u = 0; u < 8; ++u) {
+                const int n = group[64 * u];
+                const bool here = n == best && at == 8;
+                at = here ? u : at;
+                next = here ? next : max(next, n);
+            }
+            const int own = first + 8 * bg + at, other = __shfl_xor(best, 32, 64), other_cls = __shfl_xor(own, 32, 64);
+            const bool mine_wins = best > other || (best == other && !upper);       // k <= C: the winner is a class, never padding
+            if (mine_wins) {
+                group[64 * at] = kNoKey;
+#pragma unroll
+                for (int g = 0; g < NG; ++g) top[g] = g == bg ? next : top[g];
+            }
+            if (writes) {
+                const size_t o = ((size_t)b * k + j) * P + p;
+                VecIO<T>::store1(values + o, of_key(mine_wins ? best : other));
+                index[o] = mine_wins ? own : other_cls;
+            }
+        }
+        int m = kMinusInfKey;
+#pragma unroll
+        for (int g = 0; g < NG; ++g) m = max(m, top[g]);
+        m = max(m, __shfl_xor(m, 32, 64));
+        const float ref = finite_ref(of_key(m));
+        float s = 0.f;
+#pragma unroll
+        for (int g = 0; g < NG; ++g)
+            if (8 * g < half) {
+#pragma unroll
+                for (int u = 0; u < 8; ++u) s += ex2((of_key(max(mine[64 * (8 * g + u)], kMinusInfKey)) - ref) * c2);      // taken: 2^-inf
+            }
+        s += __shfl_xor(s, 32, 64);
+        if (writes) rest[(size_t)b * P + p] = s > 0.f || s != s ? ref + tau * logf(s) : -INFINITY;
     }
-    for (int j = 0; j < k; ++j) {
-        int best = top[0], bg = 0;
-#pragma unroll
-        for (int g = 1; g < NG; ++g) {
-            const bool gt = top[g] > best;
-            best = gt ? top[g] : best;
-            bg = gt ? g : bg;
-        }
-        int *group = mine + 512 * bg;
-        int at = -1, next = kNoKey;
-#pragma unroll
-        for (int u = 0; u < 8; ++u) {
-            const int n = group[64 * u];
-            const bool here = n == best && at < 0;
-            at = here ? u : at;
-            next = here ? next : max(next, n);
-        }
-        group[64 * at] = kNoKey;
-#pragma unroll
-        for (int g = 0; g < NG; ++g) top[g] = g == bg ? next : top[g];
-        if (live) {
-            const size_t o = ((size_t)b * k + j) * P + p;
-            VecIO<T>::store1(values + o, of_key(best));
-            index[o] = 8 * bg + at;
-        }
-    }
-    int m = kMinusInfKey;
-#pragma unroll
-    for (int g = 0; g < NG; ++g) m = max(m, top[g]);
-    const float ref = finite_ref(of_key(m));
-    float s = 0.f;
-    for (int c = 0; c < C; c += 8) {
-#pragma unroll
-        for (int u = 0; u < 8; ++u) {
-            const int n = mine[64 * (c + u)];
-            const float e = ex2((of_key(n) - ref) * c2);
-            s += n > kMinusInfKey ? e : 0.f;
-        }
-    }
-    if (live) rest[(size_t)b * P + p] = s > 0.f || s != s ? ref + tau * logf(s) : -INFINITY;
+}
+
+template <typename T, int NG>
+int planes_lds_launch(const T *x, T *values, int32_t *index, float *rest, long B, int C, long P, int k, float tau, float c2, hipStream_t st) {
+    const long per = (P + 31) / 32, tiles = per * B;
+    const int lds = 64 * 8 * NG * 4, resident = lds < 10240 ? 16 : 160 * 1024 / lds;      // waves per CU
+    const dim3 grid((unsigned)(tiles < 256 * resident ? tiles : 256 * resident));
+    hipLaunchKernelGGL((topk_planes_lds<T, NG>), grid, dim3(64), 0, st, x, values, index, rest, C, P, (int)per, tiles, k, tau, c2);
+    return (int)hipGetLastError();
 }
 
 // ---- contiguous rows --------------------------------------------------------------------------------------------------------------------------
@@ -458,17 +490,13 @@ int select_launch(const void *x, void *values, int32_t *index, float *rest, long
     if (P == 1) return rows_launch<T>(xi, vo, index, rest, B, C, k, tau, c2, st);
     const long per = (P + 255) / 256;
     if (per > kMaxBlocks / B) return SD_E_SHAPE;
-    if (C <= 240 && (P + 63) / 64 <= kMaxBlocks / B) {                          // a column of at most 240 keys: 60 KB of LDS
-        const long waves = (P + 63) / 64;
-        const size_t lds = (size_t)((C + 7) / 8) * 8 * 256;
-#define SD_COLUMNS(NG) hipLaunchKernelGGL((topk_planes_lds<T, NG>), dim3((unsigned)(waves * B)), dim3(64), lds, st, xi, vo, index, rest, C, P, (int)waves, k, tau, c2)
-        if (C <= 32) SD_COLUMNS(4);
-        else if (C <= 64) SD_COLUMNS(8);
-        else if (C <= 160) SD_COLUMNS(20);
-        else SD_COLUMNS(32);
+#define SD_COLUMNS(NG) planes_lds_launch<T, NG>(xi, vo, index, rest, B, C, P, k, tau, c2, st)
+    if (C <= 16) return SD_COLUMNS(1);
+    if (C <= 32) return SD_COLUMNS(2);
+    if (C <= 64) return SD_COLUMNS(4);
+    if (C <= 160) return SD_COLUMNS(10);
+    if (C <= 256) return SD_COLUMNS(16);
 #undef SD_COLUMNS
-        return (int)hipGetLastError();
-    }
     const dim3 grid((unsigned)(per * B)), block(256);
 #define SD_PLANES(K) hipLaunchKernelGGL((topk_planes<T, K>), grid, block, 0, st, xi, vo, index, rest, C, P, (int)per, k, tau, c2)
     if (k <= 4) SD_PLANES(4);
