@@ -191,7 +191,7 @@ int planes_lds_launch(const T *x, T *values, int32_t *index, float *rest, long B
 }
 
 // ---- contiguous rows --------------------------------------------------------------------------------------------------------------------------
-// NT threads per row, the row in their registers: NV 16-byte vectors each (a longer row comes by in tiles, and is read a second time).
+// NT threads per row, the row in their registers: NV 16-byte vectors each (a longer row is read twice).
 // 1: group maxima -- each of up to 256 groups of threads takes the largest of its elements.  The k-th largest of these maxima bounds the row's k-th
 // largest value from below (k different elements reach it); one wave finds it by bisection of the ordered keys, 20 bits of them: a lower bound stays
 // one.  2: elements that reach the bound -- about k of them unless the row is adverse -- go to a list in LDS, the others into the rest's sum, taken
@@ -199,60 +199,50 @@ int planes_lds_launch(const T *x, T *values, int32_t *index, float *rest, long B
 // A row with more than CAP elements at the bound (constant rows, many ties) takes the k-th key exactly, by four histograms of its bytes; a rest that
 // lies so far below the bound that its sum loses digits is summed again relative to its own maximum.
 template <typename T, int NT, int NV>
-struct RowTile {
+struct Row {
     static constexpr int N = VecIO<T>::N;
     typedef typename VecIO<T>::raw_t raw_t;
     const T *row;
     int V, head, nvec, tail;
-    raw_t reg[NV];
 
-    __device__ __forceinline__ RowTile(const T *r, int v) : row(r), V(v) {
+    __device__ __forceinline__ Row(const T *r, int v) : row(r), V(v) {
         head = row_head(r, v);
         nvec = (v - head) / N;
         tail = head + nvec * N;
     }
-    __device__ __forceinline__ int tiles() const { return nvec > NT * NV ? (nvec + NT * NV - 1) / (NT * NV) : 1; }
-    __device__ __forceinline__ void load(int tile, int tid) {
-        const raw_t *v = reinterpret_cast<const raw_t *>(row + head) + (long)tile * NT * NV;
-        const int n = nvec - tile * NT * NV;
-#pragma unroll
-        for (int u = 0; u < NV; ++u)
-            if (tid + u * NT < n) reg[u] = __builtin_nontemporal_load(v + tid + u * NT);
-    }
-    __device__ __forceinline__ void unpack(int u, float (&a)[N]) const {
+    __device__ __forceinline__ bool held() const { return nvec <= NT * NV; }
+    __device__ __forceinline__ raw_t vec(int i) const { return __builtin_nontemporal_load(reinterpret_cast<const raw_t *>(row + head) + i); }
+    static __device__ __forceinline__ void unpack(raw_t r, float (&a)[N]) {
         if constexpr (N == 4) {
 #pragma unroll
-            for (int q = 0; q < 4; ++q) a[q] = reg[u][q];
+            for (int q = 0; q < 4; ++q) a[q] = r[q];
         } else {
 #pragma unroll
-            for (int q = 0; q < 4; ++q) a[2 * q] = __uint_as_float((unsigned)reg[u][q] << 16), a[2 * q + 1] = __uint_as_float((unsigned)reg[u][q] & 0xffff0000u);
+            for (int q = 0; q < 4; ++q) a[2 * q] = __uint_as_float((unsigned)r[q] << 16), a[2 * q + 1] = __uint_as_float((unsigned)r[q] & 0xffff0000u);
         }
     }
-    // f(values, first index) for every element of the row that is this thread's; one tile: from the registers that hold it
+    // f(values, first index): the elements before and behind the vectors
     template <typename F>
-    __device__ __forceinline__ void each(int tid, bool reload, F f) {
+    __device__ __forceinline__ void ends(int tid, F f) const {
         if (tid < head) {
             const float one[1] = {VecIO<T>::load1(row + tid)};
             f(one, tid);
-        }
-        const int nt = tiles();
-        for (int tile = 0; tile < nt; ++tile) {
-            if (reload || nt > 1) load(tile, tid);
-            const int n = nvec - tile * NT * NV, first = head + tile * NT * NV * N;
-#pragma unroll
-            for (int u = 0; u < NV; ++u) {
-                if (u * NT >= n) break;
-                if (tid + u * NT < n) {
-                    float a[N];
-                    unpack(u, a);
-                    f(a, first + (tid + u * NT) * N);
-                }
-            }
         }
         if (tail + tid < V) {
             const float one[1] = {VecIO<T>::load1(row + tail + tid)};
             f(one, tail + tid);
         }
+    }
+    // ... and every element of the row that is this thread's, from memory
+    template <typename F>
+    __device__ __forceinline__ void stream(int tid, F f) const {
+#pragma unroll 1
+        for (int i = tid; i < nvec; i += NT) {
+            float a[N];
+            unpack(vec(i), a);
+            f(a, head + i * N);
+        }
+        ends(tid, f);
     }
 };
 
@@ -261,40 +251,138 @@ struct SelectShared {
     static constexpr int CAP = NT == 64 ? 256 : 1024, GROUPS = NT < 256 ? NT : 256;
     float max_of[GROUPS];
     unsigned long long entry[CAP];                    // key above, ~index below: descending keys, ascending indices
-    float left[CAP];
+    float left[CAP], sum[NT / 64];
     Online tmp[NT / 64];
     int hist[256];
     unsigned long long last;
-    int count, bin, need, ties, wave_ties[NT / 64];
+    int count, odd, bin, need, ties, wave_ties[NT / 64];
     float bound;
 };
-
 __device__ __forceinline__ unsigned long long entry_of(int key, int idx) { return ((unsigned long long)((unsigned)key ^ 0x80000000u) << 32) | (unsigned)~idx; }
 __device__ __forceinline__ int entry_key(unsigned long long e) { return (int)((unsigned)(e >> 32) ^ 0x80000000u); }
 __device__ __forceinline__ int entry_idx(unsigned long long e) { return (int)~(unsigned)e; }
 
+// The exact way for a row that the bound does not serve: the k-th key by its bytes, most significant first, then everything above it and the first of its
+// ties.  The k entries are in sh.entry on return; the sum of the others comes back per thread.
 template <typename T, int NT, int NV>
-__global__ __launch_bounds__(NT == 64 ? 256 : NT) void topk_rows(const T *__restrict__ x, T *__restrict__ values, int *__restrict__ index,
-                                                                 float *__restrict__ rest, long rows, int V, int k, float tau, float c2) {
+__device__ __forceinline__ Online exact_entries(const Row<T, NT, NV> &row, SelectShared<NT> &sh, int tid, int k, float c2) {
+    unsigned prefix = 0;
+    int need = k;                                     // counts down to the number of the k-th key's ties that belong to the k
+    for (int shift = 24; shift >= 0; shift -= 8) {
+        for (int h = tid; h < 256; h += NT) sh.hist[h] = 0;
+        group_sync<NT>();
+        const unsigned high = shift == 24 ? 0u : ~0u << (shift + 8);
+        row.stream(tid, [&](const auto &a, int) {
+            for (const float f : a) {
+                const unsigned n = (unsigned)key_of(f) ^ 0x80000000u;
+                if ((n & high) == prefix) atomicAdd(&sh.hist[(n >> shift) & 255], 1);
+            }
+        });
+        group_sync<NT>();
+        if (tid < 64) {
+            // lane l holds bins 4 l .. 4 l + 3; `above` = elements in the bins of the lanes behind it
+            int h[4], all = 0;
+#pragma unroll
+            for (int q = 0; q < 4; ++q) h[q] = sh.hist[4 * tid + q], all += h[q];
+            int run = all;
+#pragma unroll
+            for (int d = 1; d < 64; d <<= 1) {
+                const int o = __shfl_down(run, d, 64);
+                if (tid + d < 64) run += o;
+            }
+            int above = run - all;
+#pragma unroll
+            for (int q = 3; q >= 0; --q) {
+                if (above < need && above + h[q] >= need) sh.bin = 4 * tid + q, sh.need = need - above, sh.ties = h[q];
+                above += h[q];
+            }
+        }
+        group_sync<NT>();
+        prefix |= (unsigned)sh.bin << shift;
+        need = sh.need;
+        group_sync<NT>();
+    }
+    const int kth = (int)(prefix ^ 0x80000000u), ties = sh.ties;
+    if (tid == 0) sh.count = 0;
+    group_sync<NT>();
+    Online low = {-INFINITY, 0.f};
+    row.stream(tid, [&](const auto &a, int i0) {
+        constexpr int N = sizeof(a) / sizeof(float);
+        float out[N];
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const int n = key_of(a[i]);
+            out[i] = n < kth ? a[i] : -INFINITY;
+            if (n > kth) sh.entry[atomicAdd(&sh.count, 1)] = entry_of(n, i0 + i);          // k - need of them
+        }
+        online_fold(low, out, c2);
+    });
+    for (int base = 0, taken = 0; taken < need; base += NT) {        // the first `need` ties in index order; there are that many
+        const int i = base + tid;
+        const bool tie = i < row.V && key_of(VecIO<T>::load1(row.row + i)) == kth;
+        const unsigned long long vote = __ballot(tie);
+        int at = taken + __popcll(vote & ((1ull << (tid & 63)) - 1)), all = __popcll(vote);
+        if constexpr (NT > 64) {
+            if ((tid & 63) == 0) sh.wave_ties[tid >> 6] = all;
+            __syncthreads();
+            all = 0;
+            for (int w = 0; w < NT / 64; ++w) {
+                if (w < (tid >> 6)) at += sh.wave_ties[w];
+                all += sh.wave_ties[w];
+            }
+            __syncthreads();
+        }
+        if (tie && at < need) sh.entry[k - need + at] = entry_of(kth, i);
+        taken += all;
+    }
+    if (tid == 0 && ties > need) {
+        const Online t = {of_key(kth), (float)(ties - need)};
+        low = online_merge(low, t, c2);
+    }
+    group_sync<NT>();
+    return low;
+}
+
+template <typename T, int NT, int NV, int WAVES>
+__global__ __launch_bounds__(NT == 64 ? 256 : NT, WAVES) void topk_rows(const T *__restrict__ x, T *__restrict__ values, int *__restrict__ index,
+                                                                        float *__restrict__ rest, long rows, int V, int k, float tau, float c2) {
     typedef SelectShared<NT> Shared;
-    constexpr int G = NT == 64 ? 4 : 1, CAP = Shared::CAP, GROUPS = Shared::GROUPS;
+    typedef Row<T, NT, NV> R;
+    constexpr int G = NT == 64 ? 4 : 1, CAP = Shared::CAP, GROUPS = Shared::GROUPS, N = R::N, SUB = NT / 64;
     __shared__ Shared shared[G];
     Shared &sh = shared[NT == 64 ? threadIdx.x >> 6 : 0];
     const int tid = NT == 64 ? threadIdx.x & 63 : threadIdx.x;
     const long r = (long)blockIdx.x * G + (NT == 64 ? threadIdx.x >> 6 : 0);
     if (r >= rows) return;                            // whole waves (NT == 64) or never (one row per workgroup)
-    RowTile<T, NT, NV> row(x + (size_t)r * V, V);
-
-    float mine = -INFINITY;                           // NaN elements drop out here: the bound only gets lower
-    row.each(tid, true, [&](const auto &a, int) {
-        for (const float f : a) mine = fmaxf(mine, f);
-    });
-    if constexpr (NT / GROUPS > 1) {
+    const R row(x + (size_t)r * V, V);
+    typename R::raw_t reg[NV];
+    if (row.held()) {
 #pragma unroll
-        for (int d = 1; d < NT / GROUPS; d <<= 1) mine = fmaxf(mine, __shfl_xor(mine, d, 64));
+        for (int u = 0; u < NV; ++u)
+            if (tid + u * NT < row.nvec) reg[u] = row.vec(tid + u * NT);
     }
+
+    // 1: group maxima and the bound.  NaN elements drop out: the bound only gets lower.
+    float mine = -INFINITY;
+    auto largest = [&](const auto &a, int) {
+        for (const float f : a) mine = fmaxf(mine, f);
+    };
+    if (row.held()) {
+#pragma unroll
+        for (int u = 0; u < NV; ++u)
+            if (tid + u * NT < row.nvec) {
+                float a[N];
+                R::unpack(reg[u], a);
+                largest(a, 0);
+            }
+        row.ends(tid, largest);
+    } else {
+        row.stream(tid, largest);
+    }
+#pragma unroll
+    for (int d = 1; d < NT / GROUPS; d <<= 1) mine = fmaxf(mine, __shfl_xor(mine, d, 64));
     if (tid % (NT / GROUPS) == 0) sh.max_of[tid / (NT / GROUPS)] = mine;
-    if (tid == 0) sh.count = 0;
+    if (tid == 0) sh.count = sh.odd = 0;
     group_sync<NT>();
     if (tid < 64) {
         unsigned u[GROUPS / 64];
@@ -308,28 +396,26 @@ __global__ __launch_bounds__(NT == 64 ? 256 : NT) void topk_rows(const T *__rest
             for (int q = 0; q < GROUPS / 64; ++q) n += __popcll(__ballot(u[q] >= trial));
             if (n >= k) low = trial;
         }
-        if (tid == 0) sh.bound = of_key((int)(low ^ 0x80000000u));        // below -inf this is a NaN: then every element is taken
+        const int key = (int)(low ^ 0x80000000u);
+        if (tid == 0) sh.bound = key <= kMinusInfKey ? -INFINITY : of_key(key);
     }
     group_sync<NT>();
-    const float bound = sh.bound;
 
-    // the sum of the elements below the bound, relative to it: 2^{x c2 - bound c2} in one rounding.  Where bound * c2 leaves the range there is no such sum;
-    // the last step below takes it then.
-    const float shift = bound * c2;
-    const bool fits = fabsf(shift) < 1e30f;
+    // 2: list and sum.  2^{x c2 - bound c2} in one rounding.  A vector without an element at the bound goes by without a look at each; a NaN that
+    // passes so shows in the sum and sends the row the exact way.  At a bound of -inf everything is listed.
+    const float bound = sh.bound, shift = bound * c2;
     float sum = 0.f;
-    row.each(tid, false, [&](const auto &a, int i0) {
-        constexpr int N = sizeof(a) / sizeof(float);
-        float e[N];
-        bool any = false;
+    auto take = [&](const auto &a, int i0) {
+        constexpr int M = sizeof(a) / sizeof(float);
+        float e[M], m = a[0];
 #pragma unroll
-        for (int i = 0; i < N; ++i) {
-            any |= !(a[i] < bound);
+        for (int i = 0; i < M; ++i) {
+            m = fmaxf(m, a[i]);
             e[i] = ex2(fmaf(a[i], c2, -shift));
         }
-        if (any) {
+        if (!(m < bound)) {
 #pragma unroll
-            for (int i = 0; i < N; ++i)
+            for (int i = 0; i < M; ++i)
                 if (!(a[i] < bound)) {
                     e[i] = 0.f;
                     const int at = atomicAdd(&sh.count, 1);
@@ -337,129 +423,81 @@ __global__ __launch_bounds__(NT == 64 ? 256 : NT) void topk_rows(const T *__rest
                 }
         }
 #pragma unroll
-        for (int i = 0; i < N; ++i) sum += e[i];
-    });
-    if (!fits) sum = 0.f;
+        for (int i = 0; i < M; ++i) sum += e[i];
+    };
+    if (row.held()) {
+#pragma unroll
+        for (int u = 0; u < NV; ++u) {
+            const int i = tid + u * NT;
+            if (i < row.nvec) {
+                float a[N];
+                R::unpack(reg[u], a);
+                take(a, row.head + i * N);
+            }
+        }
+        row.ends(tid, take);
+    } else {
+        row.stream(tid, take);
+    }
+    if (sum != sum) sh.odd = 1;                   // also where bound * c2 leaves the range
+#pragma unroll
+    for (int d = 32; d > 0; d >>= 1) sum += __shfl_xor(sum, d, 64);
+    if ((tid & 63) == 0) sh.sum[tid >> 6] = sum;
     group_sync<NT>();
     int count = sh.count;
-    Online low = {sum > 0.f ? bound : -INFINITY, sum};
-
-    if (count > CAP) {
-        // the k-th key by its bytes, most significant first; `need` counts down to the number of its ties that belong to the k
-        unsigned prefix = 0;
-        int need = k;
-        for (int shift = 24; shift >= 0; shift -= 8) {
-            for (int h = tid; h < 256; h += NT) sh.hist[h] = 0;
-            group_sync<NT>();
-            const unsigned high = shift == 24 ? 0u : ~0u << (shift + 8);
-            row.each(tid, false, [&](const auto &a, int) {
-                for (const float f : a) {
-                    const unsigned n = (unsigned)key_of(f) ^ 0x80000000u;
-                    if ((n & high) == prefix) atomicAdd(&sh.hist[(n >> shift) & 255], 1);
-                }
-            });
-            group_sync<NT>();
-            if (tid < 64) {
-                // lane l holds bins 4 l .. 4 l + 3; `above` = elements in the bins of the lanes behind it
-                int h[4], all = 0;
-#pragma unroll
-                for (int q = 0; q < 4; ++q) h[q] = sh.hist[4 * tid + q], all += h[q];
-                int run = all;
-#pragma unroll
-                for (int d = 1; d < 64; d <<= 1) {
-                    const int o = __shfl_down(run, d, 64);
-                    if (tid + d < 64) run += o;
-                }
-                int above = run - all;
-#pragma unroll
-                for (int q = 3; q >= 0; --q) {
-                    if (above < need && above + h[q] >= need) sh.bin = 4 * tid + q, sh.need = need - above, sh.ties = h[q];
-                    above += h[q];
-                }
-            }
-            group_sync<NT>();
-            prefix |= (unsigned)sh.bin << shift;
-            need = sh.need;
-            group_sync<NT>();
-        }
-        const int kth = (int)(prefix ^ 0x80000000u);
-        const int ties = sh.ties;
-        if (tid == 0) sh.count = 0;
-        group_sync<NT>();
-        low = {-INFINITY, 0.f};
-        row.each(tid, false, [&](const auto &a, int i0) {
-            constexpr int N = sizeof(a) / sizeof(float);
-            float out[N];
-#pragma unroll
-            for (int i = 0; i < N; ++i) {
-                const int n = key_of(a[i]);
-                out[i] = n < kth ? a[i] : -INFINITY;
-                if (n > kth) {
-                    const int at = atomicAdd(&sh.count, 1);          // k - need of them
-                    sh.entry[at] = entry_of(n, i0 + i);
-                }
-            }
-            online_fold(low, out, c2);
-        });
-        for (int base = 0, taken = 0; taken < need; base += NT) {    // the first `need` ties in index order; there are that many
-            const int i = base + tid;
-            const bool tie = i < V && key_of(VecIO<T>::load1(row.row + i)) == kth;
-            const unsigned long long vote = __ballot(tie);
-            int at = taken + __popcll(vote & ((1ull << (tid & 63)) - 1)), all = __popcll(vote);
-            if constexpr (NT > 64) {
-                if ((tid & 63) == 0) sh.wave_ties[tid >> 6] = all;
-                __syncthreads();
-                all = 0;
-                for (int w = 0; w < NT / 64; ++w) {
-                    if (w < (tid >> 6)) at += sh.wave_ties[w];
-                    all += sh.wave_ties[w];
-                }
-                __syncthreads();
-            }
-            if (tie && at < need) sh.entry[k - need + at] = entry_of(kth, i);
-            taken += all;
-        }
-        if (tid == 0 && ties > need) {
-            const Online t = {of_key(kth), (float)(ties - need)};
-            low = online_merge(low, t, c2);
-        }
+    const bool exact = count > CAP || sh.odd;
+    if (exact) {
+        const Online low = online_group<NT>(exact_entries(row, sh, tid, k, c2), sh.tmp, tid, c2);
+        if (tid == 0) sh.tmp[0] = low;
         count = k;
         group_sync<NT>();
     }
 
-    for (int c = tid; c < count; c += NT) {
-        const unsigned long long e = sh.entry[c];
+    // 3: SUB threads count for one entry
+    for (int c0 = 0; c0 < count; c0 += 64) {
+        const int c = c0 + tid / SUB;
+        const unsigned long long e = sh.entry[min(c, count - 1)];
         int rank = 0;
-#pragma unroll 8
-        for (int o = 0; o < count; ++o) rank += sh.entry[o] > e;
-        const int n = entry_key(e);
-        if (rank < k) {
-            VecIO<T>::store1(values + (size_t)r * k + rank, of_key(n));
-            index[(size_t)r * k + rank] = entry_idx(e);
-            if (rank == k - 1) sh.last = e;           // the last one that is taken
-        } else {
-            sh.left[rank - k] = of_key(n);           // by rank: the order of the sum does not hang on the order of arrival
+        for (int o = tid % SUB; o < count; o += SUB) rank += sh.entry[o] > e;
+#pragma unroll
+        for (int d = 1; d < SUB; d <<= 1) rank += __shfl_xor(rank, d, 64);
+        if (c < count && tid % SUB == 0) {
+            const int n = entry_key(e);
+            if (rank < k) {
+                VecIO<T>::store1(values + (size_t)r * k + rank, of_key(n));
+                index[(size_t)r * k + rank] = entry_idx(e);
+                if (rank == k - 1) sh.last = e;   // the last one that is taken
+            } else {
+                sh.left[rank - k] = of_key(n);   // by rank: the order of the sum does not hang on the order of arrival
+            }
         }
     }
     group_sync<NT>();
-    const unsigned long long last = sh.last;
-    for (int c = tid; c < count - k; c += NT) {
-        const float left[1] = {sh.left[c]};
-        online_fold(low, left, c2);
-    }
-    low = online_group<NT>(low, sh.tmp, tid, c2);
-    if (low.s < 0x1p-64f && k < V) {                  // what is left lies far below the bound (or is -inf): relative to its own maximum
-        low = {-INFINITY, 0.f};
-        row.each(tid, false, [&](const auto &a, int i0) {
-            constexpr int N = sizeof(a) / sizeof(float);
-            float out[N];
+    Online low;
+    if (exact) {
+        low = sh.tmp[0];
+    } else {
+        float total = 0.f;
+        for (int w = 0; w < SUB; ++w) total += sh.sum[w];
+        Online l = {-INFINITY, 0.f};
+        for (int c = tid & 63; c < count - k; c += 64) {
+            const float left[1] = {sh.left[c]};
+            online_fold(l, left, c2);
+        }
+        const Online b = {total > 0.f ? bound : -INFINITY, total};
+        low = count > k ? online_merge(online_group<64>(l, nullptr, 0, c2), b, c2) : b;
+        if (low.s < 0x1p-64f && k < V) {          // what is left lies far below the bound (or is -inf): relative to its own maximum
+            const unsigned long long last = sh.last;
+            low = {-INFINITY, 0.f};
+            row.stream(tid, [&](const auto &a, int i0) {
+                constexpr int M = sizeof(a) / sizeof(float);
+                float out[M];
 #pragma unroll
-            for (int i = 0; i < N; ++i) {
-                out[i] = entry_of(key_of(a[i]), i0 + i) < last ? a[i] : -INFINITY;
-            }
-            online_fold(low, out, c2);
-        });
-        low = online_group<NT>(low, sh.tmp, tid, c2);
+                for (int i = 0; i < M; ++i) out[i] = entry_of(key_of(a[i]), i0 + i) < last ? a[i] : -INFINITY;
+                online_fold(low, out, c2);
+            });
+            low = online_group<NT>(low, sh.tmp, tid, c2);
+        }
     }
     if (tid == 0) rest[r] = low.s > 0.f || low.s != low.s ? low.m + tau * logf(low.s) : -INFINITY;
 }
@@ -469,15 +507,15 @@ template <typename T>
 int rows_launch(const T *x, T *values, int32_t *index, float *rest, long rows, int V, int k, float tau, float c2, hipStream_t st) {
     if (rows > kMaxBlocks / 4) return SD_E_SHAPE;     // workgroups of up to 1024 threads
     const long bytes = (long)V * (long)sizeof(T);
-#define SD_ROWS(NT, NV)                                                                                                                          \
-    hipLaunchKernelGGL((topk_rows<T, NT, NV>), dim3((unsigned)(NT == 64 ? (rows + 3) / 4 : rows)), dim3(NT == 64 ? 256 : NT), 0, st, x, values, index, rest, rows, \
-                       V, k, tau, c2)
-    if (k <= 32 && bytes <= 2048) SD_ROWS(64, 2);
-    else if (k <= 32 && bytes <= 8192) SD_ROWS(64, 8);
-    else if (bytes <= 16384) SD_ROWS(256, 4);
-    else if (bytes <= 65536) SD_ROWS(256, 16);
-    else if (bytes <= 131072) SD_ROWS(512, 16);
-    else SD_ROWS(1024, 16);
+#define SD_ROWS(NT, NV, WAVES)                                                                                                                              \
+    hipLaunchKernelGGL((topk_rows<T, NT, NV, WAVES>), dim3((unsigned)(NT == 64 ? (rows + 3) / 4 : rows)), dim3(NT == 64 ? 256 : NT), 0, st, x, values, index, \
+                       rest, rows, V, k, tau, c2)
+    if (k <= 32 && bytes <= 2048) SD_ROWS(64, 2, 8);
+    else if (k <= 32 && bytes <= 8192) SD_ROWS(64, 8, 5);
+    else if (bytes <= 16384) SD_ROWS(256, 4, 6);
+    else if (bytes <= 65536) SD_ROWS(256, 16, 4);
+    else if (bytes <= 131072) SD_ROWS(512, 16, 4);
+    else SD_ROWS(1024, 16, 4);
 #undef SD_ROWS
     return (int)hipGetLastError();
 }
