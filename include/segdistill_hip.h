@@ -332,14 +332,15 @@ int sd_window_attn_train_bwd(const void *qkv, const float *packed, size_t packed
  *             [0, buckets) (the caller's plan has checked it)
  *   backward  dtable[b][h] = sum_{index[p] = b} dbias[h][p]: `order` lists the pairs bucket by bucket; chunk i is order[chunk_start[i] ..
  *             chunk_start[i + 1]) with at most sd_bucket_bias_chunk() pairs of ONE bucket; bucket b owns the chunks [bucket_chunk[b],
- *             bucket_chunk[b + 1]), at least one (an empty bucket: an empty one).  fp32 sums in a fixed order, the chunks of a bucket in fp64.
+ *             bucket_chunk[b + 1]), at least one (an empty bucket: an empty one).  chunk_order: the chunks in the order they are taken (any permutation; by first pair
+ *             they share cache lines).  fp32 sums in a fixed order, the chunks of a bucket in fp64.
  *             workspace: sd_bucket_bias_workspace_bytes (0 when every bucket is one chunk).
  */
 int sd_bucket_bias_chunk(void);
 size_t sd_bucket_bias_workspace_bytes(int buckets, int chunks, int heads);
 int sd_bucket_bias_fwd(const void *table, const int32_t *index, void *out, int dtype, int buckets, int heads, long pairs, void *stream);
-int sd_bucket_bias_bwd(const void *dbias, const int32_t *order, const int32_t *chunk_start, const int32_t *bucket_chunk, void *dtable, int dtype,
-                       int buckets, int chunks, int heads, long pairs, void *workspace, size_t workspace_bytes, void *stream);
+int sd_bucket_bias_bwd(const void *dbias, const int32_t *order, const int32_t *chunk_start, const int32_t *chunk_order,
+                       const int32_t *bucket_chunk, void *dtable, int dtype, int buckets, int chunks, int heads, long pairs, void *workspace, size_t workspace_bytes, void *stream);
 
 /* ---------------------------------------------------------------------------
  * Distillation from a teacher's top logits (csrc/topk_select.hip, csrc/topk_kl.hip): the teacher's part of the pixel-wise criterion

@@ -64,7 +64,7 @@ SIGNATURES = {
     'sd_bucket_bias_chunk': (_i, []),
     'sd_bucket_bias_workspace_bytes': (_sz, [_i, _i, _i]),
     'sd_bucket_bias_fwd': (_i, [_vp, _vp, _vp, _i, _i, _i, C.c_long, _vp]),
-    'sd_bucket_bias_bwd': (_i, [_vp] * 5 + [_i, _i, _i, _i, C.c_long, _vp, _sz, _vp]),
+    'sd_bucket_bias_bwd': (_i, [_vp] * 6 + [_i, _i, _i, _i, C.c_long, _vp, _sz, _vp]),
     'sd_topk_max_entries': (_i, []),
     'sd_topk_max_classes': (_i, []),
     'sd_topk_select': (_i, [_vp, _vp, _vp, _vp, _i, C.c_long, _i, C.c_long, _i, _f, _vp]),

@@ -5,7 +5,9 @@
 //
 // Both are memory bound: the H Nq Nk bias elements are written once forward and read once backward.  The gradient is a gather, not a scatter: the
 // plan holds the pairs ordered by bucket (ascending within one), cut into chunks of at most 512; a wave sums a chunk, a second pass a bucket's
-// chunks, both in a fixed order, without atomics.  The ordered list is read once for eight heads.
+// chunks, both in a fixed order, without atomics.  The ordered list is read once for eight heads.  Buckets of single distances are diagonals of the map, a
+// pair per row, and neighbouring ones lie in the same cache lines: the chunks are taken by their first pair, on one chiplet after the other, so that those
+// that share lines run together (2048 x 2048 pairs, 32 buckets, 16 heads, fp32: 394 -> 310 MB fetched, 86 -> 62 us).
 #include <hip/hip_runtime.h>
 
 #include "cgd_device.h"
@@ -36,25 +38,39 @@ __global__ __launch_bounds__(256) void bucket_bias_fwd(const T *__restrict__ tab
 // one wave per (chunk, eight heads); DIRECT: chunk i is all of bucket i, the sums are the gradient itself
 template <typename T, bool DIRECT>
 __global__ __launch_bounds__(256) void bucket_bias_chunks(const T *__restrict__ dbias, const int *__restrict__ order, const int *__restrict__ chunk_start,
-                                                          float *__restrict__ part, T *__restrict__ dtable, int chunks, int H, long NP) {
+                                                          const int *__restrict__ chunk_order, float *__restrict__ part, T *__restrict__ dtable, int chunks, int H, long NP) {
     const int lane = threadIdx.x & 63;
-    const int c = __builtin_amdgcn_readfirstlane((int)blockIdx.x * 4 + (int)(threadIdx.x >> 6));
-    if (c >= chunks) return;
+    const int n = gridDim.x, id = blockIdx.x, rem = n % 8, xcd = id % 8;              // consecutive logical workgroups share a chiplet
+    const int wg = (xcd < rem ? xcd * (n / 8 + 1) : rem * (n / 8 + 1) + (xcd - rem) * (n / 8)) + id / 8;
+    const int nth = __builtin_amdgcn_readfirstlane(wg * 4 + (int)(threadIdx.x >> 6));
+    if (nth >= chunks) return;
+    const int c = chunk_order[nth];
     const int lo = chunk_start[c], hi = chunk_start[c + 1];
-    int at[kChunk / 64];
-#pragma unroll
-    for (int u = 0; u < kChunk / 64; ++u) at[u] = lo + u * 64 + lane < hi ? order[lo + u * 64 + lane] : -1;
     const int h0 = blockIdx.y * kBiasHeads, h1 = min(H, h0 + kBiasHeads);
+    auto put = [&](int h, float s) {
+        if constexpr (DIRECT) VecIO<T>::store1(dtable + (size_t)c * H + h, s);
+        else part[(size_t)c * H + h] = s;
+    };
+    if (lo == hi) {                                   // an empty bucket
+        for (int h = h0 + lane; h < h1; h += 64) put(h, 0.f);
+        return;
+    }
+    int at[kChunk / 64];
+    bool in[kChunk / 64];
+#pragma unroll
+    for (int u = 0; u < kChunk / 64; ++u) {
+        in[u] = lo + u * 64 + lane < hi;
+        at[u] = order[min(lo + u * 64 + lane, hi - 1)];               // lanes behind the end load the last pair again: no branch around a load
+    }
     for (int h = h0; h < h1; ++h) {
         const T *d = dbias + (size_t)h * NP;
-        float s = 0.f;
+        float v[kChunk / 64], s = 0.f;
 #pragma unroll
-        for (int u = 0; u < kChunk / 64; ++u) s += at[u] >= 0 ? VecIO<T>::load1(d + at[u]) : 0.f;
+        for (int u = 0; u < kChunk / 64; ++u) v[u] = VecIO<T>::load1(d + at[u]);
+#pragma unroll
+        for (int u = 0; u < kChunk / 64; ++u) s += in[u] ? v[u] : 0.f;
         s = wave_sum(s);
-        if (lane == 0) {
-            if constexpr (DIRECT) VecIO<T>::store1(dtable + (size_t)c * H + h, s);
-            else part[(size_t)c * H + h] = s;
-        }
+        if (lane == 0) put(h, s);
     }
 }
 
@@ -63,6 +79,7 @@ template <typename T>
 __global__ __launch_bounds__(64) void bucket_bias_join(const float *__restrict__ part, const int *__restrict__ bucket_chunk, T *__restrict__ dtable, int H) {
     const int b = blockIdx.x, h = blockIdx.y;
     double s = 0;
+#pragma unroll 8
     for (int c = bucket_chunk[b] + threadIdx.x; c < bucket_chunk[b + 1]; c += 64) s += (double)part[(size_t)c * H + h];
 #pragma unroll
     for (int d = 32; d > 0; d >>= 1) s += __shfl_xor(s, d, 64);
@@ -82,15 +99,16 @@ int fwd_launch(const void *table, const int32_t *index, void *out, int H, long N
 }
 
 template <typename T>
-int bwd_launch(const void *dbias, const int32_t *order, const int32_t *chunk_start, const int32_t *bucket_chunk, void *dtable, int nb, int chunks, int H, long NP,
+int bwd_launch(const void *dbias, const int32_t *order, const int32_t *chunk_start, const int32_t *chunk_order, const int32_t *bucket_chunk,
+               void *dtable, int nb, int chunks, int H, long NP,
                float *part, hipStream_t st) {
     const T *d = static_cast<const T *>(dbias);
     T *o = static_cast<T *>(dtable);
     const dim3 grid((unsigned)((chunks + 3) / 4), (unsigned)((H + kBiasHeads - 1) / kBiasHeads));
     if (chunks == nb) {
-        hipLaunchKernelGGL((bucket_bias_chunks<T, true>), grid, dim3(256), 0, st, d, order, chunk_start, part, o, chunks, H, NP);
+        hipLaunchKernelGGL((bucket_bias_chunks<T, true>), grid, dim3(256), 0, st, d, order, chunk_start, chunk_order, part, o, chunks, H, NP);
     } else {
-        hipLaunchKernelGGL((bucket_bias_chunks<T, false>), grid, dim3(256), 0, st, d, order, chunk_start, part, o, chunks, H, NP);
+        hipLaunchKernelGGL((bucket_bias_chunks<T, false>), grid, dim3(256), 0, st, d, order, chunk_start, chunk_order, part, o, chunks, H, NP);
         hipLaunchKernelGGL((bucket_bias_join<T>), dim3((unsigned)nb, (unsigned)H), dim3(64), 0, st, part, bucket_chunk, o, H);
     }
     return (int)hipGetLastError();
@@ -119,9 +137,9 @@ int sd_bucket_bias_fwd(const void *table, const int32_t *index, void *out, int d
     return dtype == SD_F32 ? sd::fwd_launch<float>(table, index, out, heads, pairs, st) : sd::fwd_launch<sd::bf16_t>(table, index, out, heads, pairs, st);
 }
 
-int sd_bucket_bias_bwd(const void *dbias, const int32_t *order, const int32_t *chunk_start, const int32_t *bucket_chunk, void *dtable, int dtype, int buckets,
-                       int chunks, int heads, long pairs, void *workspace, size_t workspace_bytes, void *stream) {
-    if (!dbias || !order || !chunk_start || !bucket_chunk || !dtable) return SD_E_NULL;
+int sd_bucket_bias_bwd(const void *dbias, const int32_t *order, const int32_t *chunk_start, const int32_t *chunk_order, const int32_t *bucket_chunk, void *dtable,
+                       int dtype, int buckets, int chunks, int heads, long pairs, void *workspace, size_t workspace_bytes, void *stream) {
+    if (!dbias || !order || !chunk_start || !chunk_order || !bucket_chunk || !dtable) return SD_E_NULL;
     if (dtype != SD_F32 && dtype != SD_BF16) return SD_E_DTYPE;
     if (!sd::sizes_ok(buckets, heads, pairs) || chunks < buckets || chunks > 0x3ffffff) return SD_E_SHAPE;
     const size_t need = sd_bucket_bias_workspace_bytes(buckets, chunks, heads);
@@ -130,8 +148,8 @@ int sd_bucket_bias_bwd(const void *dbias, const int32_t *order, const int32_t *c
     if ((reinterpret_cast<uintptr_t>(dbias) | reinterpret_cast<uintptr_t>(dtable)) & es) return SD_E_ALIGN;
     hipStream_t st = static_cast<hipStream_t>(stream);
     float *part = static_cast<float *>(workspace);
-    return dtype == SD_F32 ? sd::bwd_launch<float>(dbias, order, chunk_start, bucket_chunk, dtable, buckets, chunks, heads, pairs, part, st)
-                           : sd::bwd_launch<sd::bf16_t>(dbias, order, chunk_start, bucket_chunk, dtable, buckets, chunks, heads, pairs, part, st);
+    return dtype == SD_F32 ? sd::bwd_launch<float>(dbias, order, chunk_start, chunk_order, bucket_chunk, dtable, buckets, chunks, heads, pairs, part, st)
+                           : sd::bwd_launch<sd::bf16_t>(dbias, order, chunk_start, chunk_order, bucket_chunk, dtable, buckets, chunks, heads, pairs, part, st);
 }
 
 }  // extern "C"

@@ -63,6 +63,15 @@ __device__ __forceinline__ Online online_group(Online o, Online *tmp, int tid, f
     return o;
 }
 
+template <typename T>
+__device__ __forceinline__ void unpack_vec(typename VecIO<T>::raw_t r, float (&a)[VecIO<T>::N]) {
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+        if constexpr (sizeof(T) == 4) a[q] = r[q];
+        else a[2 * q] = __uint_as_float((unsigned)r[q] << 16), a[2 * q + 1] = __uint_as_float((unsigned)r[q] & 0xffff0000u);
+    }
+}
+
 // Elements that come before the first 16-byte boundary of a row.
 template <typename T>
 __device__ __forceinline__ int row_head(const T *row, int n) {

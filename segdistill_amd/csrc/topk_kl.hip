@@ -47,16 +47,21 @@ __device__ __forceinline__ void write_partial(double kl, double n, double *__res
     }
 }
 
-__global__ __launch_bounds__(256) void topk_kl_finish(const double *__restrict__ part, int n, float alpha, float *__restrict__ loss, float *__restrict__ inv_n) {
+__global__ __launch_bounds__(1024) void topk_kl_finish(const double *__restrict__ part, int n, float alpha, float *__restrict__ loss, float *__restrict__ inv_n) {
     double kl = 0, rows = 0;
-    for (int i = threadIdx.x; i < n; i += 256) kl += part[2 * i], rows += part[2 * i + 1];
-    __shared__ double acc[8];
+#pragma unroll 4
+    for (int i = threadIdx.x; i < n; i += 1024) {
+        const double2 p = reinterpret_cast<const double2 *>(part)[i];
+        kl += p.x, rows += p.y;
+    }
+    __shared__ double acc[32];
 #pragma unroll
     for (int d = 32; d > 0; d >>= 1) kl += __shfl_xor(kl, d, 64), rows += __shfl_xor(rows, d, 64);
-    if ((threadIdx.x & 63) == 0) acc[threadIdx.x >> 6] = kl, acc[4 + (threadIdx.x >> 6)] = rows;
+    if ((threadIdx.x & 63) == 0) acc[threadIdx.x >> 6] = kl, acc[16 + (threadIdx.x >> 6)] = rows;
     __syncthreads();
     if (threadIdx.x == 0) {
-        kl = acc[0] + acc[1] + acc[2] + acc[3], rows = acc[4] + acc[5] + acc[6] + acc[7];
+        kl = rows = 0;
+        for (int w = 0; w < 16; ++w) kl += acc[w], rows += acc[16 + w];
         const double inv = rows > 0 ? 1.0 / rows : 0.0;              // no row left: the loss and every gradient are 0
         loss[0] = (float)(kl * inv * (double)alpha);
         inv_n[0] = (float)inv;
@@ -67,7 +72,7 @@ __global__ __launch_bounds__(256) void topk_kl_finish(const double *__restrict__
 // The pixel's set A is a bit mask in LDS, a column per thread: words[w][thread].  Classes come by in ascending order, so the entries are met in
 // ascending order too, and the rank of an entry -- the bits below it -- is its place in a second column: no search, no sort, and a class that
 // appears twice has one place.
-template <int BT>
+constexpr int BT = 64;      // pixels per workgroup: one wave (four of them were no faster at 131072 pixels, and slower on small maps)
 struct Columns {
     unsigned *words, *ranks;
     float *vals;
@@ -78,38 +83,50 @@ struct Columns {
     }
     __device__ int rank(int c) const { return (int)ranks[(c >> 5) * BT] + __popc(words[(c >> 5) * BT] & ((1u << (c & 31)) - 1)); }
 };
-template <int BT>
-__device__ __forceinline__ int mark_entries(const Columns<BT> &col, int nwords, const Entries &e, size_t at, long P, int C) {
-    for (int w = 0; w < nwords; ++w) col.words[w * BT] = 0;
-    for (int j = 0; j < e.k; ++j) {
-        const int c = e.index[at + (size_t)j * P];
-        if ((unsigned)c < (unsigned)C) col.words[(c >> 5) * BT] |= 1u << (c & 31);
+// Eight of the pixel's entries at a time, so that their loads go out together: classes outside [0, C) become -1, their values -inf.
+constexpr int kBatch = 8;
+__device__ __forceinline__ void load_batch(const Entries &e, size_t at, long P, int C, int j0, int (&c)[kBatch], float (&v)[kBatch]) {
+#pragma unroll
+    for (int u = 0; u < kBatch; ++u) {
+        const size_t from = at + (size_t)min(j0 + u, e.k - 1) * P;
+        c[u] = e.index[from];
+        v[u] = entry_value(e, from);
     }
-    int n = 0;
-    for (int w = 0; w < nwords; ++w) col.ranks[w * BT] = n, n += __popc(col.words[w * BT]);
-    return n;
+#pragma unroll
+    for (int u = 0; u < kBatch; ++u) {
+        const bool live = j0 + u < e.k && (unsigned)c[u] < (unsigned)C;
+        c[u] = live ? c[u] : -1;
+        v[u] = live ? v[u] : -INFINITY;
+    }
 }
-// The teacher's maximum and normaliser over its live entries and the rest.
-__device__ __forceinline__ Online teacher(const Entries &e, size_t at, long stride, size_t row, int C, float c2) {
-    Online t = {-INFINITY, 0.f};
-    for (int j = 0; j < e.k; ++j) {
-        const int c = e.index[at + (size_t)j * stride];
-        const float v[1] = {(unsigned)c < (unsigned)C ? entry_value(e, at + (size_t)j * stride) : -INFINITY};
+// The mask, the ranks and the number of the classes that are listed; the teacher's maximum and normaliser over the entries and the rest.
+__device__ __forceinline__ int take_entries(const Columns &col, int nwords, const Entries &e, size_t at, size_t row, long P, int C, float c2, Online &t) {
+    for (int w = 0; w < nwords; ++w) col.words[w * BT] = 0;
+    t = {-INFINITY, 0.f};
+    for (int j0 = 0; j0 < e.k; j0 += kBatch) {
+        int c[kBatch];
+        float v[kBatch];
+        load_batch(e, at, P, C, j0, c, v);
+#pragma unroll
+        for (int u = 0; u < kBatch; ++u)
+            if (c[u] >= 0) col.words[(c[u] >> 5) * BT] |= 1u << (c[u] & 31);
         online_fold(t, v, c2);
     }
     if (e.rest) {
         const float v[1] = {e.rest[row]};
         online_fold(t, v, c2);
     }
-    return t;
+    int n = 0;
+    for (int w = 0; w < nwords; ++w) col.ranks[w * BT] = n, n += __popc(col.words[w * BT]);
+    return n;
 }
 
-template <typename T, int BT>
+template <typename T>
 __global__ __launch_bounds__(BT) void topk_kl_planes_fwd(const T *__restrict__ S, Entries e, float4 *__restrict__ stats, double *__restrict__ part, int C, long P,
                                                          int blocks_per_image, int nwords, float c2) {
     extern __shared__ __attribute__((aligned(16))) unsigned char lds[];
-    constexpr int U = 8;
-    const Columns<BT> col(lds, nwords);
+    constexpr int U = 16;                                              // divides the 32 bits of a mask word
+    const Columns col(lds, nwords);
     const long b = blockIdx.x / blocks_per_image;
     const long p = (long)(blockIdx.x - b * blocks_per_image) * BT + threadIdx.x;
     const size_t row = (size_t)b * P + p;
@@ -117,26 +134,40 @@ __global__ __launch_bounds__(BT) void topk_kl_planes_fwd(const T *__restrict__ S
     if (p < P && (!e.valid || e.valid[row])) {
         counted = 1;
         const size_t at = (size_t)b * e.k * P + p;
-        const int members = mark_entries<BT>(col, nwords, e, at, P, C);
-        const T *ps = S + (size_t)b * C * P + p;
+        // the tile's address is uniform, the lane only adds its number: one scalar add per class.  A chunk is on its way while the one before it is folded.
+        const T *tile = S + (size_t)b * C * P + (p - threadIdx.x);
         Online low = {-INFINITY, 0.f};
         int next = 0;
-        unsigned word = 0;
-        for (int c0 = 0; c0 < C; c0 += U) {
-            float z[U];
+        float z[2][U];
+        auto fetch = [&](float (&to)[U], int c0) {
+            const T *at_c = tile + (size_t)c0 * P;
 #pragma unroll
-            for (int u = 0; u < U; ++u) z[u] = c0 + u < C ? VecIO<T>::load1(ps + (size_t)(c0 + u) * P) : -INFINITY;
-            if ((c0 & 31) == 0) word = col.words[(c0 >> 5) * BT];
+            for (int u = 0; u < U; ++u) {
+                to[u] = c0 + u < C ? VecIO<T>::load1(at_c + threadIdx.x) : -INFINITY;
+                at_c += P;
+            }
+        };
+        auto fold = [&](float (&x)[U], int c0) {
+            unsigned word = col.words[(c0 >> 5) * BT] >> (c0 & 31);
 #pragma unroll
             for (int u = 0; u < U; ++u) {
                 if (word & 1) {
-                    col.vals[next * BT] = z[u];
+                    col.vals[next * BT] = x[u];
                     ++next;
-                    z[u] = -INFINITY;
+                    x[u] = -INFINITY;
                 }
                 word >>= 1;
             }
-            online_fold(low, z, c2);
+            online_fold(low, x, c2);
+        };
+        fetch(z[0], 0);
+        Online t;
+        const int members = take_entries(col, nwords, e, at, row, P, C, c2, t);
+        for (int c0 = 0; c0 < C; c0 += 2 * U) {
+            if (c0 + U < C) fetch(z[1], c0 + U);
+            fold(z[0], c0);
+            if (c0 + 2 * U < C) fetch(z[0], c0 + 2 * U);
+            if (c0 + U < C) fold(z[1], c0 + U);
         }
         float m = low.m;
         for (int j = 0; j < members; ++j) m = fmaxf(m, col.vals[j * BT]);
@@ -145,15 +176,19 @@ __global__ __launch_bounds__(BT) void topk_kl_planes_fwd(const T *__restrict__ S
         float s = qr_num;
         for (int j = 0; j < members; ++j) s += ex2((col.vals[j * BT] - r) * c2);
         const float inv_s = 1.f / s, log_s = logf(s), tau_inv = c2 * kLn2;
-        const Online t = teacher(e, at, P, row, C, c2);
         const float tr = finite_ref(t.m), inv_t = 1.f / t.s, log_t = logf(t.s);
         float pr = 0.f, w = 0.f, k = 0.f;
         if (t.s > 0.f || t.s != t.s) {
-            for (int j = 0; j < e.k; ++j) {
-                const int c = e.index[at + (size_t)j * P];
-                if ((unsigned)c >= (unsigned)C) continue;
-                const float v = entry_value(e, at + (size_t)j * P) - tr, zq = col.vals[col.rank(c) * BT] - r;
-                k += kl_term(ex2(v * c2) * inv_t, v * tau_inv - log_t, zq * tau_inv - log_s);
+            for (int j0 = 0; j0 < e.k; j0 += kBatch) {
+                int c[kBatch];
+                float v[kBatch];
+                load_batch(e, at, P, C, j0, c, v);
+#pragma unroll
+                for (int u = 0; u < kBatch; ++u)
+                    if (c[u] >= 0) {
+                        const float d = v[u] - tr, zq = col.vals[col.rank(c[u]) * BT] - r;
+                        k += kl_term(ex2(d * c2) * inv_t, d * tau_inv - log_t, zq * tau_inv - log_s);
+                    }
             }
             if (e.rest) {
                 const float v = e.rest[row] - tr;
@@ -169,13 +204,13 @@ __global__ __launch_bounds__(BT) void topk_kl_planes_fwd(const T *__restrict__ S
     write_partial<BT>(kl, counted, part);
 }
 
-template <typename T, int BT>
+template <typename T>
 __global__ __launch_bounds__(BT) void topk_kl_planes_bwd(const T *__restrict__ S, Entries e, const float4 *__restrict__ stats, const float *__restrict__ inv_n,
                                                          const float *__restrict__ upstream, T *__restrict__ dS, int C, long P, int blocks_per_image, int nwords,
                                                          float c2, float coef) {
     extern __shared__ __attribute__((aligned(16))) unsigned char lds[];
-    constexpr int U = 8;
-    const Columns<BT> col(lds, nwords);
+    constexpr int U = 16;                                              // divides the 32 bits of a mask word
+    const Columns col(lds, nwords);
     const long b = blockIdx.x / blocks_per_image;
     const long p = (long)(blockIdx.x - b * blocks_per_image) * BT + threadIdx.x;
     const size_t row = (size_t)b * P + p;
@@ -188,33 +223,52 @@ __global__ __launch_bounds__(BT) void topk_kl_planes_bwd(const T *__restrict__ S
     }
     const float g = coef * inv_n[0] * upstream[0];
     const size_t at = (size_t)b * e.k * P + p;
-    const int members = mark_entries<BT>(col, nwords, e, at, P, C);
-    const Online t = teacher(e, at, P, row, C, c2);
-    const float tr = finite_ref(t.m), inv_t = 1.f / t.s;
-    for (int j = 0; j < members; ++j) col.vals[j * BT] = 0.f;
-    for (int j = 0; j < e.k; ++j) {
-        const int c = e.index[at + (size_t)j * P];
-        if ((unsigned)c < (unsigned)C) col.vals[col.rank(c) * BT] += ex2((entry_value(e, at + (size_t)j * P) - tr) * c2) * inv_t;
-    }
-    const T *ps = S + (size_t)b * C * P + p;
+    const T *tile = S + (size_t)b * C * P + (p - threadIdx.x);
+    T *dtile = dS + (size_t)b * C * P + (p - threadIdx.x);
     const float w = st.y * g, inv_s = st.w;
     int next = 0;
-    unsigned word = 0;
-    for (int c0 = 0; c0 < C; c0 += U) {
-        float z[U];
-#pragma unroll
-        for (int u = 0; u < U; ++u) z[u] = c0 + u < C ? VecIO<T>::load1(ps + (size_t)(c0 + u) * P) : 0.f;
-        if ((c0 & 31) == 0) word = col.words[(c0 >> 5) * BT];
+    float z[2][U];
+    auto fetch = [&](float (&to)[U], int c0) {
+        const T *at_c = tile + (size_t)c0 * P;
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            float d = ex2((z[u] - st.x) * c2) * w;
+            to[u] = c0 + u < C ? VecIO<T>::load1(at_c + threadIdx.x) : 0.f;
+            at_c += P;
+        }
+    };
+    auto write = [&](const float (&x)[U], int c0) {
+        unsigned word = col.words[(c0 >> 5) * BT] >> (c0 & 31);
+        T *at_c = dtile + (size_t)c0 * P;
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            float d = ex2((x[u] - st.x) * c2) * w;
             if (word & 1) {
-                d = (ex2((z[u] - st.z) * c2) * inv_s - col.vals[next * BT]) * g;
+                d = (ex2((x[u] - st.z) * c2) * inv_s - col.vals[next * BT]) * g;
                 ++next;
             }
             word >>= 1;
-            if (c0 + u < C) VecIO<T>::store1(pd + (size_t)(c0 + u) * P, d);
+            if (c0 + u < C) VecIO<T>::store1(at_c + threadIdx.x, d);
+            at_c += P;
         }
+    };
+    fetch(z[0], 0);
+    Online t;
+    const int members = take_entries(col, nwords, e, at, row, P, C, c2, t);
+    const float tr = finite_ref(t.m), inv_t = 1.f / t.s;
+    for (int j = 0; j < members; ++j) col.vals[j * BT] = 0.f;
+    for (int j0 = 0; j0 < e.k; j0 += kBatch) {
+        int c[kBatch];
+        float v[kBatch];
+        load_batch(e, at, P, C, j0, c, v);
+#pragma unroll
+        for (int u = 0; u < kBatch; ++u)
+            if (c[u] >= 0) col.vals[col.rank(c[u]) * BT] += ex2((v[u] - tr) * c2) * inv_t;
+    }
+    for (int c0 = 0; c0 < C; c0 += 2 * U) {
+        if (c0 + U < C) fetch(z[1], c0 + U);
+        write(z[0], c0);
+        if (c0 + 2 * U < C) fetch(z[0], c0 + 2 * U);
+        if (c0 + U < C) write(z[1], c0 + U);
     }
 }
 
@@ -265,7 +319,7 @@ template <typename T, int NT>
 __global__ __launch_bounds__(NT == 64 ? 256 : NT) void topk_kl_rows_fwd(const T *__restrict__ S, Entries e, float4 *__restrict__ stats, double *__restrict__ part,
                                                                         long rows, int C, float c2) {
     extern __shared__ __attribute__((aligned(16))) unsigned char lds[];
-    constexpr int G = NT == 64 ? 4 : 1, N = VecIO<T>::N;
+    constexpr int G = NT == 64 ? 4 : 1, N = VecIO<T>::N, V = 4;
     __shared__ Online tmp[NT / 64 + 1];
     const int nwords = row_words(C);
     const int grp = NT == 64 ? threadIdx.x >> 6 : 0, tid = NT == 64 ? threadIdx.x & 63 : threadIdx.x;
@@ -291,17 +345,33 @@ __global__ __launch_bounds__(NT == 64 ? 256 : NT) void topk_kl_rows_fwd(const T 
             const float one[1] = {VecIO<T>::load1(z + tid)};
             online_fold(low, one, c2);
         }
-        for (int i = tid; i < nvec; i += NT) {
-            float a[N];
-            VecIO<T>::load(z + head + (size_t)i * N, a);
+        auto fold = [&](float (&a)[N], int i) {
             const int at = head + shift + i * N;
-            unsigned m = bits[at >> 5] >> (at & 31);
+            const unsigned m = bits[at >> 5] >> (at & 31);
             if (m & ((1u << N) - 1)) {
 #pragma unroll
                 for (int q = 0; q < N; ++q)
                     if ((m >> q) & 1) a[q] = -INFINITY;
             }
             online_fold(low, a, c2);
+        };
+        const typename VecIO<T>::raw_t *vec = reinterpret_cast<const typename VecIO<T>::raw_t *>(z + head);
+        int i = tid;
+        for (; i + (V - 1) * NT < nvec; i += V * NT) {                 // V vectors on their way at a time
+            typename VecIO<T>::raw_t raw[V];
+#pragma unroll
+            for (int u = 0; u < V; ++u) raw[u] = __builtin_nontemporal_load(vec + i + u * NT);
+#pragma unroll
+            for (int u = 0; u < V; ++u) {
+                float a[N];
+                unpack_vec<T>(raw[u], a);
+                fold(a, i + u * NT);
+            }
+        }
+        for (; i < nvec; i += NT) {
+            float a[N];
+            VecIO<T>::load(z + head + (size_t)i * N, a);
+            fold(a, i);
         }
         const int t = head + nvec * N + tid;
         if (t < C && outside(t)) {
@@ -407,7 +477,7 @@ __global__ __launch_bounds__(NT == 64 ? 256 : NT) void topk_kl_rows_bwd(const T 
 
 // ---- launches ---------------------------------------------------------------------------------------------------------------------------------
 struct Plan {
-    int threads, blocks, nwords, lds;      // threads per row (P == 1) or per workgroup (planes)
+    int threads, blocks, nwords, lds;      // threads per row (P == 1) or per workgroup (planes: one per pixel)
     long per;                              // workgroups per image (planes)
 };
 // false: not a shape these kernels launch
@@ -424,10 +494,10 @@ bool plan(long B, int C, long P, int k, Plan *pl) {
     }
     pl->nwords = (C + 31) / 32;
     const long column = 4L * (2 * pl->nwords + k);                      // bytes of LDS per pixel
-    pl->threads = column * 256 <= 32768 ? 256 : 64;
-    if (column * 64 > 64512) return false;                              // 64 KB less what the kernels hold besides
-    pl->lds = (int)column * pl->threads;
-    pl->per = (P + pl->threads - 1) / pl->threads;
+    if (column * BT > 64512) return false;                              // 64 KB less what the kernels hold besides
+    pl->threads = BT;
+    pl->lds = (int)column * BT;
+    pl->per = (P + BT - 1) / BT;
     if (pl->per > kMaxBlocks / B) return false;
     pl->blocks = (int)(pl->per * B);
     return true;
@@ -442,10 +512,9 @@ int fwd_launch(const void *S, const Entries &e, long B, int C, long P, const Pla
         if (pl.threads == 64) hipLaunchKernelGGL((topk_kl_rows_fwd<T, 64>), grid, dim3(256), pl.lds, st, s, e, stats, part, B, C, c2);
         else hipLaunchKernelGGL((topk_kl_rows_fwd<T, 256>), grid, dim3(256), pl.lds, st, s, e, stats, part, B, C, c2);
     } else {
-        if (pl.threads == 64) hipLaunchKernelGGL((topk_kl_planes_fwd<T, 64>), grid, dim3(64), pl.lds, st, s, e, stats, part, C, P, (int)pl.per, pl.nwords, c2);
-        else hipLaunchKernelGGL((topk_kl_planes_fwd<T, 256>), grid, dim3(256), pl.lds, st, s, e, stats, part, C, P, (int)pl.per, pl.nwords, c2);
+        hipLaunchKernelGGL((topk_kl_planes_fwd<T>), grid, dim3(BT), pl.lds, st, s, e, stats, part, C, P, (int)pl.per, pl.nwords, c2);
     }
-    hipLaunchKernelGGL(topk_kl_finish, dim3(1), dim3(256), 0, st, part, pl.blocks, alpha, loss, inv_n);
+    hipLaunchKernelGGL(topk_kl_finish, dim3(1), dim3(1024), 0, st, part, pl.blocks, alpha, loss, inv_n);
     return (int)hipGetLastError();
 }
 
@@ -460,10 +529,7 @@ int bwd_launch(const void *S, const Entries &e, long B, int C, long P, const Pla
         else hipLaunchKernelGGL((topk_kl_rows_bwd<T, 256>), grid, dim3(256), 0, st, s, e, stats, inv_n, upstream, d, B, C, c2, coef);
     } else {
         const dim3 grid((unsigned)pl.blocks);
-        if (pl.threads == 64)
-            hipLaunchKernelGGL((topk_kl_planes_bwd<T, 64>), grid, dim3(64), pl.lds, st, s, e, stats, inv_n, upstream, d, C, P, (int)pl.per, pl.nwords, c2, coef);
-        else
-            hipLaunchKernelGGL((topk_kl_planes_bwd<T, 256>), grid, dim3(256), pl.lds, st, s, e, stats, inv_n, upstream, d, C, P, (int)pl.per, pl.nwords, c2, coef);
+        hipLaunchKernelGGL((topk_kl_planes_bwd<T>), grid, dim3(BT), pl.lds, st, s, e, stats, inv_n, upstream, d, C, P, (int)pl.per, pl.nwords, c2, coef);
     }
     return (int)hipGetLastError();
 }
@@ -502,7 +568,7 @@ int sd_topk_kl_fwd(const void *S, const void *values, const int32_t *index, cons
     const int rc = sd::check_args(S, values, index, rest, dtype, values_dtype, B, C, P, k, tau, &pl);
     if (rc != SD_OK) return rc;
     if (!stats || !inv_rows || !loss || !workspace) return SD_E_NULL;
-    if (workspace_bytes < 2 * sizeof(double) * (size_t)pl.blocks || (reinterpret_cast<uintptr_t>(workspace) & 7)) return SD_E_WORKSPACE;
+    if (workspace_bytes < 2 * sizeof(double) * (size_t)pl.blocks || (reinterpret_cast<uintptr_t>(workspace) & 15)) return SD_E_WORKSPACE;
     if (reinterpret_cast<uintptr_t>(stats) & 15) return SD_E_ALIGN;
     const sd::Entries e = {values, index, rest, valid, values_dtype == SD_BF16, k};
     hipStream_t st = static_cast<hipStream_t>(stream);

@@ -212,15 +212,6 @@ struct Row {
     }
     __device__ __forceinline__ bool held() const { return nvec <= NT * NV; }
     __device__ __forceinline__ raw_t vec(int i) const { return __builtin_nontemporal_load(reinterpret_cast<const raw_t *>(row + head) + i); }
-    static __device__ __forceinline__ void unpack(raw_t r, float (&a)[N]) {
-        if constexpr (N == 4) {
-#pragma unroll
-            for (int q = 0; q < 4; ++q) a[q] = r[q];
-        } else {
-#pragma unroll
-            for (int q = 0; q < 4; ++q) a[2 * q] = __uint_as_float((unsigned)r[q] << 16), a[2 * q + 1] = __uint_as_float((unsigned)r[q] & 0xffff0000u);
-        }
-    }
     // f(values, first index): the elements before and behind the vectors
     template <typename F>
     __device__ __forceinline__ void ends(int tid, F f) const {
@@ -239,7 +230,7 @@ struct Row {
 #pragma unroll 1
         for (int i = tid; i < nvec; i += NT) {
             float a[N];
-            unpack(vec(i), a);
+            unpack_vec<T>(vec(i), a);
             f(a, head + i * N);
         }
         ends(tid, f);
@@ -372,7 +363,7 @@ __global__ __launch_bounds__(NT == 64 ? 256 : NT, WAVES) void topk_rows(const T 
         for (int u = 0; u < NV; ++u)
             if (tid + u * NT < row.nvec) {
                 float a[N];
-                R::unpack(reg[u], a);
+                unpack_vec<T>(reg[u], a);
                 largest(a, 0);
             }
         row.ends(tid, largest);
@@ -431,7 +422,7 @@ __global__ __launch_bounds__(NT == 64 ? 256 : NT, WAVES) void topk_rows(const T 
             const int i = tid + u * NT;
             if (i < row.nvec) {
                 float a[N];
-                R::unpack(reg[u], a);
+                unpack_vec<T>(reg[u], a);
                 take(a, row.head + i * N);
             }
         }

@@ -41,6 +41,8 @@ class BucketPlan(nn.Module):
         self.register_buffer('order', order.int(), persistent=False)
         self.register_buffer('chunk_start', torch.cat([start, start.new_tensor([flat.numel()])]).int(), persistent=False)
         self.register_buffer('bucket_chunk', bucket_chunk.int(), persistent=False)
+        first_pair = order[start.clamp(max=flat.numel() - 1)]
+        self.register_buffer('chunk_order', torch.sort(first_pair, stable=True).indices.int(), persistent=False)
 
     def extra_repr(self):
         return f'{self.shape[0]} x {self.shape[1]} pairs in {self.num_buckets} buckets'
@@ -62,7 +64,7 @@ class _BucketBiasFunction(torch.autograd.Function):
     def backward(ctx, grad_out):
         _no_double_backward('bucket_bias')
         plan = ctx.plan
-        order, start, bucket = plan._buffers['order'], plan._buffers['chunk_start'], plan._buffers['bucket_chunk']
+        order, start, by_pair, bucket = (plan._buffers[n] for n in ('order', 'chunk_start', 'chunk_order', 'bucket_chunk'))
         d = grad_out.contiguous()
         heads, nb, chunks = d.shape[0], plan.num_buckets, start.numel() - 1
         L = _lib.lib()
@@ -70,7 +72,7 @@ class _BucketBiasFunction(torch.autograd.Function):
         ws_bytes = L.sd_bucket_bias_workspace_bytes(nb, chunks, heads)
         ws = torch.empty(ws_bytes, dtype=torch.uint8, device=d.device) if ws_bytes else None
         with _launch_on(d.device) as stream:
-            rc = L.sd_bucket_bias_bwd(d.data_ptr(), order.data_ptr(), start.data_ptr(), bucket.data_ptr(), dtable.data_ptr(), _DT[d.dtype], nb, chunks, heads,
+            rc = L.sd_bucket_bias_bwd(d.data_ptr(), order.data_ptr(), start.data_ptr(), by_pair.data_ptr(), bucket.data_ptr(), dtable.data_ptr(), _DT[d.dtype], nb, chunks, heads,
                                       order.numel(), _ptr(ws), ws_bytes, stream)
         _lib.check(rc, 'sd_bucket_bias_bwd')
         return dtable, None

@@ -62,11 +62,11 @@ def test_bucket_bias_refusals(L):
     def fwd(t=P, i=P, o=P, dt=0, nb=7, h=3, n=100):
         return L.sd_bucket_bias_fwd(t, i, o, dt, nb, h, n, NULL)
 
-    def bwd(d=P, o=P, cs=P, bc=P, t=P, dt=0, nb=7, ch=9, h=3, n=100, w=P, wb=9 * 3 * 4):
-        return L.sd_bucket_bias_bwd(d, o, cs, bc, t, dt, nb, ch, h, n, w, wb, NULL)
+    def bwd(d=P, o=P, cs=P, co=P, bc=P, t=P, dt=0, nb=7, ch=9, h=3, n=100, w=P, wb=9 * 3 * 4):
+        return L.sd_bucket_bias_bwd(d, o, cs, co, bc, t, dt, nb, ch, h, n, w, wb, NULL)
     assert fwd(t=NULL) == fwd(i=NULL) == fwd(o=NULL) == E_NULL and fwd(dt=9) == E_DTYPE
     assert fwd(nb=0) == fwd(h=0) == fwd(n=0) == fwd(n=2 ** 31) == fwd(h=65536) == E_SHAPE and fwd(t=P + 2) == E_ALIGN and fwd(i=P + 2) == E_ALIGN
-    for a in ('d', 'o', 'cs', 'bc', 't'):
+    for a in ('d', 'o', 'cs', 'co', 'bc', 't'):
         assert bwd(**{a: NULL}) == E_NULL
     assert bwd(dt=9) == E_DTYPE and bwd(ch=6) == E_SHAPE and bwd(nb=0) == E_SHAPE and bwd(w=NULL) == E_WS and bwd(wb=4) == E_WS and bwd(d=P + 2) == E_ALIGN
 
@@ -100,6 +100,7 @@ def test_bucket_plan_orders_every_pair_once_and_refuses_bad_maps():
     index[index == 3] = 2
     plan = rel_bias.BucketPlan(index, 8)                                    # buckets 3, 6 and 7 are empty
     assert sorted(plan.order.tolist()) == list(range(4200)) and plan.bucket_chunk[0] == 0 and plan.bucket_chunk[-1] == plan.chunk_start.numel() - 1
+    assert sorted(plan.chunk_order.tolist()) == list(range(plan.chunk_start.numel() - 1))
     for b in range(8):
         lo, hi = plan.bucket_chunk[b].item(), plan.bucket_chunk[b + 1].item()
         assert hi > lo
