@@ -28,6 +28,8 @@ typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef short s16x8 __attribute__((ext_vector_type(8)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+typedef float f32x2 __attribute__((ext_vector_type(2)));
 typedef unsigned int u32x4 __attribute__((ext_vector_type(4)));
 constexpr int D = 32;
 
@@ -51,6 +53,9 @@ struct Lds<float> {
     static constexpr int cross_pitch(int NT) { return 32 * NT + 4; }
     static __host__ __device__ constexpr size_t cross_bytes(int N, int NT) { return (size_t)rows(N) * (32 * NT + 4) * 4; }
 
+    typedef f32x16 Operand;                                                       // a tile of P or dS as its products take it
+    static __device__ __forceinline__ Operand operand(const f32x16 &p) { return p; }
+
     // acc[m][n] += sum_d A[32 t + m][d] B[pb][d], lane n holding row pb
     template <int NT>
     static __device__ __forceinline__ void rows_product(f32x16 (&acc)[NT], const float *A, const float *B, int pb, int N, int r, int hh) {
@@ -71,7 +76,7 @@ struct Lds<float> {
     }
     // acc[d][i] += sum_j M[j][d] p[j][i], p in the accumulator layout
     template <int NT>
-    static __device__ __forceinline__ void columns_product(f32x16 &acc, const float *M, const f32x16 (&p)[NT], int N, int lane) {
+    static __device__ __forceinline__ void columns_product(f32x16 &acc, const float *M, const Operand (&p)[NT], int N, int lane) {
         const int r = lane & 31, hh = lane >> 5;
 #pragma unroll
         for (int a = 0; a < NT; ++a)
@@ -85,7 +90,7 @@ struct Lds<float> {
     }
     // the wave's query rows of p into the cross image
     template <int NT>
-    static __device__ __forceinline__ void cross_write(float *x, const f32x16 (&p)[NT], int i, int N, int hh) {
+    static __device__ __forceinline__ void cross_write(float *x, const Operand (&p)[NT], int i, int N, int hh) {
         if (i >= rows(N)) return;
 #pragma unroll
         for (int a = 0; a < NT; ++a)
@@ -136,16 +141,24 @@ struct Lds<bf16_t> {
             for (int a = 0; a < NT; ++a) acc[a] = mfma(*reinterpret_cast<const bf16x8 *>(A + min(32 * a + r, last) * PITCH + 16 * t + 8 * hh), bv, acc[a]);
         }
     }
-    // p = first + second, each bf16, to 2^-17 of p
-    static __device__ __forceinline__ void split8(const f32x16 &p, int at, bf16x8 &first, bf16x8 &second) {
+    // p = first + second, each bf16, to 2^-17 of p; elements 8 t .. 8 t + 7 of the accumulator tile in first[t], second[t].  On pairs: one conversion
+    // instruction takes two values.
+    struct Operand {
+        bf16x8 first[2], second[2];
+    };
+    static __device__ __forceinline__ Operand operand(const f32x16 &p) {
+        Operand o;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            first[i] = (__bf16)p[at + i];
-            second[i] = (__bf16)(p[at + i] - (float)first[i]);
+        for (int e = 0; e < 16; e += 2) {
+            const f32x2 v = {p[e], p[e + 1]};
+            const bf16x2 f = __builtin_convertvector(v, bf16x2), s = __builtin_convertvector(v - __builtin_convertvector(f, f32x2), bf16x2);
+            o.first[e >> 3][e & 7] = f[0], o.first[e >> 3][(e & 7) + 1] = f[1];
+            o.second[e >> 3][e & 7] = s[0], o.second[e >> 3][(e & 7) + 1] = s[1];
         }
+        return o;
     }
     template <int NT>
-    static __device__ __forceinline__ void columns_product(f32x16 &acc, const bf16_t *M, const f32x16 (&p)[NT], int N, int lane) {
+    static __device__ __forceinline__ void columns_product(f32x16 &acc, const bf16_t *M, const Operand (&p)[NT], int N, int lane) {
         const int hh = lane >> 5;
 #pragma unroll
         for (int a = 0; a < NT; ++a)
@@ -154,22 +167,18 @@ struct Lds<bf16_t> {
                 if (32 * a + 16 * t < N) {
                     const int j0 = 32 * a + 16 * t + 4 * hh;                       // accumulator rows 8 t .. 8 t + 7 are j0 .. j0 + 3 and j0 + 8 .. j0 + 11
                     const bf16x8 m = columns(M, PITCH, j0, j0 + 8, 0, lane);
-                    bf16x8 x, y;
-                    split8(p[a], 8 * t, x, y);
-                    acc = mfma(m, x, acc);
-                    acc = mfma(m, y, acc);
+                    acc = mfma(m, p[a].first[t], acc);
+                    acc = mfma(m, p[a].second[t], acc);
                 }
     }
     template <int NT>
-    static __device__ __forceinline__ void cross_write(bf16_t *x, const f32x16 (&p)[NT], int i, int N, int hh) {
+    static __device__ __forceinline__ void cross_write(bf16_t *x, const Operand (&p)[NT], int i, int N, int hh) {
         if (i >= rows(N)) return;
 #pragma unroll
         for (int a = 0; a < NT; ++a)
 #pragma unroll
             for (int t = 0; t < 2; ++t) {
-                bf16x8 first, second;
-                split8(p[a], 8 * t, first, second);
-                const u32x4 f = __builtin_bit_cast(u32x4, first), s = __builtin_bit_cast(u32x4, second);
+                const u32x4 f = __builtin_bit_cast(u32x4, p[a].first[t]), s = __builtin_bit_cast(u32x4, p[a].second[t]);
                 bf16_t *to = x + i * cross_pitch(NT) + 32 * a + 16 * t + 4 * hh;
                 *reinterpret_cast<uint2 *>(to) = make_uint2(f[0], f[1]);
                 *reinterpret_cast<uint2 *>(to + 8) = make_uint2(f[2], f[3]);
@@ -201,8 +210,13 @@ struct Stage {
     __device__ __forceinline__ void load(const T *base, long stride, int N) {
         const int row = threadIdx.x / CH, ch = threadIdx.x % CH;
 #pragma unroll
-        for (int u = 0; u < PASSES; ++u)
-            if (row + u * STEP < N) reg[u] = __builtin_nontemporal_load(reinterpret_cast<const u32x4 *>(base + (size_t)(row + u * STEP) * stride) + ch);
+        for (int u = 0; u < PASSES; ++u)              // every lane loads, rows behind the window the last one again: a register written in part stays live all along
+            reg[u] = *(reinterpret_cast<const u32x4 *>(base + (size_t)min(row + u * STEP, N - 1) * stride) + ch);
+    }
+    __device__ __forceinline__ void clear() {
+        const u32x4 z = {0u, 0u, 0u, 0u};
+#pragma unroll
+        for (int u = 0; u < PASSES; ++u) reg[u] = z;
     }
     __device__ __forceinline__ void store(T *img, int N) const {
         const int row = threadIdx.x / CH, ch = threadIdx.x % CH;
@@ -326,31 +340,37 @@ __global__ __launch_bounds__(64 * NT) __attribute__((amdgpu_waves_per_eu(3))) vo
         const T *q = base + (size_t)win * wstride;
         sq.load(q, stride, N), sk.load(q + C, stride, N), sv.load(q + 2 * C, stride, N);
     };
+    auto none = [&]() { sq.clear(), sk.clear(), sv.clear(); };          // a value on both ways: else the old one would stay live through the loop
     fetch(slab);
     zero_tail<T, NT>(Q, N), zero_tail<T, NT>(K, N), zero_tail<T, NT>(V, N);
     for (int win = slab; win < windows; win += nslab) {
         __syncthreads();                               // the previous window's images are read
         sq.store(Q, N), sk.store(K, N), sv.store(V, N);
         __syncthreads();
-        if (win + nslab < windows) fetch(win + nslab);
         const float4 *mask = nW && any[win % nW] ? reinterpret_cast<const float4 *>(packed + (size_t)(heads + win % nW) * (NT * NT * 1024)) + w * 256 + lane : nullptr;
         f32x16 p[NT], o = zero16();
 #pragma unroll
         for (int a = 0; a < NT; ++a) p[a] = zero16();
         Lds<T>::template rows_product<NT>(p, K, Q, 32 * w + r, N, r, hh);
         softmax_tile<NT>(p, bias, mask, scale, 32 * w + r < N);
-        Lds<T>::template columns_product<NT>(o, V, p, N, lane);
+        win + nslab < windows ? fetch(win + nslab) : none();          // (not before: the registers are the scores' until here)
+        typename Lds<T>::Operand po[NT];
+#pragma unroll
+        for (int a = 0; a < NT; ++a) po[a] = Lds<T>::operand(p[a]);
+        Lds<T>::template columns_product<NT>(o, V, po, N, lane);
         store_tile(out + (size_t)win * N * C + (size_t)head * D, C, 32 * w + r, N, hh, o, 1.f);
     }
 }
 
+constexpr int kBwdWaves = 2;           // waves per SIMD that the backward's registers leave room for (three: 73 spilled, bf16 76 -> 145 us)
+
 template <typename T, int NT>
-__global__ __launch_bounds__(64 * NT) __attribute__((amdgpu_waves_per_eu(2))) void window_train_bwd(const T *__restrict__ qkv, const float *__restrict__ packed, const int *__restrict__ any,
+__global__ __launch_bounds__(64 * NT, kBwdWaves) void window_train_bwd(const T *__restrict__ qkv, const float *__restrict__ packed, const int *__restrict__ any,
                                                             const T *__restrict__ dout, T *__restrict__ dqkv, float *__restrict__ slabs, int windows, int nslab, int nW,
                                                             int heads, int N, float scale) {
     extern __shared__ __attribute__((aligned(16))) unsigned char lds[];
     const size_t img = image_elems<T>(N);
-    T *Q = reinterpret_cast<T *>(lds), *K = Q + img, *V = K + img, *G = V + img, *X = G + img;
+    T *Q = reinterpret_cast<T *>(lds), *G = Q + img, *K = G + img, *V = K + img, *X = K;          // P and dS cross where K and V were
     const int lane = threadIdx.x & 63, r = lane & 31, hh = lane >> 5, w = threadIdx.x >> 6, i = 32 * w + r;
     const int job = logical_block(), slab = job / heads, head = job - slab * heads;
     const long C = (long)heads * D, stride = 3 * C, wstride = N * stride;
@@ -362,16 +382,17 @@ __global__ __launch_bounds__(64 * NT) __attribute__((amdgpu_waves_per_eu(2))) vo
         sq.load(q, stride, N), sk.load(q + C, stride, N), sv.load(q + 2 * C, stride, N);
         sg.load(gbase + (size_t)win * N * C, C, N);
     };
+    auto none = [&]() { sq.clear(), sk.clear(), sv.clear(), sg.clear(); };          // a value on both ways: else the old one would stay live through the loop
     fetch(slab);
-    zero_tail<T, NT>(Q, N), zero_tail<T, NT>(K, N), zero_tail<T, NT>(V, N), zero_tail<T, NT>(G, N);
+    zero_tail<T, NT>(Q, N), zero_tail<T, NT>(G, N);
     f32x16 db[NT];
 #pragma unroll
     for (int a = 0; a < NT; ++a) db[a] = zero16();
     for (int win = slab; win < windows; win += nslab) {
         __syncthreads();                               // the previous window's images are read
         sq.store(Q, N), sk.store(K, N), sv.store(V, N), sg.store(G, N);
+        zero_tail<T, NT>(K, N), zero_tail<T, NT>(V, N);
         __syncthreads();
-        if (win + nslab < windows) fetch(win + nslab);
         const float4 *mask = nW && any[win % nW] ? reinterpret_cast<const float4 *>(packed + (size_t)(heads + win % nW) * (NT * NT * 1024)) + w * 256 + lane : nullptr;
         T *dq = dqkv + (size_t)win * wstride + (size_t)head * D;
         f32x16 p[NT], ds[NT];
@@ -379,7 +400,6 @@ __global__ __launch_bounds__(64 * NT) __attribute__((amdgpu_waves_per_eu(2))) vo
         for (int a = 0; a < NT; ++a) p[a] = ds[a] = zero16();
         Lds<T>::template rows_product<NT>(p, K, Q, i, N, r, hh);
         softmax_tile<NT>(p, bias, mask, scale, i < N);
-        Lds<T>::template cross_write<NT>(X, p, i, N, hh);
         Lds<T>::template rows_product<NT>(ds, V, G, i, N, r, hh);
         float dot = 0.f;
 #pragma unroll
@@ -394,19 +414,25 @@ __global__ __launch_bounds__(64 * NT) __attribute__((amdgpu_waves_per_eu(2))) vo
                 ds[a][e] = i < N ? p[a][e] * (ds[a][e] - dot) : 0.f;
                 db[a][e] += ds[a][e];
             }
+        typename Lds<T>::Operand po[NT], so[NT];
+#pragma unroll
+        for (int a = 0; a < NT; ++a) po[a] = Lds<T>::operand(p[a]), so[a] = Lds<T>::operand(ds[a]);
         {
             f32x16 o = zero16();
-            Lds<T>::template columns_product<NT>(o, K, ds, N, lane);
+            Lds<T>::template columns_product<NT>(o, K, so, N, lane);
             store_tile(dq, stride, i, N, hh, o, scale);
         }
+        __syncthreads();                               // K and V are read
+        Lds<T>::template cross_write<NT>(X, po, i, N, hh);
         __syncthreads();                               // every query row of P is there
+        win + nslab < windows ? fetch(win + nslab) : none();          // (not before: the registers are the scores' and P's until here)
         {
             f32x16 o = zero16();
             Lds<T>::template cross_product<NT>(o, G, X, w, N, lane);
             store_tile(dq + 2 * C, stride, i, N, hh, o, 1.f);
         }
         __syncthreads();                               // P is read
-        Lds<T>::template cross_write<NT>(X, ds, i, N, hh);
+        Lds<T>::template cross_write<NT>(X, so, i, N, hh);
         __syncthreads();
         {
             f32x16 o = zero16();
@@ -460,13 +486,16 @@ int slabs_for(long windows, int heads, int per_cu) {
 template <typename T>
 size_t fwd_lds(int N) { return 3 * image_elems<T>(N) * sizeof(T); }
 template <typename T>
-size_t bwd_lds(int N) { return 4 * image_elems<T>(N) * sizeof(T) + Lds<T>::cross_bytes(N, N <= 32 ? 1 : 2); }
+size_t bwd_lds(int N) {
+    const size_t two = 2 * image_elems<T>(N) * sizeof(T), cross = Lds<T>::cross_bytes(N, N <= 32 ? 1 : 2);
+    return two + (two > cross ? two : cross);
+}
 int per_cu(size_t lds, int most) {
     const int n = (int)(160 * 1024 / (lds + 512));
     return n < most ? n : most;
 }
 template <typename T>
-int bwd_slabs(long windows, int heads, int N) { return slabs_for(windows, heads, per_cu(bwd_lds<T>(N), N <= 32 ? 8 : 4)); }
+int bwd_slabs(long windows, int heads, int N) { return slabs_for(windows, heads, per_cu(bwd_lds<T>(N), kBwdWaves * (N <= 32 ? 4 : 2))); }
 
 bool shape_ok(long windows, int heads, int N) { return windows > 0 && heads > 0 && windows <= 0x3fffffffL / heads && N >= 1 && N <= 64; }
 size_t table_floats(int heads, int nW, int N) { return (size_t)(heads + nW) * (N <= 32 ? 1024 : 4096); }

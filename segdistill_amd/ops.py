@@ -26,24 +26,13 @@ def _ptr(t):
     return None if t is None else t.data_ptr()
 
 
-class _launch_on:
-    """`with _launch_on(device) as stream`: the device's current stream (a raw hipStream_t); launches inside go to that device, whichever is current
-    outside."""
-
-    __slots__ = ('index', 'back')
-
-    def __init__(self, device):
-        self.index, self.back = device.index, -1
-
-    def __enter__(self):
-        if torch.cuda.current_device() != self.index:
-            self.back = torch.cuda._exchange_device(self.index)
-        return torch._C._cuda_getCurrentRawStream(self.index)
-
-    def __exit__(self, *exc):
-        if self.back >= 0:
-            torch.cuda._exchange_device(self.back)
-        return False
+def _launch(device, fn, *args):
+    """fn(*args, stream) on `device`'s current stream, whichever device is current -> the status."""
+    index = device.index
+    if torch._C._cuda_getDevice() == index:
+        return fn(*args, torch._C._cuda_getCurrentRawStream(index))
+    with torch.cuda.device(index):
+        return fn(*args, torch._C._cuda_getCurrentRawStream(index))
 
 
 def _no_double_backward(name):
@@ -715,8 +704,7 @@ def topk_logits(x, k, *, tau=1.0):
     index = torch.empty(_entry_shape(x, k), dtype=torch.int32, device=x.device)
     rest = torch.empty(_row_shape(x), dtype=torch.float32, device=x.device)
     if x.numel():
-        with _launch_on(x.device) as stream:
-            rc = L.sd_topk_select(x.data_ptr(), values.data_ptr(), index.data_ptr(), rest.data_ptr(), _DT[x.dtype], B, Cc, P, k, tau, stream)
+        rc = _launch(x.device, L.sd_topk_select, x.data_ptr(), values.data_ptr(), index.data_ptr(), rest.data_ptr(), _DT[x.dtype], B, Cc, P, k, tau)
         _lib.check(rc, 'sd_topk_select')
     return values, index, rest
 
@@ -731,9 +719,8 @@ class _TopKKLFunction(torch.autograd.Function):
         keep = torch.empty(4 * rows + 4 + ws_bytes // 4, dtype=torch.float32, device=S.device)
         loss = torch.empty((), dtype=torch.float32, device=S.device)
         at = keep.data_ptr()
-        with _launch_on(S.device) as stream:
-            rc = L.sd_topk_kl_fwd(S.data_ptr(), values.data_ptr(), index.data_ptr(), _ptr(rest), _ptr(valid), _DT[S.dtype], _DT[values.dtype], B, Cc, P, k,
-                                  tau, alpha, at, at + 16 * rows, loss.data_ptr(), at + 16 * rows + 16, ws_bytes, stream)
+        rc = _launch(S.device, L.sd_topk_kl_fwd, S.data_ptr(), values.data_ptr(), index.data_ptr(), _ptr(rest), _ptr(valid), _DT[S.dtype], _DT[values.dtype],
+                     B, Cc, P, k, tau, alpha, at, at + 16 * rows, loss.data_ptr(), at + 16 * rows + 16, ws_bytes)
         _lib.check(rc, 'sd_topk_kl_fwd')
         ctx.save_for_backward(S, values, index, rest, valid, keep)
         ctx.meta = (tau, alpha, B, Cc, P, k)
@@ -747,9 +734,8 @@ class _TopKKLFunction(torch.autograd.Function):
         dS = torch.empty_like(S)
         up = grad_loss if grad_loss.dtype == torch.float32 else grad_loss.float()
         at = keep.data_ptr()
-        with _launch_on(S.device) as stream:
-            rc = _lib.lib().sd_topk_kl_bwd(S.data_ptr(), values.data_ptr(), index.data_ptr(), _ptr(rest), _ptr(valid), _DT[S.dtype], _DT[values.dtype], B, Cc,
-                                           P, k, tau, alpha, at, at + 16 * B * P, up.data_ptr(), dS.data_ptr(), stream)
+        rc = _launch(S.device, _lib.lib().sd_topk_kl_bwd, S.data_ptr(), values.data_ptr(), index.data_ptr(), _ptr(rest), _ptr(valid), _DT[S.dtype],
+                     _DT[values.dtype], B, Cc, P, k, tau, alpha, at, at + 16 * B * P, up.data_ptr(), dS.data_ptr())
         _lib.check(rc, 'sd_topk_kl_bwd')
         return dS, None, None, None, None, None, None, None, None, None, None
 

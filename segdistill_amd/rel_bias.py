@@ -7,7 +7,7 @@ import torch
 import torch.nn as nn
 
 from . import _lib
-from .ops import _DT, _launch_on, _no_double_backward, _ptr, _require_gpu
+from .ops import _DT, _launch, _no_double_backward, _ptr, _require_gpu
 
 
 CHUNK = 512          # sd_bucket_bias_chunk(): the pairs of one bucket that one wave sums (a plan is built without the library)
@@ -54,8 +54,7 @@ class _BucketBiasFunction(torch.autograd.Function):
         nb, heads = table.shape
         index = plan._buffers['index']
         out = torch.empty((heads,) + plan.shape, dtype=table.dtype, device=table.device)
-        with _launch_on(table.device) as stream:
-            rc = _lib.lib().sd_bucket_bias_fwd(table.data_ptr(), index.data_ptr(), out.data_ptr(), _DT[table.dtype], nb, heads, index.numel(), stream)
+        rc = _launch(table.device, _lib.lib().sd_bucket_bias_fwd, table.data_ptr(), index.data_ptr(), out.data_ptr(), _DT[table.dtype], nb, heads, index.numel())
         _lib.check(rc, 'sd_bucket_bias_fwd')
         ctx.plan = plan
         return out
@@ -71,9 +70,8 @@ class _BucketBiasFunction(torch.autograd.Function):
         dtable = torch.empty(nb, heads, dtype=d.dtype, device=d.device)
         ws_bytes = L.sd_bucket_bias_workspace_bytes(nb, chunks, heads)
         ws = torch.empty(ws_bytes, dtype=torch.uint8, device=d.device) if ws_bytes else None
-        with _launch_on(d.device) as stream:
-            rc = L.sd_bucket_bias_bwd(d.data_ptr(), order.data_ptr(), start.data_ptr(), by_pair.data_ptr(), bucket.data_ptr(), dtable.data_ptr(), _DT[d.dtype], nb, chunks, heads,
-                                      order.numel(), _ptr(ws), ws_bytes, stream)
+        rc = _launch(d.device, L.sd_bucket_bias_bwd, d.data_ptr(), order.data_ptr(), start.data_ptr(), by_pair.data_ptr(), bucket.data_ptr(), dtable.data_ptr(),
+                     _DT[d.dtype], nb, chunks, heads, order.numel(), _ptr(ws), ws_bytes)
         _lib.check(rc, 'sd_bucket_bias_bwd')
         return dtable, None
 

@@ -8,7 +8,7 @@ import os
 import torch
 
 from . import _lib
-from .ops import _DT, _launch_on, _no_double_backward, _ptr, _require_gpu, _stream_ptr
+from .ops import _DT, _launch, _no_double_backward, _ptr, _require_gpu, _stream_ptr
 
 ENABLED = os.environ.get('SEGDISTILL_WINDOW_ATTN', '1') == '1'       # A/B: 0 = F.scaled_dot_product_attention with a materialised additive tensor
 
@@ -62,9 +62,8 @@ class _WindowAttentionFunction(torch.autograd.Function):
         floats = L.sd_window_attn_train_packed_floats(heads, nw, n)
         packed = torch.empty(floats, dtype=torch.float32, device=qkv.device)
         out = torch.empty(bw, n, c3 // 3, dtype=qkv.dtype, device=qkv.device)
-        with _launch_on(qkv.device) as stream:
-            rc = L.sd_window_attn_train_fwd(qkv.data_ptr(), b.data_ptr(), _ptr(m), packed.data_ptr(), floats, out.data_ptr(), dt, bw, nw, heads, n,
-                                            c3 // 3 // heads, scale, stream)
+        rc = _launch(qkv.device, L.sd_window_attn_train_fwd, qkv.data_ptr(), b.data_ptr(), _ptr(m), packed.data_ptr(), floats, out.data_ptr(), dt, bw, nw, heads,
+                     n, c3 // 3 // heads, scale)
         _lib.check(rc, 'sd_window_attn_train_fwd')
         ctx.save_for_backward(qkv, packed)
         ctx.meta = (nw, heads, scale, bias.dtype)
@@ -84,9 +83,8 @@ class _WindowAttentionFunction(torch.autograd.Function):
         dbias = torch.empty(heads, n, n, dtype=torch.float32, device=qkv.device)
         ws_bytes = L.sd_window_attn_train_workspace_bytes(dt, bw, heads, n)
         ws = torch.empty(ws_bytes, dtype=torch.uint8, device=qkv.device)
-        with _launch_on(qkv.device) as stream:
-            rc = L.sd_window_attn_train_bwd(qkv.data_ptr(), packed.data_ptr(), packed.numel(), go.data_ptr(), dqkv.data_ptr(), dbias.data_ptr(), dt, bw, nw, heads,
-                                            n, c3 // 3 // heads, scale, ws.data_ptr(), ws_bytes, stream)
+        rc = _launch(qkv.device, L.sd_window_attn_train_bwd, qkv.data_ptr(), packed.data_ptr(), packed.numel(), go.data_ptr(), dqkv.data_ptr(), dbias.data_ptr(), dt,
+                     bw, nw, heads, n, c3 // 3 // heads, scale, ws.data_ptr(), ws_bytes)
         _lib.check(rc, 'sd_window_attn_train_bwd')
         return dqkv, dbias.to(bias_dtype), None, None, None
 
