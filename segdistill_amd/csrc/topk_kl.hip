@@ -68,16 +68,18 @@ __global__ __launch_bounds__(1024) void topk_kl_finish(const double *__restrict_
     }
 }
 
-// ---- class planes [B, C, P]: one thread per pixel ------------------------------------------------------------------------------------------------
-// The pixel's set A is a bit mask in LDS, a column per thread: words[w][thread].  Classes come by in ascending order, so the entries are met in
+// ---- class planes [B, C, P]: 64 pixels per workgroup, a quarter of the classes per wave ---------------------------------------------------------
+// The pixel's set A is a bit mask in LDS, a column per pixel: words[w][pixel].  Classes come by in ascending order, so the entries are met in
 // ascending order too, and the rank of an entry -- the bits below it -- is its place in a second column: no search, no sort, and a class that
-// appears twice has one place.
-constexpr int BT = 64;      // pixels per workgroup: one wave (four of them were no faster at 131072 pixels, and slower on small maps)
+// appears twice has one place.  No branch per class either: a class outside A writes to (reads from) the column's spare place.
+// Four waves share the pixels because one wave's walk over the classes is a chain of latencies: a map of 2 x 21 x 44 pixels and 236 classes took 50 us
+// each way with one wave per 64 pixels.
+constexpr int BT = 64, kWaves = 4;
 struct Columns {
     unsigned *words, *ranks;
     float *vals;
-    __device__ Columns(unsigned char *lds, int nwords) {
-        words = reinterpret_cast<unsigned *>(lds) + threadIdx.x;
+    __device__ Columns(unsigned char *lds, int nwords, int lane) {
+        words = reinterpret_cast<unsigned *>(lds) + lane;
         ranks = words + (size_t)nwords * BT;
         vals = reinterpret_cast<float *>(ranks + (size_t)nwords * BT);
     }
@@ -121,54 +123,68 @@ __device__ __forceinline__ int take_entries(const Columns &col, int nwords, cons
     return n;
 }
 
+// classes of one wave: a multiple of the eight that are fetched together
+__device__ __forceinline__ int classes_per_wave(int C) { return ((C + 7) / 8 + kWaves - 1) / kWaves * 8; }
+
 template <typename T>
-__global__ __launch_bounds__(BT) void topk_kl_planes_fwd(const T *__restrict__ S, Entries e, float4 *__restrict__ stats, double *__restrict__ part, int C, long P,
-                                                         int blocks_per_image, int nwords, float c2) {
+__global__ __launch_bounds__(BT *kWaves) void topk_kl_planes_fwd(const T *__restrict__ S, Entries e, float4 *__restrict__ stats, double *__restrict__ part, int C, long P,
+                                                                 int blocks_per_image, int nwords, float c2) {
     extern __shared__ __attribute__((aligned(16))) unsigned char lds[];
-    constexpr int U = 16;                                              // divides the 32 bits of a mask word
-    const Columns col(lds, nwords);
+    __shared__ Online lows[kWaves][BT];
+    constexpr int U = 8;                                               // divides the 32 bits of a mask word
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const Columns col(lds, nwords, lane);
     const long b = blockIdx.x / blocks_per_image;
-    const long p = (long)(blockIdx.x - b * blocks_per_image) * BT + threadIdx.x;
-    const size_t row = (size_t)b * P + p;
-    double kl = 0, counted = 0;
-    if (p < P && (!e.valid || e.valid[row])) {
-        counted = 1;
-        const size_t at = (size_t)b * e.k * P + p;
-        // the tile's address is uniform, the lane only adds its number: one scalar add per class.  A chunk is on its way while the one before it is folded.
-        const T *tile = S + (size_t)b * C * P + (p - threadIdx.x);
-        Online low = {-INFINITY, 0.f};
-        int next = 0;
-        float z[2][U];
-        auto fetch = [&](float (&to)[U], int c0) {
-            const T *at_c = tile + (size_t)c0 * P;
+    const long p0 = (long)(blockIdx.x - b * blocks_per_image) * BT, p = p0 + lane;
+    const size_t row = (size_t)b * P + p, at = (size_t)b * e.k * P + p;
+    const bool active = p < P && (!e.valid || e.valid[row]);
+    const int lo = min(wave * classes_per_wave(C), C), hi = min(lo + classes_per_wave(C), C);
+    // the tile's address is uniform, the lane only adds its number: one scalar add per class.  A chunk is on its way while the one before it is folded.
+    const T *tile = S + (size_t)b * C * P + p0;
+    float z[2][U];
+    auto fetch = [&](float (&to)[U], int c0) {
+        const T *at_c = tile + (size_t)c0 * P;
 #pragma unroll
-            for (int u = 0; u < U; ++u) {
-                to[u] = c0 + u < C ? VecIO<T>::load1(at_c + threadIdx.x) : -INFINITY;
-                at_c += P;
-            }
-        };
+        for (int u = 0; u < U; ++u) {
+            to[u] = c0 + u < hi ? VecIO<T>::load1(at_c + lane) : -INFINITY;
+            at_c += P;
+        }
+    };
+    Online t = {-INFINITY, 0.f}, low = {-INFINITY, 0.f};
+    int members = 0;
+    if (active) {
+        if (lo < hi) fetch(z[0], lo);
+        if (wave == 0) members = take_entries(col, nwords, e, at, row, P, C, c2, t);
+    }
+    __syncthreads();
+    if (active && lo < hi) {
+        int next = col.rank(lo);
         auto fold = [&](float (&x)[U], int c0) {
             unsigned word = col.words[(c0 >> 5) * BT] >> (c0 & 31);
 #pragma unroll
             for (int u = 0; u < U; ++u) {
-                if (word & 1) {
-                    col.vals[next * BT] = x[u];
-                    ++next;
-                    x[u] = -INFINITY;
-                }
+                const bool in = word & 1;
+                col.vals[(in ? next : e.k) * BT] = x[u];               // place e.k is the spare one (waves share it: nobody reads it)
+                next += in;
+                x[u] = in ? -INFINITY : x[u];
                 word >>= 1;
             }
             online_fold(low, x, c2);
         };
-        fetch(z[0], 0);
-        Online t;
-        const int members = take_entries(col, nwords, e, at, row, P, C, c2, t);
-        for (int c0 = 0; c0 < C; c0 += 2 * U) {
-            if (c0 + U < C) fetch(z[1], c0 + U);
+        for (int c0 = lo; c0 < hi; c0 += 2 * U) {
+            if (c0 + U < hi) fetch(z[1], c0 + U);
             fold(z[0], c0);
-            if (c0 + 2 * U < C) fetch(z[0], c0 + 2 * U);
-            if (c0 + U < C) fold(z[1], c0 + U);
+            if (c0 + 2 * U < hi) fetch(z[0], c0 + 2 * U);
+            if (c0 + U < hi) fold(z[1], c0 + U);
         }
+    }
+    lows[wave][lane] = low;
+    __syncthreads();
+    if (wave) return;
+    double kl = 0;
+    if (active) {
+#pragma unroll
+        for (int w = 1; w < kWaves; ++w) low = online_merge(low, lows[w][lane], c2);
         float m = low.m;
         for (int j = 0; j < members; ++j) m = fmaxf(m, col.vals[j * BT]);
         const float r = finite_ref(m);
@@ -177,8 +193,9 @@ __global__ __launch_bounds__(BT) void topk_kl_planes_fwd(const T *__restrict__ S
         for (int j = 0; j < members; ++j) s += ex2((col.vals[j * BT] - r) * c2);
         const float inv_s = 1.f / s, log_s = logf(s), tau_inv = c2 * kLn2;
         const float tr = finite_ref(t.m), inv_t = 1.f / t.s, log_t = logf(t.s);
+        const bool says = t.s > 0.f || t.s != t.s;
         float pr = 0.f, w = 0.f, k = 0.f;
-        if (t.s > 0.f || t.s != t.s) {
+        if (says) {
             for (int j0 = 0; j0 < e.k; j0 += kBatch) {
                 int c[kBatch];
                 float v[kBatch];
@@ -199,76 +216,78 @@ __global__ __launch_bounds__(BT) void topk_kl_planes_fwd(const T *__restrict__ S
             kl = (double)k;
         }
         // a row whose teacher says nothing (no live entry, no rest) has no loss and no gradient: 1 / s = 0 and w = 0 say so to the backward
-        stats[row] = t.s > 0.f || t.s != t.s ? make_float4(finite_ref(low.m), w, r, inv_s) : make_float4(0.f, 0.f, r, 0.f);
+        stats[row] = says ? make_float4(finite_ref(low.m), w, r, inv_s) : make_float4(0.f, 0.f, r, 0.f);
     }
-    write_partial<BT>(kl, counted, part);
+    double counted = active ? 1 : 0;
+#pragma unroll
+    for (int d = 32; d > 0; d >>= 1) kl += __shfl_xor(kl, d, 64), counted += __shfl_xor(counted, d, 64);
+    if (lane == 0) part[2 * (size_t)blockIdx.x] = kl, part[2 * (size_t)blockIdx.x + 1] = counted;
 }
 
 template <typename T>
-__global__ __launch_bounds__(BT) void topk_kl_planes_bwd(const T *__restrict__ S, Entries e, const float4 *__restrict__ stats, const float *__restrict__ inv_n,
-                                                         const float *__restrict__ upstream, T *__restrict__ dS, int C, long P, int blocks_per_image, int nwords,
-                                                         float c2, float coef) {
+__global__ __launch_bounds__(BT *kWaves) void topk_kl_planes_bwd(const T *__restrict__ S, Entries e, const float4 *__restrict__ stats, const float *__restrict__ inv_n,
+                                                                 const float *__restrict__ upstream, T *__restrict__ dS, int C, long P, int blocks_per_image, int nwords,
+                                                                 float c2, float coef) {
     extern __shared__ __attribute__((aligned(16))) unsigned char lds[];
-    constexpr int U = 16;                                              // divides the 32 bits of a mask word
-    const Columns col(lds, nwords);
+    constexpr int U = 8;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const Columns col(lds, nwords, lane);
     const long b = blockIdx.x / blocks_per_image;
-    const long p = (long)(blockIdx.x - b * blocks_per_image) * BT + threadIdx.x;
-    const size_t row = (size_t)b * P + p;
-    if (p >= P) return;
-    T *pd = dS + (size_t)b * C * P + p;
-    const float4 st = !e.valid || e.valid[row] ? stats[row] : make_float4(0.f, 0.f, 0.f, 0.f);
-    if (st.y == 0.f && st.w == 0.f) {
-        for (int c = 0; c < C; ++c) VecIO<T>::store1(pd + (size_t)c * P, 0.f);
-        return;
-    }
-    const float g = coef * inv_n[0] * upstream[0];
-    const size_t at = (size_t)b * e.k * P + p;
-    const T *tile = S + (size_t)b * C * P + (p - threadIdx.x);
-    T *dtile = dS + (size_t)b * C * P + (p - threadIdx.x);
-    const float w = st.y * g, inv_s = st.w;
-    int next = 0;
+    const long p0 = (long)(blockIdx.x - b * blocks_per_image) * BT, p = p0 + lane;
+    const size_t row = (size_t)b * P + p, at = (size_t)b * e.k * P + p;
+    const float4 st = p < P && (!e.valid || e.valid[row]) ? stats[row] : make_float4(0.f, 0.f, 0.f, 0.f);
+    const bool active = st.y != 0.f || st.w != 0.f;                    // otherwise the row's gradient is 0 and nothing of it is read
+    const int lo = min(wave * classes_per_wave(C), C), hi = min(lo + classes_per_wave(C), C);
+    const T *tile = S + (size_t)b * C * P + p0;
+    T *dtile = dS + (size_t)b * C * P + p0;
     float z[2][U];
     auto fetch = [&](float (&to)[U], int c0) {
         const T *at_c = tile + (size_t)c0 * P;
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            to[u] = c0 + u < C ? VecIO<T>::load1(at_c + threadIdx.x) : 0.f;
+            to[u] = active && c0 + u < hi ? VecIO<T>::load1(at_c + lane) : 0.f;
             at_c += P;
         }
     };
+    if (lo < hi) fetch(z[0], lo);
+    if (wave == 0 && active) {
+        Online t;
+        const int members = take_entries(col, nwords, e, at, row, P, C, c2, t);
+        const float tr = finite_ref(t.m), inv_t = 1.f / t.s;
+        for (int j = 0; j < members; ++j) col.vals[j * BT] = 0.f;
+        for (int j0 = 0; j0 < e.k; j0 += kBatch) {
+            int c[kBatch];
+            float v[kBatch];
+            load_batch(e, at, P, C, j0, c, v);
+#pragma unroll
+            for (int u = 0; u < kBatch; ++u)
+                if (c[u] >= 0) col.vals[col.rank(c[u]) * BT] += ex2((v[u] - tr) * c2) * inv_t;
+        }
+    }
+    __syncthreads();
+    if (p >= P || lo >= hi) return;
+    const float g = coef * inv_n[0] * upstream[0], w = st.y * g, inv_s = st.w;
+    int next = active ? col.rank(lo) : 0;
     auto write = [&](const float (&x)[U], int c0) {
-        unsigned word = col.words[(c0 >> 5) * BT] >> (c0 & 31);
+        unsigned word = active ? col.words[(c0 >> 5) * BT] >> (c0 & 31) : 0u;
         T *at_c = dtile + (size_t)c0 * P;
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            float d = ex2((x[u] - st.x) * c2) * w;
-            if (word & 1) {
-                d = (ex2((x[u] - st.z) * c2) * inv_s - col.vals[next * BT]) * g;
-                ++next;
-            }
+            const bool in = word & 1;
+            const float v = col.vals[(in ? next : e.k) * BT];          // (outside A: whatever the spare place holds)
+            const float q = ex2((x[u] - (in ? st.z : st.x)) * c2);
+            const float d = in ? fmaf(q, inv_s, -v) * g : q * w;
+            next += in;
             word >>= 1;
-            if (c0 + u < C) VecIO<T>::store1(at_c + threadIdx.x, d);
+            if (c0 + u < hi) VecIO<T>::store1(at_c + lane, active ? d : 0.f);
             at_c += P;
         }
     };
-    fetch(z[0], 0);
-    Online t;
-    const int members = take_entries(col, nwords, e, at, row, P, C, c2, t);
-    const float tr = finite_ref(t.m), inv_t = 1.f / t.s;
-    for (int j = 0; j < members; ++j) col.vals[j * BT] = 0.f;
-    for (int j0 = 0; j0 < e.k; j0 += kBatch) {
-        int c[kBatch];
-        float v[kBatch];
-        load_batch(e, at, P, C, j0, c, v);
-#pragma unroll
-        for (int u = 0; u < kBatch; ++u)
-            if (c[u] >= 0) col.vals[col.rank(c[u]) * BT] += ex2((v[u] - tr) * c2) * inv_t;
-    }
-    for (int c0 = 0; c0 < C; c0 += 2 * U) {
-        if (c0 + U < C) fetch(z[1], c0 + U);
+    for (int c0 = lo; c0 < hi; c0 += 2 * U) {
+        if (c0 + U < hi) fetch(z[1], c0 + U);
         write(z[0], c0);
-        if (c0 + 2 * U < C) fetch(z[0], c0 + 2 * U);
-        if (c0 + U < C) write(z[1], c0 + U);
+        if (c0 + 2 * U < hi) fetch(z[0], c0 + 2 * U);
+        if (c0 + U < hi) write(z[1], c0 + U);
     }
 }
 
@@ -493,8 +512,8 @@ bool plan(long B, int C, long P, int k, Plan *pl) {
         return true;
     }
     pl->nwords = (C + 31) / 32;
-    const long column = 4L * (2 * pl->nwords + k);                      // bytes of LDS per pixel
-    if (column * BT > 64512) return false;                              // 64 KB less what the kernels hold besides
+    const long column = 4L * (2 * pl->nwords + k + 1);                  // bytes of LDS per pixel
+    if (column * BT > 62464) return false;                              // 64 KB less what the kernels hold besides
     pl->threads = BT;
     pl->lds = (int)column * BT;
     pl->per = (P + BT - 1) / BT;
@@ -512,7 +531,7 @@ int fwd_launch(const void *S, const Entries &e, long B, int C, long P, const Pla
         if (pl.threads == 64) hipLaunchKernelGGL((topk_kl_rows_fwd<T, 64>), grid, dim3(256), pl.lds, st, s, e, stats, part, B, C, c2);
         else hipLaunchKernelGGL((topk_kl_rows_fwd<T, 256>), grid, dim3(256), pl.lds, st, s, e, stats, part, B, C, c2);
     } else {
-        hipLaunchKernelGGL((topk_kl_planes_fwd<T>), grid, dim3(BT), pl.lds, st, s, e, stats, part, C, P, (int)pl.per, pl.nwords, c2);
+        hipLaunchKernelGGL((topk_kl_planes_fwd<T>), grid, dim3(BT * kWaves), pl.lds, st, s, e, stats, part, C, P, (int)pl.per, pl.nwords, c2);
     }
     hipLaunchKernelGGL(topk_kl_finish, dim3(1), dim3(1024), 0, st, part, pl.blocks, alpha, loss, inv_n);
     return (int)hipGetLastError();
@@ -529,7 +548,7 @@ int bwd_launch(const void *S, const Entries &e, long B, int C, long P, const Pla
         else hipLaunchKernelGGL((topk_kl_rows_bwd<T, 256>), grid, dim3(256), 0, st, s, e, stats, inv_n, upstream, d, B, C, c2, coef);
     } else {
         const dim3 grid((unsigned)pl.blocks);
-        hipLaunchKernelGGL((topk_kl_planes_bwd<T>), grid, dim3(BT), pl.lds, st, s, e, stats, inv_n, upstream, d, C, P, (int)pl.per, pl.nwords, c2, coef);
+        hipLaunchKernelGGL((topk_kl_planes_bwd<T>), grid, dim3(BT * kWaves), pl.lds, st, s, e, stats, inv_n, upstream, d, C, P, (int)pl.per, pl.nwords, c2, coef);
     }
     return (int)hipGetLastError();
 }

@@ -36,7 +36,7 @@ class BucketPlan(nn.Module):
         owner = torch.repeat_interleave(torch.arange(nb, device=flat.device), chunks)
         within = torch.arange(owner.numel(), device=flat.device) - bucket_chunk[owner]
         start = (torch.cumsum(count, 0) - count)[owner] + within * CHUNK
-        self.num_buckets, self.shape = nb, tuple(index.shape)
+        self.num_buckets, self.num_chunks, self.num_pairs, self.shape = nb, owner.numel(), flat.numel(), tuple(index.shape)
         self.register_buffer('index', flat.int().view(index.shape), persistent=False)
         self.register_buffer('order', order.int(), persistent=False)
         self.register_buffer('chunk_start', torch.cat([start, start.new_tensor([flat.numel()])]).int(), persistent=False)
@@ -52,9 +52,9 @@ class _BucketBiasFunction(torch.autograd.Function):
     @staticmethod
     def forward(ctx, table, plan):
         nb, heads = table.shape
-        index = plan._buffers['index']
         out = torch.empty((heads,) + plan.shape, dtype=table.dtype, device=table.device)
-        rc = _launch(table.device, _lib.lib().sd_bucket_bias_fwd, table.data_ptr(), index.data_ptr(), out.data_ptr(), _DT[table.dtype], nb, heads, index.numel())
+        rc = _launch(table.device, _lib.lib().sd_bucket_bias_fwd, table.data_ptr(), plan._buffers['index'].data_ptr(), out.data_ptr(), _DT[table.dtype], nb, heads,
+                     plan.num_pairs)
         _lib.check(rc, 'sd_bucket_bias_fwd')
         ctx.plan = plan
         return out
@@ -63,15 +63,15 @@ class _BucketBiasFunction(torch.autograd.Function):
     def backward(ctx, grad_out):
         _no_double_backward('bucket_bias')
         plan = ctx.plan
-        order, start, by_pair, bucket = (plan._buffers[n] for n in ('order', 'chunk_start', 'chunk_order', 'bucket_chunk'))
+        held, nb, chunks = plan._buffers, plan.num_buckets, plan.num_chunks
         d = grad_out.contiguous()
-        heads, nb, chunks = d.shape[0], plan.num_buckets, start.numel() - 1
+        heads = d.shape[0]
         L = _lib.lib()
         dtable = torch.empty(nb, heads, dtype=d.dtype, device=d.device)
-        ws_bytes = L.sd_bucket_bias_workspace_bytes(nb, chunks, heads)
+        ws_bytes = L.sd_bucket_bias_workspace_bytes(nb, chunks, heads) if chunks > nb else 0
         ws = torch.empty(ws_bytes, dtype=torch.uint8, device=d.device) if ws_bytes else None
-        rc = _launch(d.device, L.sd_bucket_bias_bwd, d.data_ptr(), order.data_ptr(), start.data_ptr(), by_pair.data_ptr(), bucket.data_ptr(), dtable.data_ptr(),
-                     _DT[d.dtype], nb, chunks, heads, order.numel(), _ptr(ws), ws_bytes)
+        rc = _launch(d.device, L.sd_bucket_bias_bwd, d.data_ptr(), held['order'].data_ptr(), held['chunk_start'].data_ptr(), held['chunk_order'].data_ptr(),
+                     held['bucket_chunk'].data_ptr(), dtable.data_ptr(), _DT[d.dtype], nb, chunks, heads, plan.num_pairs, _ptr(ws), ws_bytes)
         _lib.check(rc, 'sd_bucket_bias_bwd')
         return dtable, None
 

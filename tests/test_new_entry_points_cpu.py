@@ -49,7 +49,7 @@ def test_topk_kl_refusals(L):
         assert f(S=P + 1) == E_ALIGN and f(st=P + 4) == E_ALIGN and f(vdt=1, v=P + 1) == E_ALIGN and f(r=P + 2) == E_ALIGN
     assert fwd(wb=ws - 1) == E_WS and fwd(w=P + 4) == E_WS and bwd(d=P + 2) == E_ALIGN
     assert L.sd_topk_kl_supported(8, 150, 16384, 128) and L.sd_topk_kl_supported(4, 262144, 1, 128) and not L.sd_topk_kl_supported(2 ** 40, 150, 1, 3)
-    for C in (1, 31, 32, 33, 150, 1984):                                     # what is called supported fits the LDS that a launch may ask for
+    for C in (1, 31, 32, 33, 150, 1760):                                     # what is called supported fits the LDS that a launch may ask for
         for k in (1, 10, 64, 128):
             assert L.sd_topk_kl_supported(1, C, 7, k)
 
