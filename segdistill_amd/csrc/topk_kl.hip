@@ -503,7 +503,8 @@ struct Plan {
 bool plan(long B, int C, long P, int k, Plan *pl) {
     if (P == 1) {
         pl->nwords = row_words(C);
-        pl->threads = C <= 2048 ? 64 : 256;
+        // a wave per short row; a long one by four waves, or by sixteen where there are too few rows to fill the 256 CUs with fours
+        pl->threads = C <= 2048 ? 64 : B >= 1024 ? 256 : 1024;
         const long wgs = pl->threads == 64 ? (B + 3) / 4 : B;
         if (wgs > kMaxBlocks) return false;
         pl->blocks = (int)(wgs < 4096 ? wgs : 4096);
@@ -529,7 +530,8 @@ int fwd_launch(const void *S, const Entries &e, long B, int C, long P, const Pla
     const dim3 grid((unsigned)pl.blocks);
     if (P == 1) {
         if (pl.threads == 64) hipLaunchKernelGGL((topk_kl_rows_fwd<T, 64>), grid, dim3(256), pl.lds, st, s, e, stats, part, B, C, c2);
-        else hipLaunchKernelGGL((topk_kl_rows_fwd<T, 256>), grid, dim3(256), pl.lds, st, s, e, stats, part, B, C, c2);
+        else if (pl.threads == 256) hipLaunchKernelGGL((topk_kl_rows_fwd<T, 256>), grid, dim3(256), pl.lds, st, s, e, stats, part, B, C, c2);
+        else hipLaunchKernelGGL((topk_kl_rows_fwd<T, 1024>), grid, dim3(1024), pl.lds, st, s, e, stats, part, B, C, c2);
     } else {
         hipLaunchKernelGGL((topk_kl_planes_fwd<T>), grid, dim3(BT * kWaves), pl.lds, st, s, e, stats, part, C, P, (int)pl.per, pl.nwords, c2);
     }
@@ -545,7 +547,8 @@ int bwd_launch(const void *S, const Entries &e, long B, int C, long P, const Pla
     if (P == 1) {
         const dim3 grid((unsigned)pl.per);
         if (pl.threads == 64) hipLaunchKernelGGL((topk_kl_rows_bwd<T, 64>), grid, dim3(256), 0, st, s, e, stats, inv_n, upstream, d, B, C, c2, coef);
-        else hipLaunchKernelGGL((topk_kl_rows_bwd<T, 256>), grid, dim3(256), 0, st, s, e, stats, inv_n, upstream, d, B, C, c2, coef);
+        else if (pl.threads == 256) hipLaunchKernelGGL((topk_kl_rows_bwd<T, 256>), grid, dim3(256), 0, st, s, e, stats, inv_n, upstream, d, B, C, c2, coef);
+        else hipLaunchKernelGGL((topk_kl_rows_bwd<T, 1024>), grid, dim3(1024), 0, st, s, e, stats, inv_n, upstream, d, B, C, c2, coef);
     } else {
         const dim3 grid((unsigned)pl.blocks);
         hipLaunchKernelGGL((topk_kl_planes_bwd<T>), grid, dim3(BT * kWaves), pl.lds, st, s, e, stats, inv_n, upstream, d, C, P, (int)pl.per, pl.nwords, c2, coef);
