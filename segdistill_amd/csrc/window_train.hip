@@ -497,7 +497,7 @@ int per_cu(size_t lds, int most) {
 template <typename T>
 int bwd_slabs(long windows, int heads, int N) { return slabs_for(windows, heads, per_cu(bwd_lds<T>(N), kBwdWaves * (N <= 32 ? 4 : 2))); }
 
-bool shape_ok(long windows, int heads, int N) { return windows > 0 && heads > 0 && windows <= 0x3fffffffL / heads && N >= 1 && N <= 64; }
+bool shape_ok(long windows, int heads, int N) { return windows > 0 && heads > 0 && heads <= 65535 && windows <= 0x3fffffffL / heads && N >= 1 && N <= 64; }
 size_t table_floats(int heads, int nW, int N) { return (size_t)(heads + nW) * (N <= 32 ? 1024 : 4096); }
 
 int check_args(const void *qkv, const float *packed, size_t packed_floats, int dtype, long windows, int nW, int heads, int N, int d) {

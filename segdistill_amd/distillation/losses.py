@@ -328,6 +328,8 @@ class TopKLoss(KLDLoss):
         return None
 
     def forward(self, x_student, x_teacher, gt, n_iter):
+        if x_student.shape[1] != x_teacher.shape[1]:
+            raise ValueError(f'TopKLoss: the student tap has {x_student.shape[1]} classes, the teacher tap {x_teacher.shape[1]}')
         alpha, alpha_t, _ = self._prepare(x_student, x_student.shape[1], n_iter)
         if self.resize_config:
             size = tuple(int(v) for v in (x_teacher if self.resize_config.get('target', 'gt') == 'teacher' else gt).shape[2:])

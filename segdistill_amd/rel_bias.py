@@ -56,22 +56,23 @@ class _BucketBiasFunction(torch.autograd.Function):
         rc = _launch(table.device, _lib.lib().sd_bucket_bias_fwd, table.data_ptr(), plan._buffers['index'].data_ptr(), out.data_ptr(), _DT[table.dtype], nb, heads,
                      plan.num_pairs)
         _lib.check(rc, 'sd_bucket_bias_fwd')
-        ctx.plan = plan
+        ctx.plan, ctx.held = plan, tuple(plan._buffers[n] for n in ('order', 'chunk_start', 'chunk_order', 'bucket_chunk'))      # (the plan may move meanwhile)
         return out
 
     @staticmethod
     def backward(ctx, grad_out):
         _no_double_backward('bucket_bias')
         plan = ctx.plan
-        held, nb, chunks = plan._buffers, plan.num_buckets, plan.num_chunks
+        order, start, by_pair, bucket = ctx.held
+        nb, chunks = plan.num_buckets, plan.num_chunks
         d = grad_out.contiguous()
         heads = d.shape[0]
         L = _lib.lib()
         dtable = torch.empty(nb, heads, dtype=d.dtype, device=d.device)
         ws_bytes = L.sd_bucket_bias_workspace_bytes(nb, chunks, heads) if chunks > nb else 0
         ws = torch.empty(ws_bytes, dtype=torch.uint8, device=d.device) if ws_bytes else None
-        rc = _launch(d.device, L.sd_bucket_bias_bwd, d.data_ptr(), held['order'].data_ptr(), held['chunk_start'].data_ptr(), held['chunk_order'].data_ptr(),
-                     held['bucket_chunk'].data_ptr(), dtable.data_ptr(), _DT[d.dtype], nb, chunks, heads, plan.num_pairs, _ptr(ws), ws_bytes)
+        rc = _launch(d.device, L.sd_bucket_bias_bwd, d.data_ptr(), order.data_ptr(), start.data_ptr(), by_pair.data_ptr(), bucket.data_ptr(),
+                     dtable.data_ptr(), _DT[d.dtype], nb, chunks, heads, plan.num_pairs, _ptr(ws), ws_bytes)
         _lib.check(rc, 'sd_bucket_bias_bwd')
         return dtable, None
 

@@ -110,3 +110,15 @@ def test_refusals():
             rel_bias.bucket_bias(bad, plan)
     with pytest.raises(TypeError):
         rel_bias.bucket_bias(torch.zeros(9, 2, device='cuda').half(), plan)
+
+
+def test_the_plan_may_move_between_forward_and_backward():
+    from segdistill_amd import rel_bias
+    plan = rel_bias.BucketPlan(_window_index(4, 4), 49).cuda()
+    table = torch.randn(49, 3, device='cuda', requires_grad=True)
+    out = rel_bias.bucket_bias(table, plan)
+    want = torch.autograd.grad(out, table, torch.ones_like(out), retain_graph=True)[0]
+    plan.cpu()
+    assert torch.equal(torch.autograd.grad(out, table, torch.ones_like(out), retain_graph=True)[0], want)
+    with pytest.raises(RuntimeError, match='second derivative'):
+        torch.autograd.grad(out, table, torch.ones_like(out), create_graph=True)

@@ -442,3 +442,56 @@ def test_refusals():
     loss = ops.topk_kl(e, ve, ie, re, tau=1.0, alpha=1.0)
     loss.backward()
     assert float(loss) == 0 and e.grad.shape == (0, 10)
+
+
+def test_two_calls_at_once_and_a_second_derivative():
+    """two criteria on the same leaf in one graph, on two streams at once; create_graph is refused instead of answered with constants"""
+    from segdistill_amd import ops
+    g = torch.Generator(device='cuda').manual_seed(13)
+    S = torch.randn(3, 4000, device='cuda', generator=g)
+    v, i, r = _teacher(S, 6, 1.0, g, torch.float32)
+    parts = []
+    for rest in (r, None):
+        a = S.clone().requires_grad_()
+        ops.topk_kl(a, v, i, rest, tau=1.0, alpha=1.0).backward()
+        parts.append(a.grad)
+    both = S.clone().requires_grad_()
+    (ops.topk_kl(both, v, i, r, tau=1.0, alpha=1.0) + ops.topk_kl(both, v, i, None, tau=1.0, alpha=1.0)).backward()
+    assert torch.equal(both.grad, parts[0] + parts[1])
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    out = []
+    for k, s in enumerate(streams * 3):
+        with torch.cuda.stream(s):
+            a = S.clone().requires_grad_()
+            loss = ops.topk_kl(a, v, i, (r, None)[k % 2], tau=1.0, alpha=1.0)
+            out.append((ops.topk_logits(a.detach(), 6), torch.autograd.grad(loss, a)[0]))
+    torch.cuda.synchronize()
+    want = ops.topk_logits(S, 6)
+    for k, (top, d) in enumerate(out):
+        assert torch.equal(d, parts[k % 2]) and all(torch.equal(p, q) for p, q in zip(top, want))
+    a = S.clone().requires_grad_()
+    with pytest.raises(RuntimeError, match='second derivative'):
+        torch.autograd.grad(ops.topk_kl(a, v, i, r, tau=1.0, alpha=1.0), a, create_graph=True)
+
+
+def test_module_refuses_taps_of_different_classes():
+    from segdistill_amd.distillation.losses import TopKLoss
+    with pytest.raises(ValueError, match='classes'):
+        TopKLoss(k=3)(torch.zeros(1, 19, 4, 4, device='cuda'), torch.zeros(1, 21, 4, 4, device='cuda'), torch.zeros(1, 1, 4, 4, device='cuda'), 1)
+
+
+def test_module_resizes_both_taps_to_the_label_size():
+    from segdistill_amd import ops
+    from segdistill_amd.distillation.losses import TopKLoss
+    g = torch.Generator(device='cuda').manual_seed(14)
+    s = torch.randn(2, 19, 9, 9, device='cuda', generator=g).requires_grad_()
+    t = torch.randn(2, 19, 9, 9, device='cuda', generator=g)
+    gt = torch.randint(0, 19, (2, 1, 36, 36), device='cuda', generator=g)
+    loss = TopKLoss(k=4, tau=2.0, alpha=2.0, rest=False, resize_config=dict(mode='bilinear', align_corners=False))(s, t, gt, 1)
+    su, tu = (torch.nn.functional.interpolate(x, size=(36, 36), mode='bilinear', align_corners=False) for x in (s, t))
+    v, i, r = ops.topk_logits(tu, 4, tau=2.0)
+    want = ops.topk_kl(su, v, i, None, tau=2.0, alpha=2.0)
+    assert float(loss) == pytest.approx(float(want), rel=1e-4)
+    a, b = torch.autograd.grad(loss, s)[0], torch.autograd.grad(want, s)[0]
+    assert float((a - b).norm() / b.norm()) < 1e-4
