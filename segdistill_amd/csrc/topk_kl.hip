@@ -28,8 +28,9 @@ __device__ __forceinline__ float entry_value(const Entries &e, size_t at) {
     return e.values_bf16 ? VecIO<bf16_t>::load1(static_cast<const bf16_t *>(e.values) + at) : static_cast<const float *>(e.values)[at];
 }
 
-// p log(p / q) with 0 log 0 = 0, from p and the logarithms
-__device__ __forceinline__ float kl_term(float p, float logp, float logq) { return p > 0.f || p != p ? p * (logp - logq) : 0.f; }
+// p log(p / q) with 0 log 0 = 0, from p and the logarithm of the ratio.  A row's last steps are in 64 bits: its KL is a small difference of logarithms of
+// size ten, whose rounding to 32 bits (5e-7) would be the loss's whole error where student and teacher agree.
+__device__ __forceinline__ double kl_term(double p, double log_ratio) { return p > 0 || p != p ? p * log_ratio : 0.0; }
 
 // The workgroup's sum of row losses and its number of counted rows -> part[2 * block], part[2 * block + 1].
 template <int NT>
@@ -189,13 +190,16 @@ __global__ __launch_bounds__(BT *kWaves) void topk_kl_planes_fwd(const T *__rest
         for (int j = 0; j < members; ++j) m = fmaxf(m, col.vals[j * BT]);
         const float r = finite_ref(m);
         const float qr_num = low.s * ex2((low.m - r) * c2);
-        float s = qr_num;
+        double s = qr_num;
         for (int j = 0; j < members; ++j) s += ex2((col.vals[j * BT] - r) * c2);
-        const float inv_s = 1.f / s, log_s = logf(s), tau_inv = c2 * kLn2;
-        const float tr = finite_ref(t.m), inv_t = 1.f / t.s, log_t = logf(t.s);
+        const float inv_s = (float)(1.0 / s), tr = finite_ref(t.m);
         const bool says = t.s > 0.f || t.s != t.s;
-        float pr = 0.f, w = 0.f, k = 0.f;
+        float w = 0.f;
         if (says) {
+            // the teacher's normaliser once more, then with it the terms: both walk the same entries
+            const double ti = (double)c2 * (double)kLn2;
+            const float er = e.rest ? ex2((e.rest[row] - tr) * c2) : 0.f;
+            double ts = er, terms = 0, weights = 0;                    // sum_j e_j (v_j - z_j) / tau and sum_j e_j over the live entries
             for (int j0 = 0; j0 < e.k; j0 += kBatch) {
                 int c[kBatch];
                 float v[kBatch];
@@ -203,17 +207,18 @@ __global__ __launch_bounds__(BT *kWaves) void topk_kl_planes_fwd(const T *__rest
 #pragma unroll
                 for (int u = 0; u < kBatch; ++u)
                     if (c[u] >= 0) {
-                        const float d = v[u] - tr, zq = col.vals[col.rank(c[u]) * BT] - r;
-                        k += kl_term(ex2(d * c2) * inv_t, d * tau_inv - log_t, zq * tau_inv - log_s);
+                        const float ej = ex2((v[u] - tr) * c2);
+                        const double d = ((double)v[u] - (double)tr) - ((double)col.vals[col.rank(c[u]) * BT] - (double)r);
+                        terms += kl_term(ej, d * ti);
+                        weights += ej;
                     }
             }
-            if (e.rest) {
-                const float v = e.rest[row] - tr;
-                pr = ex2(v * c2) * inv_t;
-                k += kl_term(pr, v * tau_inv - log_t, (low.m - r) * tau_inv + logf(low.s) - log_s);
-            }
-            w = low.s > 0.f || low.s != low.s ? (qr_num * inv_s - pr) / low.s : 0.f;
-            kl = (double)k;
+            ts += weights;
+            const double log_ratio = log(s) - log(ts), inv_t = 1.0 / ts;
+            kl = terms * inv_t + kl_term(weights * inv_t, log_ratio);
+            const double pr = er * inv_t;
+            if (e.rest) kl += kl_term(pr, (((double)e.rest[row] - (double)tr) - ((double)low.m - (double)r)) * ti - log((double)low.s) + log_ratio);
+            w = low.s > 0.f || low.s != low.s ? (float)((qr_num / s - pr) / low.s) : 0.f;
         }
         // a row whose teacher says nothing (no live entry, no rest) has no loss and no gradient: 1 / s = 0 and w = 0 say so to the backward
         stats[row] = says ? make_float4(finite_ref(low.m), w, r, inv_s) : make_float4(0.f, 0.f, r, 0.f);
@@ -343,7 +348,6 @@ __global__ __launch_bounds__(NT == 64 ? 256 : NT) void topk_kl_rows_fwd(const T 
     const int nwords = row_words(C);
     const int grp = NT == 64 ? threadIdx.x >> 6 : 0, tid = NT == 64 ? threadIdx.x & 63 : threadIdx.x;
     unsigned *bits = reinterpret_cast<unsigned *>(lds) + (size_t)grp * nwords;
-    const float tau_inv = c2 * kLn2;
     double kl = 0, counted = 0;
     for (int w = tid; w < nwords; w += NT) bits[w] = 0;
     for (long row = (long)blockIdx.x * G + grp; row < rows; row += (long)gridDim.x * G) {
@@ -407,30 +411,30 @@ __global__ __launch_bounds__(NT == 64 ? 256 : NT) void topk_kl_rows_fwd(const T 
             }
             m = wave_max(m);
             const float r = finite_ref(m), qr_num = low.s * ex2((low.m - r) * c2);
-            float s = 0.f;
+            // every lane's share of: the student's normaliser, the teacher's, sum_j e_j (v_j - z_j) / tau
+            const double ti = (double)c2 * (double)kLn2;
+            double s = 0, weights = 0, terms = 0;
 #pragma unroll
-            for (int h = 0; h < 2; ++h) s += x.first[h] ? ex2((zj[h] - r) * c2) : 0.f;
-            s = wave_sum(s) + qr_num;
-            const float inv_s = 1.f / s, log_s = logf(s), inv_t = 1.f / x.ts, log_t = logf(x.ts);
-            float k = 0.f;
-#pragma unroll
-            for (int h = 0; h < 2; ++h)
+            for (int h = 0; h < 2; ++h) {
+                s += x.first[h] ? ex2((zj[h] - r) * c2) : 0.f;
                 if (x.c[h] >= 0) {
-                    const float v = x.v[h] - x.tr;
-                    k += kl_term(ex2(v * c2) * inv_t, v * tau_inv - log_t, (zj[h] - r) * tau_inv - log_s);
+                    const float ej = ex2((x.v[h] - x.tr) * c2);
+                    terms += kl_term(ej, (((double)x.v[h] - (double)x.tr) - ((double)zj[h] - (double)r)) * ti);
+                    weights += ej;
                 }
-            k = wave_sum(k);
-            const bool says = x.ts > 0.f || x.ts != x.ts;
-            float pr = 0.f;
-            if (e.rest) {
-                const float v = e.rest[row] - x.tr;
-                pr = ex2(v * c2) * inv_t;
-                k += kl_term(pr, v * tau_inv - log_t, (low.m - r) * tau_inv + logf(low.s) - log_s);
             }
+#pragma unroll
+            for (int d = 32; d > 0; d >>= 1) s += __shfl_xor(s, d, 64), weights += __shfl_xor(weights, d, 64), terms += __shfl_xor(terms, d, 64);
+            s += qr_num;
+            const bool says = x.ts > 0.f || x.ts != x.ts;
+            const float er = e.rest ? ex2((e.rest[row] - x.tr) * c2) : 0.f;
+            const double ts = weights + er, log_ratio = log(s) - log(ts), inv_t = 1.0 / ts, pr = er * inv_t;
+            double k = terms * inv_t + kl_term(weights * inv_t, log_ratio);
+            if (e.rest) k += kl_term(pr, (((double)e.rest[row] - (double)x.tr) - ((double)low.m - (double)r)) * ti - log((double)low.s) + log_ratio);
             if (tid == 0) {
-                const float w = low.s > 0.f || low.s != low.s ? (qr_num * inv_s - pr) / low.s : 0.f;
-                stats[row] = says ? make_float4(finite_ref(low.m), w, r, inv_s) : make_float4(0.f, 0.f, r, 0.f);
-                kl += says ? (double)k : 0.0;
+                const float w = low.s > 0.f || low.s != low.s ? (float)((qr_num / s - pr) / low.s) : 0.f;
+                stats[row] = says ? make_float4(finite_ref(low.m), w, r, (float)(1.0 / s)) : make_float4(0.f, 0.f, r, 0.f);
+                kl += says ? k : 0.0;
                 counted += 1;
             }
 #pragma unroll
