@@ -564,7 +564,7 @@ int check_args(const void *S, const void *values, const int32_t *index, const fl
                Plan *pl) {
     if (!S || !values || !index) return SD_E_NULL;
     if ((dtype != SD_F32 && dtype != SD_BF16) || (values_dtype != SD_F32 && values_dtype != SD_BF16)) return SD_E_DTYPE;
-    if (B <= 0 || C <= 0 || P <= 0 || k <= 0 || B > 0x7fffffffL || P > 0x7fffffffL || !(tau > 0.f) || !isfinite(tau)) return SD_E_SHAPE;
+    if (B <= 0 || C <= 0 || P <= 0 || k <= 0 || B > 0x7fffffffL || P > 0x7fffffffL || !(tau >= kTauMin && tau <= kTauMax)) return SD_E_SHAPE;
     if (k > kTopkMax || C > kTopkMaxClasses || !plan(B, C, P, k, pl)) return SD_E_UNSUPPORTED;
     const uintptr_t es = dtype == SD_F32 ? 3 : 1, ev = values_dtype == SD_F32 ? 3 : 1;
     if ((reinterpret_cast<uintptr_t>(S) & es) || (reinterpret_cast<uintptr_t>(values) & ev) ||

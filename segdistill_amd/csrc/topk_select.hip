@@ -1,7 +1,7 @@
 // topk_select.hip -- the k largest logits of every row, their indices, and what the others weigh, gfx950.
 //
 //   values, index : descending, equal values by ascending index (NaN counts as the largest value, -0 equals +0)
-//   rest          : tau * log sum_{c not chosen} exp(x_c / tau)   (-inf when nothing is left over)
+//   rest          : tau * log sum_{c not chosen} exp(x_c / tau)   (-inf when nothing is left over, +inf and NaN where one of those is)
 // so that softmax([values, rest] / tau) is the row's softmax with everything unchosen folded into one more class.
 //
 // A row is a pixel's classes (stride P: class planes [B, C, P]) or contiguous (P == 1).  Both forms read the logits once from memory and write
@@ -63,7 +63,7 @@ __global__ __launch_bounds__(256) void topk_planes(const T *__restrict__ x, T *_
                     key[j] = above ? key[j > 0 ? j - 1 : 0] : (here ? n : key[j]);
                 }
             }
-            if (last) online_fold(low, out, c2);
+            if (last) online_fold<true>(low, out, c2);
         }
         const int take = last ? k - base : K;
 #pragma unroll
@@ -74,7 +74,7 @@ __global__ __launch_bounds__(256) void topk_planes(const T *__restrict__ x, T *_
                 index[o] = idx[j];
             } else {
                 const float left[1] = {of_key(key[j] < kMinusInfKey ? kMinusInfKey : key[j])};
-                online_fold(low, left, c2);
+                online_fold<true>(low, left, c2);
             }
         }
         bound_key = key[K - 1], bound_idx = idx[K - 1];
@@ -168,7 +168,7 @@ __global__ __launch_bounds__(64) void topk_planes_lds(const T *__restrict__ x, T
 #pragma unroll
         for (int g = 0; g < NG; ++g) m = max(m, top[g]);
         m = max(m, __shfl_xor(m, 32, 64));
-        const float ref = finite_ref(of_key(m));
+        const float ref = finite_ref<true>(of_key(m));
         float s = 0.f;
 #pragma unroll
         for (int g = 0; g < NG; ++g)
@@ -306,7 +306,7 @@ __device__ __forceinline__ Online exact_entries(const Row<T, NT, NV> &row, Selec
             out[i] = n < kth ? a[i] : -INFINITY;
             if (n > kth) sh.entry[atomicAdd(&sh.count, 1)] = entry_of(n, i0 + i);          // k - need of them
         }
-        online_fold(low, out, c2);
+        online_fold<true>(low, out, c2);
     });
     for (int base = 0, taken = 0; taken < need; base += NT) {        // the first `need` ties in index order; there are that many
         const int i = base + tid;
@@ -328,7 +328,7 @@ __device__ __forceinline__ Online exact_entries(const Row<T, NT, NV> &row, Selec
     }
     if (tid == 0 && ties > need) {
         const Online t = {of_key(kth), (float)(ties - need)};
-        low = online_merge(low, t, c2);
+        low = online_merge<true>(low, t, c2);
     }
     group_sync<NT>();
     return low;
@@ -438,7 +438,7 @@ __global__ __launch_bounds__(NT == 64 ? 256 : NT, WAVES) void topk_rows(const T 
     int count = sh.count;
     const bool exact = count > CAP || sh.odd;
     if (exact) {
-        const Online low = online_group<NT>(exact_entries(row, sh, tid, k, c2), sh.tmp, tid, c2);
+        const Online low = online_group<NT, true>(exact_entries(row, sh, tid, k, c2), sh.tmp, tid, c2);
         if (tid == 0) sh.tmp[0] = low;
         count = k;
         group_sync<NT>();
@@ -473,10 +473,10 @@ __global__ __launch_bounds__(NT == 64 ? 256 : NT, WAVES) void topk_rows(const T 
         Online l = {-INFINITY, 0.f};
         for (int c = tid & 63; c < count - k; c += 64) {
             const float left[1] = {sh.left[c]};
-            online_fold(l, left, c2);
+            online_fold<true>(l, left, c2);
         }
         const Online b = {total > 0.f ? bound : -INFINITY, total};
-        low = count > k ? online_merge(online_group<64>(l, nullptr, 0, c2), b, c2) : b;
+        low = count > k ? online_merge<true>(online_group<64, true>(l, nullptr, 0, c2), b, c2) : b;
         if (low.s < 0x1p-64f && k < V) {          // what is left lies far below the bound (or is -inf): relative to its own maximum
             const unsigned long long last = sh.last;
             low = {-INFINITY, 0.f};
@@ -485,22 +485,32 @@ __global__ __launch_bounds__(NT == 64 ? 256 : NT, WAVES) void topk_rows(const T 
                 float out[M];
 #pragma unroll
                 for (int i = 0; i < M; ++i) out[i] = entry_of(key_of(a[i]), i0 + i) < last ? a[i] : -INFINITY;
-                online_fold(low, out, c2);
+                online_fold<true>(low, out, c2);
             });
-            low = online_group<NT>(low, sh.tmp, tid, c2);
+            low = online_group<NT, true>(low, sh.tmp, tid, c2);
         }
     }
     if (tid == 0) rest[r] = low.s > 0.f || low.s != low.s ? low.m + tau * logf(low.s) : -INFINITY;
 }
 
+// A launch holds fewer than 2^32 threads: more rows than that go in several.
+template <typename T, int NT, int NV, int WAVES>
+void rows_launch_as(const T *x, T *values, int32_t *index, float *rest, long rows, int V, int k, float tau, float c2, hipStream_t st) {
+    constexpr int G = NT == 64 ? 4 : 1, threads = NT == 64 ? 256 : NT;
+    const long most = kMaxBlocks * 256 / threads * G;
+    for (long r = 0; r < rows; r += most) {
+        const long n = rows - r < most ? rows - r : most;
+        hipLaunchKernelGGL((topk_rows<T, NT, NV, WAVES>), dim3((unsigned)((n + G - 1) / G)), dim3(threads), 0, st, x + (size_t)r * V, values + (size_t)r * k,
+                           index + (size_t)r * k, rest + r, n, V, k, tau, c2);
+    }
+}
+
 // Threads and registers by the row's bytes: a wave per row up to 8 KB (its 64 group maxima serve k <= 32), else a workgroup whose registers hold the row.
 template <typename T>
 int rows_launch(const T *x, T *values, int32_t *index, float *rest, long rows, int V, int k, float tau, float c2, hipStream_t st) {
-    if (rows > kMaxBlocks / 4) return SD_E_SHAPE;     // workgroups of up to 1024 threads
+    if (rows > 0x3fffffffL) return SD_E_SHAPE;
     const long bytes = (long)V * (long)sizeof(T);
-#define SD_ROWS(NT, NV, WAVES)                                                                                                                              \
-    hipLaunchKernelGGL((topk_rows<T, NT, NV, WAVES>), dim3((unsigned)(NT == 64 ? (rows + 3) / 4 : rows)), dim3(NT == 64 ? 256 : NT), 0, st, x, values, index, \
-                       rest, rows, V, k, tau, c2)
+#define SD_ROWS(NT, NV, WAVES) rows_launch_as<T, NT, NV, WAVES>(x, values, index, rest, rows, V, k, tau, c2, st)
     if (k <= 32 && bytes <= 2048) SD_ROWS(64, 2, 8);
     else if (k <= 32 && bytes <= 8192) SD_ROWS(64, 8, 5);
     else if (bytes <= 16384) SD_ROWS(256, 4, 6);
@@ -548,7 +558,7 @@ int sd_topk_max_classes(void) { return sd::kTopkMaxClasses; }
 int sd_topk_select(const void *x, void *values, int32_t *index, float *rest, int dtype, long B, int C, long P, int k, float tau, void *stream) {
     if (!x || !values || !index || !rest) return SD_E_NULL;
     if (dtype != SD_F32 && dtype != SD_BF16) return SD_E_DTYPE;
-    if (B <= 0 || C <= 0 || P <= 0 || k <= 0 || k > C || B > 0x7fffffffL || P > 0x7fffffffL || !(tau > 0.f) || !isfinite(tau)) return SD_E_SHAPE;
+    if (B <= 0 || C <= 0 || P <= 0 || k <= 0 || k > C || B > 0x7fffffffL || P > 0x7fffffffL || !(tau >= sd::kTauMin && tau <= sd::kTauMax)) return SD_E_SHAPE;
     if (k > sd::kTopkMax || C > sd::kTopkMaxClasses) return SD_E_UNSUPPORTED;
     const uintptr_t es = dtype == SD_F32 ? 4 : 2;
     if (((reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(values)) & (es - 1)) ||

@@ -679,8 +679,8 @@ def _entry_shape(x, k):
 
 def _check_tau(tau):
     tau = float(tau)
-    if not (tau > 0 and math.isfinite(tau)):
-        raise ValueError(f'tau must be a positive number, got {tau}')
+    if not 1e-37 <= tau <= 1e37:                                       # 1 / tau and what it is multiplied by stay normal fp32 numbers
+        raise ValueError(f'tau must be a positive number (1e-37 .. 1e37), got {tau}')
     return tau
 
 
@@ -690,7 +690,7 @@ def topk_logits(x, k, *, tau=1.0):
 
     x: class planes [B, C, H, W] (-> values, index [B, k, H, W], rest [B, H, W]) or rows with the classes last ([R, C], [B, N, C] -> [..., k],
     [...]); fp32 or bf16.  values descend (equal ones by ascending class; NaN counts as the largest), index is int32, rest is fp32 and stands for
-    all other classes at this temperature: tau * log(sum of exp(x / tau) over them), -inf for k = C.  No gradient."""
+    all other classes at this temperature: tau * log(sum of exp(x / tau) over them), -inf for k = C, inf or NaN where a class left over is.  No gradient."""
     _require_gpu(x)
     B, Cc, P = _class_layout(x, 'topk_logits')
     if x.dtype not in _DT:

@@ -127,3 +127,14 @@ def test_cpu_tensors_are_refused():
         window_attn.attention(torch.zeros(1, 4, 96), torch.zeros(1, 4, 4), None, 1, 1.0)
     with pytest.raises(RuntimeError, match='GPU only'):
         TopKLoss(k=2)(torch.zeros(1, 3, 2, 2), torch.zeros(1, 3, 2, 2), torch.zeros(1, 1, 4, 4), 1)
+
+
+def test_temperatures_whose_reciprocal_is_no_normal_number_are_refused(L):
+    from segdistill_amd import ops
+    for tau in (1e-39, 3e-39, 2e38, 3.4e38):
+        assert L.sd_topk_select(P, P, P, P, 0, 2, 10, 1, 3, tau, NULL) == E_SHAPE
+        assert L.sd_topk_kl_fwd(P, P, P, NULL, NULL, 0, 0, 2, 10, 6, 3, tau, 1.0, P, P, P, P, 1 << 20, NULL) == E_SHAPE
+    for tau in (1e-38, 1e38, 0.0, -1.0, math.nan, math.inf):
+        with pytest.raises(ValueError, match='tau'):
+            ops._check_tau(tau)
+    assert ops._check_tau(1) == 1.0 and ops._check_tau(1e-3) == 1e-3

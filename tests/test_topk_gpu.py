@@ -109,6 +109,41 @@ def test_select_adverse_rows(shape, kind, dtype):
     _check_select(x, k, 1.0)
 
 
+@pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize('shape', [(3, 700), (2, 5003), (2, 40000), (2, 70, 5, 9), (2, 300, 3, 4)])
+@pytest.mark.parametrize('count', [12, 13, 40, 70])
+def test_infinities_and_nan_that_are_left_over(shape, count, dtype):
+    """more infinities than entries: the rest is their sum, inf; more NaN than entries: NaN; infinities behind NaN: inf"""
+    from segdistill_amd import ops
+    g = torch.Generator(device='cuda').manual_seed(count)
+    n, k = shape[1], 12
+    x = torch.randn(shape, device='cuda', generator=g).to(dtype)
+    at = torch.randperm(n, device='cuda', generator=g)[:count]
+    x[:, at] = math.inf
+    _, _, rest = _check_select(x, k, 1.0)                                            # count = k: the finite ones are what is left
+    assert bool(torch.isposinf(rest).all()) == (count > k)
+    x[:, at[:k]] = math.nan
+    v, i, rest = ops.topk_logits(x, k)
+    assert v.isnan().all() and (i.sort(1).values == at[:k].sort().values.view((1, k) + (1,) * (len(shape) - 2))).all()
+    assert bool(torch.isposinf(rest).all()) == (count > k)
+    x[:, at] = math.nan
+    v, i, rest = ops.topk_logits(x, k)
+    assert v.isnan().all() and bool(rest.isnan().all()) == (count > k)
+
+
+def test_more_rows_than_one_launch_holds():
+    from segdistill_amd import ops
+    rows = 4 * 0xffffff + 37                                                         # four rows per workgroup, 2^24 - 1 workgroups
+    x = torch.randn(rows, 2, device='cuda', generator=torch.Generator(device='cuda').manual_seed(3))
+    v, i, rest = ops.topk_logits(x, 1)
+    second = (x[:, 1] > x[:, 0])
+    assert torch.equal(v[:, 0], x.amax(1)) and torch.equal(i[:, 0], second.int())
+    # rest = b + log s with s = 2^(a c2 - b c2) of the one that is left, a, relative to b >= a.  In steps of U: the shift b c2 rounds by |b|, c2 and the
+    # argument by 2 |a - b|, the exponential by 2, the logarithm by 2 |a - b|, the result by |a|: at most |a| + |b| + 4 |a - b| + 2 <= 5 (|a| + |b|) + 2
+    low = x.amin(1)
+    assert ((rest - low).abs() <= U * (5 * x.abs().sum(1) + 2)).all()
+
+
 def test_select_takes_strided_and_offset_views():
     g = torch.Generator(device='cuda').manual_seed(6)
     base = torch.randn(1 + 3 * 4001, device='cuda', generator=g)
