@@ -91,7 +91,8 @@ class WindowAttention(nn.Module):
         rel = (coords[:, :, None] - coords[:, None, :]).permute(1, 2, 0)   # [N, N, 2]
         index = (rel[..., 0] + wh - 1) * (2 * ww - 1) + (rel[..., 1] + ww - 1)
         self.register_buffer('relative_position_index', index)
-        self.bias_plan = rel_bias.BucketPlan(index, self.relative_position_bias_table.shape[0])
+        self.bias_plan = None
+        self._plan_of_loaded_index(self, None)
         self.register_load_state_dict_post_hook(WindowAttention._plan_of_loaded_index)
         self.qkv = nn.Linear(dim, dim * 3, bias=qkv_bias)
         self.attn_drop = nn.Dropout(attn_drop)
@@ -102,8 +103,8 @@ class WindowAttention(nn.Module):
 
     @staticmethod
     def _plan_of_loaded_index(self, _keys):
-        """a checkpoint brings its own relative_position_index"""
-        if not torch.equal(self.bias_plan.index, self.relative_position_index.to(torch.int32)):
+        """a checkpoint brings its own relative_position_index, and the only one to a module that was built on the meta device"""
+        if not self.relative_position_index.is_meta:
             self.bias_plan = rel_bias.BucketPlan(self.relative_position_index, self.relative_position_bias_table.shape[0])
 
     def _bias_packed(self, n, h):
@@ -145,12 +146,12 @@ class WindowAttention(nn.Module):
             out = window_attn.forward_packed(qkv.contiguous(), self._bias_packed(n, h), *self._mask_packed(mask), h, self.scale)
             return self.proj_drop(self.proj(out))
         if (torch.is_grad_enabled() and (qkv.requires_grad or tbl.requires_grad) and not (self.training and self.attn_drop.p > 0)
-                and window_attn.train_supported(qkv, n, c // h) and (mask is None or bw % mask.shape[0] == 0)):
+                and window_attn.train_supported(qkv, n, c // h) and rel_bias.supported(tbl) and (mask is None or bw % mask.shape[0] == 0)):
             # a graph to build (a Swin student): the same product with its gradients, one kernel each way (csrc/window_train.hip)
             return self.proj_drop(self.proj(window_attn.attention(qkv, rel_bias.bucket_bias(tbl, self.bias_plan), mask, h, self.scale)))
         q, k, v = qkv.reshape(bw, n, 3, h, c // h).permute(2, 0, 3, 1, 4)
         def additive():
-            if tbl.is_cuda and tbl.requires_grad:
+            if tbl.requires_grad and rel_bias.supported(tbl):
                 bias = rel_bias.bucket_bias(tbl, self.bias_plan)                                        # [h,N,N]
             else:
                 bias = tbl[self.relative_position_index.view(-1)].view(n, n, h).permute(2, 0, 1)

@@ -77,6 +77,11 @@ class _BucketBiasFunction(torch.autograd.Function):
         return dtable, None
 
 
+def supported(table):
+    """bucket_bias takes a table of this type on this device."""
+    return table.is_cuda and table.dtype in _DT
+
+
 def bucket_bias(table, plan):
     """table [num_buckets, heads] (fp32 or bf16) -> bias [heads, Nq, Nk] = table[index].permute(2, 0, 1), with a deterministic gradient for the table."""
     _require_gpu(table)

@@ -138,3 +138,19 @@ def test_temperatures_whose_reciprocal_is_no_normal_number_are_refused(L):
         with pytest.raises(ValueError, match='tau'):
             ops._check_tau(tau)
     assert ops._check_tau(1) == 1.0 and ops._check_tau(1e-3) == 1e-3
+
+
+def test_window_attention_built_on_the_meta_device_gets_its_plan_with_the_loaded_index():
+    from segdistill_amd.backbones.swin import WindowAttention
+    real = WindowAttention(64, (3, 4), 2)
+    for assign in (False, True):
+        with torch.device('meta'):
+            att = WindowAttention(64, (3, 4), 2)
+        assert att.bias_plan is None and set(att.state_dict()) == set(real.state_dict())
+        if not assign:
+            att.to_empty(device='cpu')
+        att.load_state_dict(real.state_dict(), assign=assign)
+        for name, t in real.bias_plan.named_buffers():
+            assert torch.equal(t, dict(att.bias_plan.named_buffers())[name]), name
+    x = torch.randn(4, 12, 64)
+    assert torch.equal(att(x), real(x))

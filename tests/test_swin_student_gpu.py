@@ -78,6 +78,21 @@ def test_a_loaded_index_gives_the_plan():
     assert torch.equal(att.bias_plan.index.long(), sd['relative_position_index']) and att.bias_plan.index.is_cuda
 
 
+def test_a_type_that_the_kernels_do_not_take_keeps_the_modules_path():
+    from segdistill_amd import rel_bias
+    from segdistill_amd.backbones.swin import WindowAttention
+    torch.manual_seed(1)
+    att = WindowAttention(64, (4, 4), 2).double()
+    x = torch.randn(6, 16, 64, dtype=torch.float64)
+    ref = copy.deepcopy(att)
+    ref(x).square().sum().backward()
+    att.cuda()
+    assert not rel_bias.supported(att.relative_position_bias_table) and not rel_bias.supported(att.relative_position_bias_table.half())
+    att(x.cuda()).square().sum().backward()
+    for (n, p), q in zip(att.named_parameters(), ref.parameters()):
+        assert float((p.grad.cpu() - q.grad).abs().max()) <= 1e-12 * float(q.grad.abs().max()), n
+
+
 def _model():
     import segdistill_amd
     from segdistill_amd.builder import build_segmentor
