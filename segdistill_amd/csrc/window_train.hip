@@ -7,108 +7,106 @@
 // A row of S lives in one wave's registers, so the backward takes the softmax again instead of reading statistics or the output: it reads qkv
 // and dO and writes dqkv.  A row whose mask leaves nothing (-inf everywhere) has O = 0 and no gradient.
 //
-// A workgroup keeps one head and walks over windows; wave w of its NT = ceil(N / 32) waves owns the 32 queries of tile w, then (dV, dK) the 32 keys
+// A workgroup keeps one head and walks over windows; wave w of its NA = ceil(N / 16) waves owns the 16 queries of tile w, then (dV, dK) the 16 keys
 // of tile w.  The operands of a window come into LDS as rows, 16 bytes per thread, and the next window's are on their way to registers meanwhile.
-// S^T = K Q^T puts query i = 32 w + (lane & 31) on the lane and keys j = 32 a + 8 (e >> 2) + (e & 3) + 4 hh into the accumulators (hh = lane >> 5):
-// the softmax is in-lane plus one exchange with the other half-wave, and P^T is the B operand of O^T = V^T P^T as it stands.  The products that sum
-// over queries need the lane to be the key: P, then dS, cross through LDS.  The bias gradient of all windows of a workgroup stays in its accumulators
-// and leaves once, as one slab; the slabs are joined in slab order.
-//   fp32 storage: v_mfma_f32_32x32x2_f32, exact products.
-//   bf16 storage: v_mfma_f32_32x32x16_bf16 on the operands as stored.  P and dS enter their products as two bf16 terms (the value and what its
-//   rounding left): one term alone would put an error as large as the result's own rounding on every output; the second costs 12 of 32 MFMAs.
+// S^T = K Q^T puts query i = 16 w + (lane & 15) on the lane and its keys into the accumulators.  The rows of K enter in an order (key_of_row) that makes
+// accumulator s = 4 a + e of the lanes q = lane >> 4 the keys 4 s + q: only NS = ceil(N / 4) accumulators hold keys, and NS is known to the compiler (13 of
+// 16 for 7 x 7 windows).  The softmax is in-lane plus two exchanges, and P^T is the B operand of O^T = V^T P^T as it stands.  The products that sum over queries need the lane to be the key: P, then dS,
+// cross through LDS.  The bias gradient of all windows of a workgroup stays in its accumulators and leaves once, as one slab; the slabs are joined in
+// slab order.
+//   fp32 storage: v_mfma_f32_16x16x4_f32, exact products.
+//   bf16 storage: v_mfma_f32_16x16x32_bf16 on the operands as stored.  P and dS enter their products as two bf16 terms (the
+//   value and what its rounding left): one term alone would put an error as large as the result's own rounding on every output.
 //   Softmax, dS and the bias gradient are fp32.  Operand columns come from the row images by transposed LDS reads (ds_read_b64_tr_b16).
 #include <math.h>
+
+#include <type_traits>
 
 #include "cgd_device.h"
 
 namespace sd {
 namespace {
 
-typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef short s16x8 __attribute__((ext_vector_type(8)));
-typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
-typedef float f32x2 __attribute__((ext_vector_type(2)));
+typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef unsigned int u32x4 __attribute__((ext_vector_type(4)));
 constexpr int D = 32;
-
-__device__ __forceinline__ f32x16 zero16() {
-    f32x16 z;
-#pragma unroll
-    for (int e = 0; e < 16; ++e) z[e] = 0.f;
-    return z;
-}
+constexpr f32x4 kZero4 = {0.f, 0.f, 0.f, 0.f};
 
 // ---- products on LDS images ------------------------------------------------------------------------------------------------------------------
-// An image holds rows of 32 elements, PITCH apart (16-byte rows that start on different banks); rows [N, rows(N)) are zero.  The cross image holds one
-// row of keys per query.
+// An image holds 16 NA rows of 32 elements, PITCH apart (16-byte pieces of 16 rows cover the banks); rows behind the window are zero.  The cross image
+// holds one row of keys per query, a tile's keys in the order of the accumulators.  r = lane & 15, q = lane >> 4; sums over tokens run in steps s, token
+// 4 s + q.
+__device__ __forceinline__ int key_of_row(int r) { return 4 * (r & 3) + (r >> 2); }
+constexpr int tiles_of(int NS) { return (NS + 3) / 4; }
 template <typename T>
 struct Lds;
 
 template <>
 struct Lds<float> {
     static constexpr int PITCH = 36, CHUNKS = 8;                                  // CHUNKS: 16-byte pieces of a row
-    static __host__ __device__ constexpr int rows(int N) { return (N + 7) & ~7; }
-    static constexpr int cross_pitch(int NT) { return 32 * NT + 4; }
-    static __host__ __device__ constexpr size_t cross_bytes(int N, int NT) { return (size_t)rows(N) * (32 * NT + 4) * 4; }
+    static __host__ __device__ constexpr int cross_pitch(int NA) { return 16 * NA + 4; }
+    static __host__ __device__ constexpr size_t cross_bytes(int NA) { return (size_t)16 * NA * cross_pitch(NA) * 4; }
 
-    typedef f32x16 Operand;                                                       // a tile of P or dS as its products take it
-    static __device__ __forceinline__ Operand operand(const f32x16 &p) { return p; }
-
-    // acc[m][n] += sum_d A[32 t + m][d] B[pb][d], lane n holding row pb
-    template <int NT>
-    static __device__ __forceinline__ void rows_product(f32x16 (&acc)[NT], const float *A, const float *B, int pb, int N, int r, int hh) {
-        const int last = rows(N) - 1;                                             // rows behind the image: any finite row, masked by the caller
-        const float *b = B + min(pb, last) * PITCH + 16 * hh;
+    template <int NA>
+    struct Operand {                                                              // the wave's tiles of P or dS as their products take them
+        f32x4 v[NA];
+    };
+    template <int NA>
+    static __device__ __forceinline__ Operand<NA> operand(const f32x4 (&p)[NA]) {
+        Operand<NA> o;
 #pragma unroll
-        for (int u = 0; u < 4; ++u) {
-            const float4 bv = *reinterpret_cast<const float4 *>(b + 4 * u);
+        for (int a = 0; a < NA; ++a) o.v[a] = p[a];
+        return o;
+    }
+    // acc[a][m][n] += sum_d A[16 a + key_of_row(m)][d] B[16 w + n][d]
+    template <int NA>
+    static __device__ __forceinline__ void rows_product(f32x4 (&acc)[NA], const float *A, const float *B, int w, int lane) {
+        const int r = lane & 15, d = 8 * (lane >> 4);
+        const float *pa = A + key_of_row(r) * PITCH + d, *pb = B + (16 * w + r) * PITCH + d;
 #pragma unroll
-            for (int a = 0; a < NT; ++a) {
-                const float4 av = *reinterpret_cast<const float4 *>(A + min(32 * a + r, last) * PITCH + 16 * hh + 4 * u);
-                acc[a] = __builtin_amdgcn_mfma_f32_32x32x2f32(av.x, bv.x, acc[a], 0, 0, 0);
-                acc[a] = __builtin_amdgcn_mfma_f32_32x32x2f32(av.y, bv.y, acc[a], 0, 0, 0);
-                acc[a] = __builtin_amdgcn_mfma_f32_32x32x2f32(av.z, bv.z, acc[a], 0, 0, 0);
-                acc[a] = __builtin_amdgcn_mfma_f32_32x32x2f32(av.w, bv.w, acc[a], 0, 0, 0);
+        for (int u = 0; u < 2; ++u) {
+            const f32x4 bv = *reinterpret_cast<const f32x4 *>(pb + 4 * u);
+#pragma unroll
+            for (int a = 0; a < NA; ++a) {
+                const f32x4 av = *reinterpret_cast<const f32x4 *>(pa + 16 * a * PITCH + 4 * u);
+#pragma unroll
+                for (int c = 0; c < 4; ++c) acc[a] = __builtin_amdgcn_mfma_f32_16x16x4f32(av[c], bv[c], acc[a], 0, 0, 0);
             }
         }
     }
-    // acc[d][i] += sum_j M[j][d] p[j][i], p in the accumulator layout
-    template <int NT>
-    static __device__ __forceinline__ void columns_product(f32x16 &acc, const float *M, const Operand (&p)[NT], int N, int lane) {
-        const int r = lane & 31, hh = lane >> 5;
+    // acc[h][d][i] += sum_j M[j][16 h + d] p[j][i]
+    template <int NS>
+    static __device__ __forceinline__ void columns_product(f32x4 (&acc)[2], const float *M, const Operand<tiles_of(NS)> &p, int lane) {
+        const float *m = M + (lane >> 4) * PITCH + (lane & 15);
 #pragma unroll
-        for (int a = 0; a < NT; ++a)
+        for (int s = 0; s < NS; ++s)
 #pragma unroll
-            for (int g = 0; g < 4; ++g)
-                if (32 * a + 8 * g < N) {
-#pragma unroll
-                    for (int c = 0; c < 4; ++c)
-                        acc = __builtin_amdgcn_mfma_f32_32x32x2f32(M[(32 * a + 8 * g + c + 4 * hh) * PITCH + r], p[a][4 * g + c], acc, 0, 0, 0);
-                }
+            for (int h = 0; h < 2; ++h) acc[h] = __builtin_amdgcn_mfma_f32_16x16x4f32(m[4 * s * PITCH + 16 * h], p.v[s >> 2][s & 3], acc[h], 0, 0, 0);
     }
     // the wave's query rows of p into the cross image
-    template <int NT>
-    static __device__ __forceinline__ void cross_write(float *x, const Operand (&p)[NT], int i, int N, int hh) {
-        if (i >= rows(N)) return;
+    template <int NA>
+    static __device__ __forceinline__ void cross_write(float *x, const Operand<NA> &p, int w, int lane) {
+        float *to = x + (16 * w + (lane & 15)) * cross_pitch(NA) + 4 * (lane >> 4);
 #pragma unroll
-        for (int a = 0; a < NT; ++a)
-#pragma unroll
-            for (int g = 0; g < 4; ++g)
-                *reinterpret_cast<float4 *>(x + i * cross_pitch(NT) + 32 * a + 8 * g + 4 * hh) =
-                    make_float4(p[a][4 * g], p[a][4 * g + 1], p[a][4 * g + 2], p[a][4 * g + 3]);
+        for (int a = 0; a < NA; ++a) *reinterpret_cast<f32x4 *>(to + 16 * a) = p.v[a];
     }
-    // acc[d][j] += sum_i M[i][d] x[i][j], lane column j = 32 tile + (lane & 31)
-    template <int NT>
-    static __device__ __forceinline__ void cross_product(f32x16 &acc, const float *M, const float *x, int tile, int N, int lane) {
-        const int r = lane & 31, hh = lane >> 5;
-        for (int i0 = 0; i0 < N; i0 += 8) {
+    // acc[h][d][n] += sum_i M[i][16 h + d] x[i][16 w + n]: key 16 w + key_of_row(n)
+    template <int NS>
+    static __device__ __forceinline__ void cross_product(f32x4 (&acc)[2], const float *M, const float *x, int w, int lane) {
+        constexpr int pitch = cross_pitch(tiles_of(NS));
+        const int r = lane & 15, q = lane >> 4;
+        const float *m = M + q * PITCH + r, *b = x + q * pitch + 16 * w + r;
 #pragma unroll
-            for (int c = 0; c < 4; ++c) {
-                const int i = i0 + c + 4 * hh;
-                acc = __builtin_amdgcn_mfma_f32_32x32x2f32(M[i * PITCH + r], x[i * cross_pitch(NT) + 32 * tile + r], acc, 0, 0, 0);
-            }
+        for (int s = 0; s < NS; ++s) {
+            const float bv = b[4 * s * pitch];
+#pragma unroll
+            for (int h = 0; h < 2; ++h) acc[h] = __builtin_amdgcn_mfma_f32_16x16x4f32(m[4 * s * PITCH + 16 * h], bv, acc[h], 0, 0, 0);
         }
     }
 };
@@ -116,102 +114,112 @@ struct Lds<float> {
 template <>
 struct Lds<bf16_t> {
     static constexpr int PITCH = 40, CHUNKS = 4;
-    static __host__ __device__ constexpr int rows(int N) { return (N + 15) & ~15; }
-    static constexpr int cross_pitch(int NT) { return 32 * NT + 8; }
-    static __host__ __device__ constexpr size_t plane(int N, int NT) { return (size_t)rows(N) * (32 * NT + 8); }       // elements of one of the two terms
-    static __host__ __device__ constexpr size_t cross_bytes(int N, int NT) { return 2 * plane(N, NT) * 2; }
+    static __host__ __device__ constexpr int cross_pitch(int NA) { return 16 * NA + 8; }
+    static __host__ __device__ constexpr size_t plane(int NA) { return (size_t)16 * NA * cross_pitch(NA); }       // elements of one of the two terms
+    static __host__ __device__ constexpr size_t cross_bytes(int NA) { return 2 * plane(NA) * 2; }
 
-    static __device__ __forceinline__ f32x16 mfma(bf16x8 a, bf16x8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
-    // four rows x 16 columns per 16 lanes, delivered by column: lane 16 g + li gets column col0 + 16 g + li of rows row .. row + 3 (then row2 .. row2 + 3)
-    static __device__ __forceinline__ bf16x8 columns(const bf16_t *img, int pitch, int row, int row2, int col0, int lane) {
+    // four rows x 16 columns per 16 lanes, delivered by column: lane 16 q + r gets column r of the rows q, q + 4, q + 8, q + 12 behind `img`
+    static __device__ __forceinline__ s16x4 columns(const bf16_t *img, int pitch, int lane) {
         typedef s16x4 __attribute__((address_space(3))) * lds_p;
-        const int li = lane & 15, off = (li >> 2) * pitch + col0 + 16 * ((lane >> 4) & 1) + 4 * (li & 3);
-        const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_p)(img + row * pitch + off));
-        const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_p)(img + row2 * pitch + off));
+        const int li = lane & 15;
+        return __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_p)(img + ((lane >> 4) + 4 * (li >> 2)) * pitch + 4 * (li & 3)));
+    }
+    static __device__ __forceinline__ bf16x8 join(s16x4 lo, s16x4 hi) {
         const s16x8 v = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
         return __builtin_bit_cast(bf16x8, v);
     }
-    template <int NT>
-    static __device__ __forceinline__ void rows_product(f32x16 (&acc)[NT], const bf16_t *A, const bf16_t *B, int pb, int N, int r, int hh) {
-        const int last = rows(N) - 1;
-#pragma unroll
-        for (int t = 0; t < 2; ++t) {
-            const bf16x8 bv = *reinterpret_cast<const bf16x8 *>(B + min(pb, last) * PITCH + 16 * t + 8 * hh);
-#pragma unroll
-            for (int a = 0; a < NT; ++a) acc[a] = mfma(*reinterpret_cast<const bf16x8 *>(A + min(32 * a + r, last) * PITCH + 16 * t + 8 * hh), bv, acc[a]);
-        }
+    // An odd last tile goes with a zero one.  (Not by the 16-deep form: hipcc lets it follow the 32-deep one on the same accumulator without the wait that
+    // their different lengths need, and its first rows come out wrong.)
+    static __device__ __forceinline__ f32x4 mfma32(s16x4 a0, s16x4 a1, s16x4 b0, s16x4 b1, f32x4 c) {
+        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(join(a0, a1), join(b0, b1), c, 0, 0, 0);
     }
-    // p = first + second, each bf16, to 2^-17 of p; elements 8 t .. 8 t + 7 of the accumulator tile in first[t], second[t].  On pairs: one conversion
-    // instruction takes two values.
+
+    // p = first + second, each bf16, to 2^-17 of p.  On pairs: one conversion instruction takes two values.
+    template <int NA>
     struct Operand {
-        bf16x8 first[2], second[2];
+        s16x4 first[NA], second[NA];
     };
-    static __device__ __forceinline__ Operand operand(const f32x16 &p) {
-        Operand o;
+    template <int NA>
+    static __device__ __forceinline__ Operand<NA> operand(const f32x4 (&p)[NA]) {
+        Operand<NA> o;
 #pragma unroll
-        for (int e = 0; e < 16; e += 2) {
-            const f32x2 v = {p[e], p[e + 1]};
-            const bf16x2 f = __builtin_convertvector(v, bf16x2), s = __builtin_convertvector(v - __builtin_convertvector(f, f32x2), bf16x2);
-            o.first[e >> 3][e & 7] = f[0], o.first[e >> 3][(e & 7) + 1] = f[1];
-            o.second[e >> 3][e & 7] = s[0], o.second[e >> 3][(e & 7) + 1] = s[1];
+        for (int a = 0; a < NA; ++a) {
+            bf16x4 f, s;
+#pragma unroll
+            for (int e = 0; e < 4; e += 2) {
+                const f32x2 v = {p[a][e], p[a][e + 1]};
+                const bf16x2 f2 = __builtin_convertvector(v, bf16x2), s2 = __builtin_convertvector(v - __builtin_convertvector(f2, f32x2), bf16x2);
+                f[e] = f2[0], f[e + 1] = f2[1];
+                s[e] = s2[0], s[e + 1] = s2[1];
+            }
+            o.first[a] = __builtin_bit_cast(s16x4, f);
+            o.second[a] = __builtin_bit_cast(s16x4, s);
         }
         return o;
     }
-    template <int NT>
-    static __device__ __forceinline__ void columns_product(f32x16 &acc, const bf16_t *M, const Operand (&p)[NT], int N, int lane) {
-        const int hh = lane >> 5;
+    template <int NA>
+    static __device__ __forceinline__ void rows_product(f32x4 (&acc)[NA], const bf16_t *A, const bf16_t *B, int w, int lane) {
+        const int r = lane & 15, d = 8 * (lane >> 4);
+        const bf16_t *pa = A + key_of_row(r) * PITCH + d;
+        const bf16x8 bv = *reinterpret_cast<const bf16x8 *>(B + (16 * w + r) * PITCH + d);
 #pragma unroll
-        for (int a = 0; a < NT; ++a)
-#pragma unroll
-            for (int t = 0; t < 2; ++t)
-                if (32 * a + 16 * t < N) {
-                    const int j0 = 32 * a + 16 * t + 4 * hh;                       // accumulator rows 8 t .. 8 t + 7 are j0 .. j0 + 3 and j0 + 8 .. j0 + 11
-                    const bf16x8 m = columns(M, PITCH, j0, j0 + 8, 0, lane);
-                    acc = mfma(m, p[a].first[t], acc);
-                    acc = mfma(m, p[a].second[t], acc);
-                }
+        for (int a = 0; a < NA; ++a) acc[a] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(*reinterpret_cast<const bf16x8 *>(pa + 16 * a * PITCH), bv, acc[a], 0, 0, 0);
     }
-    template <int NT>
-    static __device__ __forceinline__ void cross_write(bf16_t *x, const Operand (&p)[NT], int i, int N, int hh) {
-        if (i >= rows(N)) return;
+    template <int NS, int NA = tiles_of(NS)>
+    static __device__ __forceinline__ void columns_product(f32x4 (&acc)[2], const bf16_t *M, const Operand<NA> &p, int lane) {
 #pragma unroll
-        for (int a = 0; a < NT; ++a)
+        for (int h = 0; h < 2; ++h) {
+            s16x4 m[NA];
 #pragma unroll
-            for (int t = 0; t < 2; ++t) {
-                const u32x4 f = __builtin_bit_cast(u32x4, p[a].first[t]), s = __builtin_bit_cast(u32x4, p[a].second[t]);
-                bf16_t *to = x + i * cross_pitch(NT) + 32 * a + 16 * t + 4 * hh;
-                *reinterpret_cast<uint2 *>(to) = make_uint2(f[0], f[1]);
-                *reinterpret_cast<uint2 *>(to + 8) = make_uint2(f[2], f[3]);
-                *reinterpret_cast<uint2 *>(to + plane(N, NT)) = make_uint2(s[0], s[1]);
-                *reinterpret_cast<uint2 *>(to + plane(N, NT) + 8) = make_uint2(s[2], s[3]);
+            for (int a = 0; a < NA; ++a) m[a] = columns(M + 16 * a * PITCH + 16 * h, PITCH, lane);
+#pragma unroll
+            for (int a = 0; a < NA; a += 2) {
+                const s16x4 zero = {0, 0, 0, 0};
+                const bool pair = a + 1 < NA;
+                const int b = pair ? a + 1 : a;
+                acc[h] = mfma32(m[a], pair ? m[b] : zero, p.first[a], pair ? p.first[b] : zero, acc[h]);
+                acc[h] = mfma32(m[a], pair ? m[b] : zero, p.second[a], pair ? p.second[b] : zero, acc[h]);
             }
-    }
-    template <int NT>
-    static __device__ __forceinline__ void cross_product(f32x16 &acc, const bf16_t *M, const bf16_t *x, int tile, int N, int lane) {
-        const int hh = lane >> 5;
-        for (int i0 = 0; i0 < N; i0 += 16) {
-            const int i = i0 + 8 * hh;
-            const bf16x8 m = columns(M, PITCH, i, i + 4, 0, lane);
-            acc = mfma(m, columns(x, cross_pitch(NT), i, i + 4, 32 * tile, lane), acc);
-            acc = mfma(m, columns(x + plane(N, NT), cross_pitch(NT), i, i + 4, 32 * tile, lane), acc);
         }
+    }
+    template <int NA>
+    static __device__ __forceinline__ void cross_write(bf16_t *x, const Operand<NA> &p, int w, int lane) {
+        bf16_t *to = x + (16 * w + (lane & 15)) * cross_pitch(NA) + 4 * (lane >> 4);
+#pragma unroll
+        for (int a = 0; a < NA; ++a) {
+            *reinterpret_cast<s16x4 *>(to + 16 * a) = p.first[a];
+            *reinterpret_cast<s16x4 *>(to + plane(NA) + 16 * a) = p.second[a];
+        }
+    }
+    template <int NS, int NA = tiles_of(NS)>
+    static __device__ __forceinline__ void cross_product(f32x4 (&acc)[2], const bf16_t *M, const bf16_t *x, int w, int lane) {
+        Operand<NA> p;
+#pragma unroll
+        for (int a = 0; a < NA; ++a) {
+            const bf16_t *from = x + 16 * a * cross_pitch(NA) + 16 * w;
+            p.first[a] = columns(from, cross_pitch(NA), lane);
+            p.second[a] = columns(from + plane(NA), cross_pitch(NA), lane);
+        }
+        columns_product<NS>(acc, M, p, lane);
     }
 };
 
 template <typename T>
-__host__ __device__ constexpr size_t image_elems(int N) { return (size_t)Lds<T>::rows(N) * Lds<T>::PITCH; }
+__host__ __device__ constexpr size_t image_elems(int NA) { return (size_t)16 * NA * Lds<T>::PITCH; }
 
 // ---- staging -----------------------------------------------------------------------------------------------------------------------------------
-// A matrix of N rows of 32 elements, `stride` apart, through registers into an image: NT waves move 64 NT / CHUNKS rows at a time.
-template <typename T, int NT>
+// A matrix of N rows of 32 elements, `stride` apart, through registers into an image: NA waves move 64 NA / CHUNKS rows at a time.
+template <typename T, int NA>
 struct Stage {
-    static constexpr int CH = Lds<T>::CHUNKS, STEP = 64 * NT / CH, PASSES = 32 * NT / STEP;
+    static constexpr int CH = Lds<T>::CHUNKS, STEP = 64 * NA / CH, PASSES = 16 * NA / STEP;
     u32x4 reg[PASSES];
-    __device__ __forceinline__ void load(const T *base, long stride, int N) {
-        const int row = threadIdx.x / CH, ch = threadIdx.x % CH;
+    // `base` is the workgroup's, the lane adds a 32-bit offset (64 rows of 3 * 65535 heads * 128 bytes stay below 2^31)
+    __device__ __forceinline__ void load(const T *base, unsigned stride, int N) {
+        const unsigned row = threadIdx.x / CH, ch = threadIdx.x % CH;
+        const char *from = reinterpret_cast<const char *>(base);
 #pragma unroll
         for (int u = 0; u < PASSES; ++u)              // every lane loads, rows behind the window the last one again: a register written in part stays live all along
-            reg[u] = *(reinterpret_cast<const u32x4 *>(base + (size_t)min(row + u * STEP, N - 1) * stride) + ch);
+            reg[u] = *reinterpret_cast<const u32x4 *>(from + (min(row + u * STEP, (unsigned)N - 1) * (stride * (unsigned)sizeof(T)) + ch * 16));
     }
     __device__ __forceinline__ void clear() {
         const u32x4 z = {0u, 0u, 0u, 0u};
@@ -226,12 +234,11 @@ struct Stage {
     }
 };
 // the zero rows behind an image's last one
-template <typename T, int NT>
+template <typename T, int NA>
 __device__ __forceinline__ void zero_tail(T *img, int N) {
-    const int chunks = (Lds<T>::rows(N) - N) * Lds<T>::CHUNKS;
-    for (int u = threadIdx.x; u < chunks; u += 64 * NT) {
+    for (int u = N * Lds<T>::CHUNKS + threadIdx.x; u < 16 * NA * Lds<T>::CHUNKS; u += 64 * NA) {
         const u32x4 z = {0u, 0u, 0u, 0u};
-        *(reinterpret_cast<u32x4 *>(img + (N + u / Lds<T>::CHUNKS) * Lds<T>::PITCH) + u % Lds<T>::CHUNKS) = z;
+        *(reinterpret_cast<u32x4 *>(img + u / Lds<T>::CHUNKS * Lds<T>::PITCH) + u % Lds<T>::CHUNKS) = z;
     }
 }
 
@@ -240,78 +247,76 @@ __device__ __forceinline__ void store4(T *p, float x, float y, float z, float w)
     if constexpr (sizeof(T) == 4) {
         *reinterpret_cast<float4 *>(p) = make_float4(x, y, z, w);
     } else {
+        const f32x2 a = {x, y}, b = {z, w};
         *reinterpret_cast<uint2 *>(p) =
-            make_uint2((unsigned)f32_to_bf16(x) | ((unsigned)f32_to_bf16(y) << 16), (unsigned)f32_to_bf16(z) | ((unsigned)f32_to_bf16(w) << 16));
+            make_uint2(__builtin_bit_cast(unsigned, __builtin_convertvector(a, bf16x2)), __builtin_bit_cast(unsigned, __builtin_convertvector(b, bf16x2)));
     }
 }
-// an accumulator tile whose rows are d and whose column is the lane's token
+// two accumulator tiles whose rows are d and whose column is the lane's token
 template <typename T>
-__device__ __forceinline__ void store_tile(T *__restrict__ base, long stride, int p, int N, int hh, const f32x16 &o, float mul) {
+__device__ __forceinline__ void store_tile(T *__restrict__ base, unsigned stride, int p, int N, int lane, const f32x4 (&o)[2], float mul) {
     if (p >= N) return;
-    T *dst = base + (size_t)p * stride + 4 * hh;
+    T *dst = reinterpret_cast<T *>(reinterpret_cast<char *>(base) + ((unsigned)p * stride + 4 * (lane >> 4)) * (unsigned)sizeof(T));
 #pragma unroll
-    for (int g = 0; g < 4; ++g) store4(dst + 8 * g, o[4 * g] * mul, o[4 * g + 1] * mul, o[4 * g + 2] * mul, o[4 * g + 3] * mul);
+    for (int h = 0; h < 2; ++h) store4(dst + 16 * h, o[h][0] * mul, o[h][1] * mul, o[h][2] * mul, o[h][3] * mul);
 }
 
 // ---- the softmax of one query tile ---------------------------------------------------------------------------------------------------------------
-// p: K Q^T on entry, probabilities on return.  bias / mask: packed tables at (tile, lane).
-template <int NT>
-__device__ __forceinline__ void softmax_tile(f32x16 (&p)[NT], const float4 *__restrict__ bias, const float4 *__restrict__ mask, float scale, bool live) {
+// over the four lanes that hold a query's keys
+__device__ __forceinline__ float row_max(float v) {
+    v = fmaxf(v, __shfl_xor(v, 16, 64));
+    return fmaxf(v, __shfl_xor(v, 32, 64));
+}
+__device__ __forceinline__ float row_sum(float v) {
+    v += __shfl_xor(v, 16, 64);
+    return v + __shfl_xor(v, 32, 64);
+}
+// what is added to the wave's scores: the tiles of the bias, and of the mask if it says anything
+template <int NA>
+__device__ __forceinline__ void load_added(f32x4 (&t)[NA], const float *__restrict__ packed, int head, int mask, int w, int lane) {
+    const f32x4 *from = reinterpret_cast<const f32x4 *>(packed) + w * NA * 64 + lane;
 #pragma unroll
-    for (int a = 0; a < NT; ++a)
+    for (int a = 0; a < NA; ++a) t[a] = from[(size_t)head * (NA * NA * 64) + a * 64];
+    if (mask >= 0) {
 #pragma unroll
-        for (int g = 0; g < 4; ++g) {
-            const float4 v = bias[(a * NT * 4 + g) * 64];
-            p[a][4 * g] = fmaf(p[a][4 * g], scale, v.x), p[a][4 * g + 1] = fmaf(p[a][4 * g + 1], scale, v.y);
-            p[a][4 * g + 2] = fmaf(p[a][4 * g + 2], scale, v.z), p[a][4 * g + 3] = fmaf(p[a][4 * g + 3], scale, v.w);
-        }
-    if (mask) {
-#pragma unroll
-        for (int a = 0; a < NT; ++a)
-#pragma unroll
-            for (int g = 0; g < 4; ++g) {
-                const float4 v = mask[(a * NT * 4 + g) * 64];
-                p[a][4 * g] += v.x, p[a][4 * g + 1] += v.y, p[a][4 * g + 2] += v.z, p[a][4 * g + 3] += v.w;
-            }
+        for (int a = 0; a < NA; ++a) t[a] += from[(size_t)mask * (NA * NA * 64) + a * 64];
     }
-    float m = -INFINITY;
+}
+// p: K Q^T on entry, e^(S - max) on return, 0 in the accumulators without keys -> 1 / sum, 0 for a row that has nothing left
+template <int NS, int NA = tiles_of(NS)>
+__device__ __forceinline__ float softmax_tile(f32x4 (&p)[NA], const f32x4 (&added)[NA], float scale) {
+    float m = -INFINITY, l = 0.f;
 #pragma unroll
-    for (int a = 0; a < NT; ++a)
+    for (int s = 0; s < NS; ++s) {
+        p[s >> 2][s & 3] = fmaf(p[s >> 2][s & 3], scale, added[s >> 2][s & 3]);
+        m = fmaxf(m, p[s >> 2][s & 3]);
+    }
+    m = row_max(m);
+    if (m == -INFINITY) m = 0.f;                      // nothing left: every term is 0
 #pragma unroll
-        for (int e = 0; e < 16; ++e) m = fmaxf(m, p[a][e]);
-    m = fmaxf(m, __shfl_xor(m, 32, 64));
-    if (m == -INFINITY) m = 0.f;                      // nothing left: every probability is 0
-    float l = 0.f;
-#pragma unroll
-    for (int a = 0; a < NT; ++a)
-#pragma unroll
-        for (int e = 0; e < 16; ++e) {
-            p[a][e] = ex2((p[a][e] - m) * 1.4426950408889634f);
-            l += p[a][e];
-        }
-    l += __shfl_xor(l, 32, 64);
-    const float inv = l == 0.f ? 0.f : 1.f / l;
-#pragma unroll
-    for (int a = 0; a < NT; ++a)
-#pragma unroll
-        for (int e = 0; e < 16; ++e) p[a][e] = live ? p[a][e] * inv : 0.f;        // a query row behind the window holds nothing
+    for (int s = 0; s < 4 * NA; ++s) {
+        p[s >> 2][s & 3] = s < NS ? ex2((p[s >> 2][s & 3] - m) * 1.4426950408889634f) : 0.f;
+        l += p[s >> 2][s & 3];
+    }
+    l = row_sum(l);
+    return l == 0.f ? 0.f : 1.f / l;
 }
 
 // ---- tables --------------------------------------------------------------------------------------------------------------------------------------
-// bias [heads][N][N], then mask [nW][N][N], into the accumulator layout [a][b][e >> 2][lane][e & 3]: padded keys -inf in the bias and 0 in the mask,
+// bias [heads][N][N], then mask [nW][N][N], into the accumulator layout [query tile][key tile][lane][e], key 16 a + 4 e + (lane >> 4): padded keys -inf in the bias and 0 in the mask,
 // padded queries 0; any[w] = the mask of window w has a nonzero entry
-template <int NT>
+template <int NA>
 __global__ __launch_bounds__(256) void window_tables(const float *__restrict__ bias, const float *__restrict__ mask, float *__restrict__ packed, int *__restrict__ any,
                                                      int heads, int N) {
     const int t = blockIdx.x;
     const float *src = t < heads ? bias + (size_t)t * N * N : mask + (size_t)(t - heads) * N * N;
     const float pad = t < heads ? -INFINITY : 0.f;
     int nonzero = 0;
-    for (int at = threadIdx.x; at < NT * NT * 1024; at += 256) {
-        const int c = at & 3, lane = (at >> 2) & 63, g = (at >> 8) & 3, ab = at >> 10, b = ab % NT, a = ab / NT;
-        const int j = 32 * a + 8 * g + c + 4 * (lane >> 5), i = 32 * b + (lane & 31);
+    for (int at = threadIdx.x; at < NA * NA * 256; at += 256) {
+        const int e = at & 3, lane = (at >> 2) & 63, ab = at >> 8, a = ab % NA, b = ab / NA;
+        const int j = 16 * a + 4 * e + (lane >> 4), i = 16 * b + (lane & 15);
         const float v = j >= N ? pad : (i < N ? src[(size_t)i * N + j] : 0.f);
-        packed[(size_t)t * (NT * NT * 1024) + at] = v;
+        packed[(size_t)t * (NA * NA * 256) + at] = v;
         nonzero |= v != 0.f;
     }
     nonzero = __syncthreads_or(nonzero);
@@ -324,139 +329,140 @@ __device__ __forceinline__ int logical_block() {
     return (x < rem ? x * (q + 1) : rem * (q + 1) + (x - rem) * q) + id / 8;
 }
 
-template <typename T, int NT>
-__global__ __launch_bounds__(64 * NT) __attribute__((amdgpu_waves_per_eu(3))) void window_train_fwd(const T *__restrict__ qkv, const float *__restrict__ packed, const int *__restrict__ any, T *__restrict__ out,
-                                                            int windows, int nslab, int nW, int heads, int N, float scale) {
+// waves per SIMD that the registers leave room for
+template <typename T>
+constexpr int kFwdWaves = sizeof(T) == 4 ? 5 : 6;
+constexpr int kBwdWaves = 4;
+
+template <typename T, int NS, int NA = tiles_of(NS)>
+__global__ __launch_bounds__(64 * NA, kFwdWaves<T>) void window_train_fwd(const T *__restrict__ qkv, const float *__restrict__ packed, const int *__restrict__ any,
+                                                                          T *__restrict__ out, int windows, int nslab, int nW, int heads, int N, float scale) {
     extern __shared__ __attribute__((aligned(16))) unsigned char lds[];
-    const size_t img = image_elems<T>(N);
+    constexpr size_t img = image_elems<T>(NA);
     T *Q = reinterpret_cast<T *>(lds), *K = Q + img, *V = K + img;
-    const int lane = threadIdx.x & 63, r = lane & 31, hh = lane >> 5, w = threadIdx.x >> 6;
+    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, i = 16 * w + (lane & 15);
     const int job = logical_block(), slab = job / heads, head = job - slab * heads;
-    const long C = (long)heads * D, stride = 3 * C, wstride = N * stride;
+    const int C = heads * D, stride = 3 * C;
+    const long wstride = (long)N * stride;
     const T *base = qkv + (size_t)head * D;
-    const float4 *bias = reinterpret_cast<const float4 *>(packed + (size_t)head * (NT * NT * 1024)) + w * 256 + lane;
-    Stage<T, NT> sq, sk, sv;
+    Stage<T, NA> sq, sk, sv;
     auto fetch = [&](int win) {
         const T *q = base + (size_t)win * wstride;
         sq.load(q, stride, N), sk.load(q + C, stride, N), sv.load(q + 2 * C, stride, N);
     };
     auto none = [&]() { sq.clear(), sk.clear(), sv.clear(); };          // a value on both ways: else the old one would stay live through the loop
     fetch(slab);
-    zero_tail<T, NT>(Q, N), zero_tail<T, NT>(K, N), zero_tail<T, NT>(V, N);
+    zero_tail<T, NA>(Q, N), zero_tail<T, NA>(K, N), zero_tail<T, NA>(V, N);
     for (int win = slab; win < windows; win += nslab) {
         __syncthreads();                               // the previous window's images are read
         sq.store(Q, N), sk.store(K, N), sv.store(V, N);
+        f32x4 added[NA];
+        int table = head;
+        asm volatile("" : "+s"(table));                // loaded anew: kept over the loop it would not fit the registers
+        load_added<NA>(added, packed, table, nW && any[win % nW] ? heads + win % nW : -1, w, lane);
+        win + nslab < windows ? fetch(win + nslab) : none();          // behind the tables: what is asked for first arrives first
         __syncthreads();
-        const float4 *mask = nW && any[win % nW] ? reinterpret_cast<const float4 *>(packed + (size_t)(heads + win % nW) * (NT * NT * 1024)) + w * 256 + lane : nullptr;
-        f32x16 p[NT], o = zero16();
+        f32x4 p[NA], o[2] = {kZero4, kZero4};
 #pragma unroll
-        for (int a = 0; a < NT; ++a) p[a] = zero16();
-        Lds<T>::template rows_product<NT>(p, K, Q, 32 * w + r, N, r, hh);
-        softmax_tile<NT>(p, bias, mask, scale, 32 * w + r < N);
-        win + nslab < windows ? fetch(win + nslab) : none();          // (not before: the registers are the scores' until here)
-        typename Lds<T>::Operand po[NT];
-#pragma unroll
-        for (int a = 0; a < NT; ++a) po[a] = Lds<T>::operand(p[a]);
-        Lds<T>::template columns_product<NT>(o, V, po, N, lane);
-        store_tile(out + (size_t)win * N * C + (size_t)head * D, C, 32 * w + r, N, hh, o, 1.f);
+        for (int a = 0; a < NA; ++a) p[a] = kZero4;
+        Lds<T>::template rows_product<NA>(p, K, Q, w, lane);
+        const float inv = softmax_tile<NS>(p, added, scale);
+        Lds<T>::template columns_product<NS>(o, V, Lds<T>::template operand<NA>(p), lane);
+        store_tile(out + (size_t)win * N * C + (size_t)head * D, C, i, N, lane, o, inv);
     }
 }
 
-constexpr int kBwdWaves = 2;           // waves per SIMD that the backward's registers leave room for (three: 73 spilled, bf16 76 -> 145 us)
-
-template <typename T, int NT>
-__global__ __launch_bounds__(64 * NT, kBwdWaves) void window_train_bwd(const T *__restrict__ qkv, const float *__restrict__ packed, const int *__restrict__ any,
-                                                            const T *__restrict__ dout, T *__restrict__ dqkv, float *__restrict__ slabs, int windows, int nslab, int nW,
-                                                            int heads, int N, float scale) {
+template <typename T, int NS, int NA = tiles_of(NS)>
+__global__ __launch_bounds__(64 * NA, kBwdWaves) void window_train_bwd(const T *__restrict__ qkv, const float *__restrict__ packed, const int *__restrict__ any,
+                                                                       const T *__restrict__ dout, T *__restrict__ dqkv, float *__restrict__ slabs, int windows, int nslab, int nW,
+                                                                       int heads, int N, float scale) {
     extern __shared__ __attribute__((aligned(16))) unsigned char lds[];
-    const size_t img = image_elems<T>(N);
+    constexpr size_t img = image_elems<T>(NA);
     T *Q = reinterpret_cast<T *>(lds), *G = Q + img, *K = G + img, *V = K + img, *X = K;          // P and dS cross where K and V were
-    const int lane = threadIdx.x & 63, r = lane & 31, hh = lane >> 5, w = threadIdx.x >> 6, i = 32 * w + r;
+    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, i = 16 * w + (lane & 15), j = 16 * w + key_of_row(lane & 15);
     const int job = logical_block(), slab = job / heads, head = job - slab * heads;
-    const long C = (long)heads * D, stride = 3 * C, wstride = N * stride;
+    const int C = heads * D, stride = 3 * C;
+    const long wstride = (long)N * stride;
     const T *base = qkv + (size_t)head * D, *gbase = dout + (size_t)head * D;
-    const float4 *bias = reinterpret_cast<const float4 *>(packed + (size_t)head * (NT * NT * 1024)) + w * 256 + lane;
-    Stage<T, NT> sq, sk, sv, sg;
+    Stage<T, NA> sq, sk, sv, sg;
     auto fetch = [&](int win) {
         const T *q = base + (size_t)win * wstride;
         sq.load(q, stride, N), sk.load(q + C, stride, N), sv.load(q + 2 * C, stride, N);
         sg.load(gbase + (size_t)win * N * C, C, N);
     };
-    auto none = [&]() { sq.clear(), sk.clear(), sv.clear(), sg.clear(); };          // a value on both ways: else the old one would stay live through the loop
+    auto none = [&]() { sq.clear(), sk.clear(), sv.clear(), sg.clear(); };
     fetch(slab);
-    zero_tail<T, NT>(Q, N), zero_tail<T, NT>(G, N);
-    f32x16 db[NT];
+    zero_tail<T, NA>(Q, N), zero_tail<T, NA>(G, N);
+    f32x4 db[NA];
 #pragma unroll
-    for (int a = 0; a < NT; ++a) db[a] = zero16();
+    for (int a = 0; a < NA; ++a) db[a] = kZero4;
     for (int win = slab; win < windows; win += nslab) {
         __syncthreads();                               // the previous window's images are read
         sq.store(Q, N), sk.store(K, N), sv.store(V, N), sg.store(G, N);
-        zero_tail<T, NT>(K, N), zero_tail<T, NT>(V, N);
+        zero_tail<T, NA>(K, N), zero_tail<T, NA>(V, N);
+        f32x4 added[NA];
+        int table = head;
+        asm volatile("" : "+s"(table));                // loaded anew: kept over the loop it would not fit the registers
+        load_added<NA>(added, packed, table, nW && any[win % nW] ? heads + win % nW : -1, w, lane);
         __syncthreads();
-        const float4 *mask = nW && any[win % nW] ? reinterpret_cast<const float4 *>(packed + (size_t)(heads + win % nW) * (NT * NT * 1024)) + w * 256 + lane : nullptr;
         T *dq = dqkv + (size_t)win * wstride + (size_t)head * D;
-        f32x16 p[NT], ds[NT];
+        f32x4 p[NA], ds[NA];
 #pragma unroll
-        for (int a = 0; a < NT; ++a) p[a] = ds[a] = zero16();
-        Lds<T>::template rows_product<NT>(p, K, Q, i, N, r, hh);
-        softmax_tile<NT>(p, bias, mask, scale, i < N);
-        Lds<T>::template rows_product<NT>(ds, V, G, i, N, r, hh);
+        for (int a = 0; a < NA; ++a) p[a] = ds[a] = kZero4;
+        Lds<T>::template rows_product<NA>(p, K, Q, w, lane);
+        const float inv = softmax_tile<NS>(p, added, scale);
+        Lds<T>::template rows_product<NA>(ds, V, G, w, lane);
         float dot = 0.f;
 #pragma unroll
-        for (int a = 0; a < NT; ++a)
+        for (int s = 0; s < NS; ++s) {
+            p[s >> 2][s & 3] = i < N ? p[s >> 2][s & 3] * inv : 0.f;              // a query row behind the window holds nothing
+            dot = fmaf(p[s >> 2][s & 3], ds[s >> 2][s & 3], dot);
+        }
+        dot = row_sum(dot);
 #pragma unroll
-            for (int e = 0; e < 16; ++e) dot = fmaf(p[a][e], ds[a][e], dot);
-        dot += __shfl_xor(dot, 32, 64);
-#pragma unroll
-        for (int a = 0; a < NT; ++a)
-#pragma unroll
-            for (int e = 0; e < 16; ++e) {
-                ds[a][e] = i < N ? p[a][e] * (ds[a][e] - dot) : 0.f;
-                db[a][e] += ds[a][e];
-            }
-        typename Lds<T>::Operand po[NT], so[NT];
-#pragma unroll
-        for (int a = 0; a < NT; ++a) po[a] = Lds<T>::operand(p[a]), so[a] = Lds<T>::operand(ds[a]);
+        for (int s = 0; s < 4 * NA; ++s) {
+            ds[s >> 2][s & 3] = s < NS ? p[s >> 2][s & 3] * (ds[s >> 2][s & 3] - dot) : 0.f;
+            db[s >> 2][s & 3] += ds[s >> 2][s & 3];
+        }
+        const auto po = Lds<T>::template operand<NA>(p), so = Lds<T>::template operand<NA>(ds);
         {
-            f32x16 o = zero16();
-            Lds<T>::template columns_product<NT>(o, K, so, N, lane);
-            store_tile(dq, stride, i, N, hh, o, scale);
+            f32x4 o[2] = {kZero4, kZero4};
+            Lds<T>::template columns_product<NS>(o, K, so, lane);
+            store_tile(dq, stride, i, N, lane, o, scale);
         }
         __syncthreads();                               // K and V are read
-        Lds<T>::template cross_write<NT>(X, po, i, N, hh);
+        Lds<T>::template cross_write<NA>(X, po, w, lane);
         __syncthreads();                               // every query row of P is there
         win + nslab < windows ? fetch(win + nslab) : none();          // (not before: the registers are the scores' and P's until here)
         {
-            f32x16 o = zero16();
-            Lds<T>::template cross_product<NT>(o, G, X, w, N, lane);
-            store_tile(dq + 2 * C, stride, i, N, hh, o, 1.f);
+            f32x4 o[2] = {kZero4, kZero4};
+            Lds<T>::template cross_product<NS>(o, G, X, w, lane);
+            store_tile(dq + 2 * C, stride, j, N, lane, o, 1.f);
         }
         __syncthreads();                               // P is read
-        Lds<T>::template cross_write<NT>(X, so, i, N, hh);
+        Lds<T>::template cross_write<NA>(X, so, w, lane);
         __syncthreads();
         {
-            f32x16 o = zero16();
-            Lds<T>::template cross_product<NT>(o, Q, X, w, N, lane);
-            store_tile(dq + C, stride, i, N, hh, o, scale);
+            f32x4 o[2] = {kZero4, kZero4};
+            Lds<T>::template cross_product<NS>(o, Q, X, w, lane);
+            store_tile(dq + C, stride, j, N, lane, o, scale);
         }
     }
-    float4 *to = reinterpret_cast<float4 *>(slabs + (size_t)job * (NT * NT * 1024)) + w * 256 + lane;
+    f32x4 *to = reinterpret_cast<f32x4 *>(slabs + (size_t)job * (NA * NA * 256)) + w * NA * 64 + lane;
 #pragma unroll
-    for (int a = 0; a < NT; ++a)
-#pragma unroll
-        for (int g = 0; g < 4; ++g) to[(a * NT * 4 + g) * 64] = make_float4(db[a][4 * g], db[a][4 * g + 1], db[a][4 * g + 2], db[a][4 * g + 3]);
+    for (int a = 0; a < NA; ++a) to[a * 64] = db[a];
 }
 
 // dbias[head][i][j] = the sum of the slabs, unpacked.  Sixteen waves take every sixteenth slab of the same 64 float4 each; their sums join in wave order.
-template <int NT>
+template <int NA>
 __global__ __launch_bounds__(1024) void window_train_dbias(const float *__restrict__ slabs, float *__restrict__ dbias, int nslab, int heads, int N) {
     __shared__ float4 part[16][64];
-    const int head = blockIdx.y, lane = threadIdx.x & 63, wv = threadIdx.x >> 6, at = blockIdx.x * 64 + lane;      // float4 number at of the table
-    const float4 *src = reinterpret_cast<const float4 *>(slabs) + (size_t)head * (NT * NT * 256) + at;
+    const int head = blockIdx.y, lane = threadIdx.x & 63, wv = threadIdx.x >> 6, ab = blockIdx.x;      // one pair of tiles
+    const float4 *src = reinterpret_cast<const float4 *>(slabs) + ((size_t)head * (NA * NA) + ab) * 64 + lane;
     float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 4
     for (int k = wv; k < nslab; k += 16) {
-        const float4 v = src[(size_t)k * heads * (NT * NT * 256)];
+        const float4 v = src[(size_t)k * heads * (NA * NA * 64)];
         s.x += v.x, s.y += v.y, s.z += v.z, s.w += v.w;
     }
     part[wv][lane] = s;
@@ -467,38 +473,40 @@ __global__ __launch_bounds__(1024) void window_train_dbias(const float *__restri
         const float4 v = part[k][lane];
         s.x += v.x, s.y += v.y, s.z += v.z, s.w += v.w;
     }
-    const int l = at & 63, g = (at >> 6) & 3, ab = at >> 8, b = ab % NT, a = ab / NT;
-    const int j = 32 * a + 8 * g + 4 * (l >> 5), i = 32 * b + (l & 31);
+    const int j = 16 * (ab % NA) + (lane >> 4), i = 16 * (ab / NA) + (lane & 15);
     if (i >= N) return;
     float *to = dbias + ((size_t)head * N + i) * N + j;
     if (j < N) to[0] = s.x;
-    if (j + 1 < N) to[1] = s.y;
-    if (j + 2 < N) to[2] = s.z;
-    if (j + 3 < N) to[3] = s.w;
+    if (j + 4 < N) to[4] = s.y;
+    if (j + 8 < N) to[8] = s.z;
+    if (j + 12 < N) to[12] = s.w;
 }
 
 // ---- launches ---------------------------------------------------------------------------------------------------------------------------------
-// Workgroups of a pass: as many as fit the 256 CUs at once (`per_cu`, by LDS), each with the same number of windows but for the last ones.
+// Workgroups of a pass: as many as fit the 256 CUs at once (`per_cu`, by LDS and registers), each with the same number of windows but for the last ones.
 int slabs_for(long windows, int heads, int per_cu) {
     const long per = (windows * heads + 256L * per_cu - 1) / (256L * per_cu);
     return (int)((windows + per - 1) / per);
 }
+constexpr int steps(int N) { return (N + 3) / 4; }
+constexpr int tiles(int N) { return tiles_of(steps(N)); }
 template <typename T>
-size_t fwd_lds(int N) { return 3 * image_elems<T>(N) * sizeof(T); }
+size_t fwd_lds(int NA) { return 3 * image_elems<T>(NA) * sizeof(T); }
 template <typename T>
-size_t bwd_lds(int N) {
-    const size_t two = 2 * image_elems<T>(N) * sizeof(T), cross = Lds<T>::cross_bytes(N, N <= 32 ? 1 : 2);
+size_t bwd_lds(int NA) {
+    const size_t two = 2 * image_elems<T>(NA) * sizeof(T), cross = Lds<T>::cross_bytes(NA);
     return two + (two > cross ? two : cross);
 }
-int per_cu(size_t lds, int most) {
-    const int n = (int)(160 * 1024 / (lds + 512));
-    return n < most ? n : most;
+int per_cu(size_t lds, int waves_per_simd, int NA) {
+    const int by_lds = (int)(160 * 1024 / (lds + 512)), by_waves = 4 * waves_per_simd / NA;
+    return by_lds < by_waves ? by_lds : by_waves;
 }
 template <typename T>
-int bwd_slabs(long windows, int heads, int N) { return slabs_for(windows, heads, per_cu(bwd_lds<T>(N), kBwdWaves * (N <= 32 ? 4 : 2))); }
+int bwd_slabs(long windows, int heads, int N) { return slabs_for(windows, heads, per_cu(bwd_lds<T>(tiles(N)), kBwdWaves, tiles(N))); }
 
 bool shape_ok(long windows, int heads, int N) { return windows > 0 && heads > 0 && heads <= 65535 && windows <= 0x3fffffffL / heads && N >= 1 && N <= 64; }
-size_t table_floats(int heads, int nW, int N) { return (size_t)(heads + nW) * (N <= 32 ? 1024 : 4096); }
+size_t table_elems(int N) { return (size_t)tiles(N) * tiles(N) * 256; }
+size_t table_floats(int heads, int nW, int N) { return (size_t)(heads + nW) * table_elems(N); }
 
 int check_args(const void *qkv, const float *packed, size_t packed_floats, int dtype, long windows, int nW, int heads, int N, int d) {
     if (!qkv || !packed) return SD_E_NULL;
@@ -510,25 +518,34 @@ int check_args(const void *qkv, const float *packed, size_t packed_floats, int d
     return SD_OK;
 }
 
-template <typename T, int NT>
+template <typename T, int NS, int NA = tiles_of(NS)>
 int fwd_launch(const void *qkv, const float *bias, const float *mask, float *packed, void *out, long windows, int nW, int heads, int N, float scale, hipStream_t st) {
     int *any = reinterpret_cast<int *>(packed + table_floats(heads, nW, N));
-    hipLaunchKernelGGL((window_tables<NT>), dim3((unsigned)(heads + nW)), dim3(256), 0, st, bias, mask, packed, any, heads, N);
-    const size_t lds = fwd_lds<T>(N);
-    const int ns = slabs_for(windows, heads, per_cu(lds, N <= 32 ? 12 : 6));
-    hipLaunchKernelGGL((window_train_fwd<T, NT>), dim3((unsigned)(ns * heads)), dim3(64 * NT), lds, st, static_cast<const T *>(qkv), packed, any, static_cast<T *>(out),
+    hipLaunchKernelGGL((window_tables<NA>), dim3((unsigned)(heads + nW)), dim3(256), 0, st, bias, mask, packed, any, heads, N);
+    const size_t lds = fwd_lds<T>(NA);
+    const int ns = slabs_for(windows, heads, per_cu(lds, kFwdWaves<T>, NA));
+    hipLaunchKernelGGL((window_train_fwd<T, NS>), dim3((unsigned)(ns * heads)), dim3(64 * NA), lds, st, static_cast<const T *>(qkv), packed, any, static_cast<T *>(out),
                        (int)windows, ns, nW, heads, N, scale);
     return (int)hipGetLastError();
 }
-template <typename T, int NT>
+template <typename T, int NS, int NA = tiles_of(NS)>
 int bwd_launch(const void *qkv, const float *packed, const void *dout, void *dqkv, float *dbias, long windows, int nW, int heads, int N, float scale, float *slabs,
                hipStream_t st) {
     const int *any = reinterpret_cast<const int *>(packed + table_floats(heads, nW, N));
     const int ns = bwd_slabs<T>(windows, heads, N);
-    hipLaunchKernelGGL((window_train_bwd<T, NT>), dim3((unsigned)(ns * heads)), dim3(64 * NT), bwd_lds<T>(N), st, static_cast<const T *>(qkv), packed, any,
+    hipLaunchKernelGGL((window_train_bwd<T, NS>), dim3((unsigned)(ns * heads)), dim3(64 * NA), bwd_lds<T>(NA), st, static_cast<const T *>(qkv), packed, any,
                        static_cast<const T *>(dout), static_cast<T *>(dqkv), slabs, (int)windows, ns, nW, heads, N, scale);
-    hipLaunchKernelGGL((window_train_dbias<NT>), dim3(NT * NT * 4, (unsigned)heads), dim3(1024), 0, st, slabs, dbias, ns, heads, N);
+    hipLaunchKernelGGL((window_train_dbias<NA>), dim3(NA * NA, (unsigned)heads), dim3(1024), 0, st, slabs, dbias, ns, heads, N);
     return (int)hipGetLastError();
+}
+
+// fn(NS as a compile-time constant) for the window's NS
+template <int NS = 16, typename F>
+int with_steps(int ns, F fn) {
+    if constexpr (NS > 1) {
+        if (ns < NS) return with_steps<NS - 1>(ns, fn);
+    }
+    return fn(std::integral_constant<int, NS>());
 }
 
 }  // namespace
@@ -551,16 +568,16 @@ int sd_window_attn_train_fwd(const void *qkv, const float *bias, const float *ma
     if ((reinterpret_cast<uintptr_t>(out) & 15) || ((reinterpret_cast<uintptr_t>(bias) | reinterpret_cast<uintptr_t>(mask)) & 3)) return SD_E_ALIGN;
     hipStream_t st = static_cast<hipStream_t>(stream);
     const int N = tokens_per_window;
-#define SD_FWD(T, NT) sd::fwd_launch<T, NT>(qkv, bias, mask, packed, out, windows, mask_windows, heads, N, scale, st)
-    if (dtype == SD_F32) return N <= 32 ? SD_FWD(float, 1) : SD_FWD(float, 2);
-    return N <= 32 ? SD_FWD(sd::bf16_t, 1) : SD_FWD(sd::bf16_t, 2);
-#undef SD_FWD
+    return sd::with_steps(sd::steps(N), [&](auto ns) {
+        return dtype == SD_F32 ? sd::fwd_launch<float, ns()>(qkv, bias, mask, packed, out, windows, mask_windows, heads, N, scale, st)
+                               : sd::fwd_launch<sd::bf16_t, ns()>(qkv, bias, mask, packed, out, windows, mask_windows, heads, N, scale, st);
+    });
 }
 
 size_t sd_window_attn_train_workspace_bytes(int dtype, long windows, int heads, int tokens_per_window) {
     if (!sd::shape_ok(windows, heads, tokens_per_window) || (dtype != SD_F32 && dtype != SD_BF16)) return 0;
     const int N = tokens_per_window, ns = dtype == SD_F32 ? sd::bwd_slabs<float>(windows, heads, N) : sd::bwd_slabs<sd::bf16_t>(windows, heads, N);
-    return (size_t)ns * heads * (N <= 32 ? 1024 : 4096) * sizeof(float);
+    return (size_t)ns * heads * sd::table_elems(N) * sizeof(float);
 }
 
 int sd_window_attn_train_bwd(const void *qkv, const float *packed, size_t packed_floats, const void *dout, void *dqkv, float *dbias, int dtype, long windows,
@@ -574,10 +591,10 @@ int sd_window_attn_train_bwd(const void *qkv, const float *packed, size_t packed
     hipStream_t st = static_cast<hipStream_t>(stream);
     const int N = tokens_per_window;
     float *slabs = static_cast<float *>(workspace);
-#define SD_BWD(T, NT) sd::bwd_launch<T, NT>(qkv, packed, dout, dqkv, dbias, windows, mask_windows, heads, N, scale, slabs, st)
-    if (dtype == SD_F32) return N <= 32 ? SD_BWD(float, 1) : SD_BWD(float, 2);
-    return N <= 32 ? SD_BWD(sd::bf16_t, 1) : SD_BWD(sd::bf16_t, 2);
-#undef SD_BWD
+    return sd::with_steps(sd::steps(N), [&](auto ns) {
+        return dtype == SD_F32 ? sd::bwd_launch<float, ns()>(qkv, packed, dout, dqkv, dbias, windows, mask_windows, heads, N, scale, slabs, st)
+                               : sd::bwd_launch<sd::bf16_t, ns()>(qkv, packed, dout, dqkv, dbias, windows, mask_windows, heads, N, scale, slabs, st);
+    });
 }
 
 }  // extern "C"
