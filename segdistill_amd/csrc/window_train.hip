@@ -9,9 +9,10 @@
 //
 // A workgroup keeps one head and walks over windows; wave w of its NA = ceil(N / 16) waves owns the 16 queries of tile w, then (dV, dK) the 16 keys
 // of tile w.  The operands of a window come into LDS as rows, 16 bytes per thread, and the next window's are on their way to registers meanwhile.
-// S^T = K Q^T puts query i = 16 w + (lane & 15) on the lane and its keys into the accumulators.  The rows of K enter in an order (key_of_row) that makes
-// accumulator s = 4 a + e of the lanes q = lane >> 4 the keys 4 s + q: only NS = ceil(N / 4) accumulators hold keys, and NS is known to the compiler (13 of
-// 16 for 7 x 7 windows).  The softmax is in-lane plus two exchanges, and P^T is the B operand of O^T = V^T P^T as it stands.  The products that sum over queries need the lane to be the key: P, then dS,
+// S^T = K Q^T puts query i = 16 w + (lane & 15) on the lane and its keys into the accumulators: keys 16 a + 4 q + e of the lanes q = lane >> 4 in
+// accumulator e of tile a.  A last tile that is not full takes the rows of K in another order (spread), keys 16 a + 4 e + q: the keys it lacks are then
+// whole accumulators, NS = ceil(N / 4) hold keys, and NS is known to the compiler (13 of 16 for 7 x 7 windows).  The softmax is in-lane plus two exchanges,
+// and P^T is the B operand of O^T = V^T P^T as it stands.  The products that sum over queries need the lane to be the key: P, then dS,
 // cross through LDS.  The bias gradient of all windows of a workgroup stays in its accumulators and leaves once, as one slab; the slabs are joined in
 // slab order.
 //   fp32 storage: v_mfma_f32_16x16x4_f32, exact products.
@@ -40,17 +41,20 @@ constexpr f32x4 kZero4 = {0.f, 0.f, 0.f, 0.f};
 
 // ---- products on LDS images ------------------------------------------------------------------------------------------------------------------
 // An image holds 16 NA rows of 32 elements, PITCH apart (16-byte pieces of 16 rows cover the banks); rows behind the window are zero.  The cross image
-// holds one row of keys per query, a tile's keys in the order of the accumulators.  r = lane & 15, q = lane >> 4; sums over tokens run in steps s, token
-// 4 s + q.
-__device__ __forceinline__ int key_of_row(int r) { return 4 * (r & 3) + (r >> 2); }
+// holds one row of keys per query, a tile's keys in the order of the accumulators.  r = lane & 15, q = lane >> 4.  Sums over tokens take them in the order of
+// the accumulators, too: token_of(q, e, spread) of tile a in step 4 a + e.
 constexpr int tiles_of(int NS) { return (NS + 3) / 4; }
+__host__ __device__ constexpr bool spread_tile(int a, int NS) { return a == NS / 4; }            // the tile that is not full, if there is one
+__device__ __forceinline__ int token_of(int q, int e, bool spread) { return spread ? 4 * e + q : 4 * q + e; }
+__device__ __forceinline__ int token_of_row(int r, bool spread) { return token_of(r >> 2, r & 3, spread); }      // the tile's row r holds accumulator r & 3 of q = r >> 2
 template <typename T>
 struct Lds;
 
 template <>
 struct Lds<float> {
     static constexpr int PITCH = 36, CHUNKS = 8;                                  // CHUNKS: 16-byte pieces of a row
-    static __host__ __device__ constexpr int cross_pitch(int NA) { return 16 * NA + 4; }
+    static __device__ __forceinline__ int chunk(int, int ch) { return ch; }
+    static __host__ __device__ constexpr int cross_pitch(int NA) { return 16 * NA + 4; }          // 16 columns of every fourth row cover the banks, as those of an image
     static __host__ __device__ constexpr size_t cross_bytes(int NA) { return (size_t)16 * NA * cross_pitch(NA) * 4; }
 
     template <int NA>
@@ -64,30 +68,33 @@ struct Lds<float> {
         for (int a = 0; a < NA; ++a) o.v[a] = p[a];
         return o;
     }
-    // acc[a][m][n] += sum_d A[16 a + key_of_row(m)][d] B[16 w + n][d]
-    template <int NA>
+    // acc[a][m][n] += sum_d A[16 a + token_of_row(m)][d] B[16 w + n][d]
+    template <int NS, int NA = tiles_of(NS)>
     static __device__ __forceinline__ void rows_product(f32x4 (&acc)[NA], const float *A, const float *B, int w, int lane) {
         const int r = lane & 15, d = 8 * (lane >> 4);
-        const float *pa = A + key_of_row(r) * PITCH + d, *pb = B + (16 * w + r) * PITCH + d;
+        const float *full = A + r * PITCH + d, *part = A + token_of_row(r, true) * PITCH + d, *pb = B + (16 * w + r) * PITCH + d;
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
             const f32x4 bv = *reinterpret_cast<const f32x4 *>(pb + 4 * u);
+            f32x4 av[NA];
 #pragma unroll
-            for (int a = 0; a < NA; ++a) {
-                const f32x4 av = *reinterpret_cast<const f32x4 *>(pa + 16 * a * PITCH + 4 * u);
+            for (int a = 0; a < NA; ++a) av[a] = *reinterpret_cast<const f32x4 *>((spread_tile(a, NS) ? part : full) + 16 * a * PITCH + 4 * u);
 #pragma unroll
-                for (int c = 0; c < 4; ++c) acc[a] = __builtin_amdgcn_mfma_f32_16x16x4f32(av[c], bv[c], acc[a], 0, 0, 0);
-            }
+            for (int c = 0; c < 4; ++c)
+#pragma unroll
+                for (int a = 0; a < NA; ++a) acc[a] = __builtin_amdgcn_mfma_f32_16x16x4f32(av[a][c], bv[c], acc[a], 0, 0, 0);
         }
     }
     // acc[h][d][i] += sum_j M[j][16 h + d] p[j][i]
     template <int NS>
     static __device__ __forceinline__ void columns_product(f32x4 (&acc)[2], const float *M, const Operand<tiles_of(NS)> &p, int lane) {
-        const float *m = M + (lane >> 4) * PITCH + (lane & 15);
+        const int q = lane >> 4, r = lane & 15;
 #pragma unroll
-        for (int s = 0; s < NS; ++s)
+        for (int s = 0; s < NS; ++s) {
+            const float *m = M + (16 * (s >> 2) + token_of(q, s & 3, spread_tile(s >> 2, NS))) * PITCH + r;
 #pragma unroll
-            for (int h = 0; h < 2; ++h) acc[h] = __builtin_amdgcn_mfma_f32_16x16x4f32(m[4 * s * PITCH + 16 * h], p.v[s >> 2][s & 3], acc[h], 0, 0, 0);
+            for (int h = 0; h < 2; ++h) acc[h] = __builtin_amdgcn_mfma_f32_16x16x4f32(m[16 * h], p.v[s >> 2][s & 3], acc[h], 0, 0, 0);
+        }
     }
     // the wave's query rows of p into the cross image
     template <int NA>
@@ -96,33 +103,36 @@ struct Lds<float> {
 #pragma unroll
         for (int a = 0; a < NA; ++a) *reinterpret_cast<f32x4 *>(to + 16 * a) = p.v[a];
     }
-    // acc[h][d][n] += sum_i M[i][16 h + d] x[i][16 w + n]: key 16 w + key_of_row(n)
+    // acc[h][d][n] += sum_i M[i][16 h + d] x[i][16 w + n]
     template <int NS>
     static __device__ __forceinline__ void cross_product(f32x4 (&acc)[2], const float *M, const float *x, int w, int lane) {
         constexpr int pitch = cross_pitch(tiles_of(NS));
-        const int r = lane & 15, q = lane >> 4;
-        const float *m = M + q * PITCH + r, *b = x + q * pitch + 16 * w + r;
+        const int q = lane >> 4, r = lane & 15;
 #pragma unroll
         for (int s = 0; s < NS; ++s) {
-            const float bv = b[4 * s * pitch];
+            const int i = 16 * (s >> 2) + token_of(q, s & 3, spread_tile(s >> 2, NS));
+            const float bv = x[i * pitch + 16 * w + r];
 #pragma unroll
-            for (int h = 0; h < 2; ++h) acc[h] = __builtin_amdgcn_mfma_f32_16x16x4f32(m[4 * s * PITCH + 16 * h], bv, acc[h], 0, 0, 0);
+            for (int h = 0; h < 2; ++h) acc[h] = __builtin_amdgcn_mfma_f32_16x16x4f32(M[i * PITCH + 16 * h + r], bv, acc[h], 0, 0, 0);
         }
     }
 };
 
 template <>
 struct Lds<bf16_t> {
-    static constexpr int PITCH = 40, CHUNKS = 4;
-    static __host__ __device__ constexpr int cross_pitch(int NA) { return 16 * NA + 8; }
+    // Rows are an odd number of eight banks apart, so that the 32 lanes of a transposed read (four rows x 16 columns for each 16 of them) meet every bank
+    // once; rows 8 .. 15 of a tile have neighbouring 16-byte pieces exchanged, so that 16 rows do where they are read or written by rows.
+    static constexpr int PITCH = 48, CHUNKS = 4;
+    static __device__ __forceinline__ int chunk(int row, int ch) { return ch ^ ((row >> 3) & 1); }
+    static __host__ __device__ constexpr int cross_pitch(int NA) { return NA == 1 ? 16 : NA == 4 ? 80 : 48; }
     static __host__ __device__ constexpr size_t plane(int NA) { return (size_t)16 * NA * cross_pitch(NA); }       // elements of one of the two terms
     static __host__ __device__ constexpr size_t cross_bytes(int NA) { return 2 * plane(NA) * 2; }
 
-    // four rows x 16 columns per 16 lanes, delivered by column: lane 16 q + r gets column r of the rows q, q + 4, q + 8, q + 12 behind `img`
-    static __device__ __forceinline__ s16x4 columns(const bf16_t *img, int pitch, int lane) {
+    // four rows x 16 columns per 16 lanes, delivered by column: lane 16 q + r gets column r of the four tokens that the lanes q hold
+    static __device__ __forceinline__ s16x4 columns(const bf16_t *tile, int pitch, bool spread, int lane) {
         typedef s16x4 __attribute__((address_space(3))) * lds_p;
-        const int li = lane & 15;
-        return __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_p)(img + ((lane >> 4) + 4 * (li >> 2)) * pitch + 4 * (li & 3)));
+        const int row = token_of(lane >> 4, (lane >> 2) & 3, spread);
+        return __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_p)(tile + row * pitch + 8 * chunk(row, (lane >> 1) & 1) + 4 * (lane & 1)));
     }
     static __device__ __forceinline__ bf16x8 join(s16x4 lo, s16x4 hi) {
         const s16x8 v = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
@@ -157,13 +167,26 @@ struct Lds<bf16_t> {
         }
         return o;
     }
-    template <int NA>
+    template <int NS, int NA = tiles_of(NS)>
     static __device__ __forceinline__ void rows_product(f32x4 (&acc)[NA], const bf16_t *A, const bf16_t *B, int w, int lane) {
-        const int r = lane & 15, d = 8 * (lane >> 4);
-        const bf16_t *pa = A + key_of_row(r) * PITCH + d;
-        const bf16x8 bv = *reinterpret_cast<const bf16x8 *>(B + (16 * w + r) * PITCH + d);
+        const int r = lane & 15, q = lane >> 4;
+        const bf16x8 bv = *reinterpret_cast<const bf16x8 *>(B + (16 * w + r) * PITCH + 8 * chunk(r, q));
 #pragma unroll
-        for (int a = 0; a < NA; ++a) acc[a] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(*reinterpret_cast<const bf16x8 *>(pa + 16 * a * PITCH), bv, acc[a], 0, 0, 0);
+        for (int a = 0; a < NA; ++a) {
+            const int row = token_of_row(r, spread_tile(a, NS));
+            acc[a] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(*reinterpret_cast<const bf16x8 *>(A + (16 * a + row) * PITCH + 8 * chunk(row, q)), bv, acc[a], 0, 0, 0);
+        }
+    }
+    template <int NA>
+    static __device__ __forceinline__ void product(f32x4 &acc, const s16x4 (&m)[NA], const Operand<NA> &p) {
+#pragma unroll
+        for (int a = 0; a < NA; a += 2) {
+            const s16x4 zero = {0, 0, 0, 0};
+            const bool pair = a + 1 < NA;
+            const int b = pair ? a + 1 : a;
+            acc = mfma32(m[a], pair ? m[b] : zero, p.first[a], pair ? p.first[b] : zero, acc);
+            acc = mfma32(m[a], pair ? m[b] : zero, p.second[a], pair ? p.second[b] : zero, acc);
+        }
     }
     template <int NS, int NA = tiles_of(NS)>
     static __device__ __forceinline__ void columns_product(f32x4 (&acc)[2], const bf16_t *M, const Operand<NA> &p, int lane) {
@@ -171,20 +194,14 @@ struct Lds<bf16_t> {
         for (int h = 0; h < 2; ++h) {
             s16x4 m[NA];
 #pragma unroll
-            for (int a = 0; a < NA; ++a) m[a] = columns(M + 16 * a * PITCH + 16 * h, PITCH, lane);
-#pragma unroll
-            for (int a = 0; a < NA; a += 2) {
-                const s16x4 zero = {0, 0, 0, 0};
-                const bool pair = a + 1 < NA;
-                const int b = pair ? a + 1 : a;
-                acc[h] = mfma32(m[a], pair ? m[b] : zero, p.first[a], pair ? p.first[b] : zero, acc[h]);
-                acc[h] = mfma32(m[a], pair ? m[b] : zero, p.second[a], pair ? p.second[b] : zero, acc[h]);
-            }
+            for (int a = 0; a < NA; ++a) m[a] = columns(M + 16 * a * PITCH + 16 * h, PITCH, spread_tile(a, NS), lane);
+            product<NA>(acc[h], m, p);
         }
     }
     template <int NA>
     static __device__ __forceinline__ void cross_write(bf16_t *x, const Operand<NA> &p, int w, int lane) {
-        bf16_t *to = x + (16 * w + (lane & 15)) * cross_pitch(NA) + 4 * (lane >> 4);
+        const int r = lane & 15;
+        bf16_t *to = x + (16 * w + r) * cross_pitch(NA) + 8 * chunk(r, lane >> 5) + 4 * ((lane >> 4) & 1);
 #pragma unroll
         for (int a = 0; a < NA; ++a) {
             *reinterpret_cast<s16x4 *>(to + 16 * a) = p.first[a];
@@ -197,10 +214,16 @@ struct Lds<bf16_t> {
 #pragma unroll
         for (int a = 0; a < NA; ++a) {
             const bf16_t *from = x + 16 * a * cross_pitch(NA) + 16 * w;
-            p.first[a] = columns(from, cross_pitch(NA), lane);
-            p.second[a] = columns(from + plane(NA), cross_pitch(NA), lane);
+            p.first[a] = columns(from, cross_pitch(NA), false, lane);
+            p.second[a] = columns(from + plane(NA), cross_pitch(NA), false, lane);
         }
-        columns_product<NS>(acc, M, p, lane);
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            s16x4 m[NA];
+#pragma unroll
+            for (int a = 0; a < NA; ++a) m[a] = columns(M + 16 * a * PITCH + 16 * h, PITCH, false, lane);
+            product<NA>(acc[h], m, p);
+        }
     }
 };
 
@@ -230,7 +253,7 @@ struct Stage {
         const int row = threadIdx.x / CH, ch = threadIdx.x % CH;
 #pragma unroll
         for (int u = 0; u < PASSES; ++u)
-            if (row + u * STEP < N) *(reinterpret_cast<u32x4 *>(img + (row + u * STEP) * Lds<T>::PITCH) + ch) = reg[u];
+            if (row + u * STEP < N) *(reinterpret_cast<u32x4 *>(img + (row + u * STEP) * Lds<T>::PITCH) + Lds<T>::chunk(row + u * STEP, ch)) = reg[u];
     }
 };
 // the zero rows behind an image's last one
@@ -271,16 +294,23 @@ __device__ __forceinline__ float row_sum(float v) {
     v += __shfl_xor(v, 16, 64);
     return v + __shfl_xor(v, 32, 64);
 }
-// what is added to the wave's scores: the tiles of the bias, and of the mask if it says anything
+// what is added to the wave's scores: its tiles of the bias, plus those of the mask if it says anything
 template <int NA>
-__device__ __forceinline__ void load_added(f32x4 (&t)[NA], const float *__restrict__ packed, int head, int mask, int w, int lane) {
-    const f32x4 *from = reinterpret_cast<const f32x4 *>(packed) + w * NA * 64 + lane;
+__device__ __forceinline__ const f32x4 *table_tiles(const float *packed, int table, int w, int lane) {
+    return reinterpret_cast<const f32x4 *>(packed) + (size_t)table * (NA * NA * 64) + w * NA * 64 + lane;
+}
+template <int NA>
+__device__ __forceinline__ void load_bias(f32x4 (&t)[NA], const float *__restrict__ packed, int head, int w, int lane) {
+    const f32x4 *from = table_tiles<NA>(packed, head, w, lane);
 #pragma unroll
-    for (int a = 0; a < NA; ++a) t[a] = from[(size_t)head * (NA * NA * 64) + a * 64];
-    if (mask >= 0) {
+    for (int a = 0; a < NA; ++a) t[a] = from[a * 64];
+}
+template <int NA>
+__device__ __forceinline__ void add_mask(f32x4 (&t)[NA], const float *__restrict__ packed, const int *__restrict__ any, int heads, int win, int nW, int w, int lane) {
+    if (nW == 0 || !any[win % nW]) return;
+    const f32x4 *from = table_tiles<NA>(packed, heads + win % nW, w, lane);
 #pragma unroll
-        for (int a = 0; a < NA; ++a) t[a] += from[(size_t)mask * (NA * NA * 64) + a * 64];
-    }
+    for (int a = 0; a < NA; ++a) t[a] += from[a * 64];
 }
 // p: K Q^T on entry, e^(S - max) on return, 0 in the accumulators without keys -> 1 / sum, 0 for a row that has nothing left
 template <int NS, int NA = tiles_of(NS)>
@@ -303,7 +333,7 @@ __device__ __forceinline__ float softmax_tile(f32x4 (&p)[NA], const f32x4 (&adde
 }
 
 // ---- tables --------------------------------------------------------------------------------------------------------------------------------------
-// bias [heads][N][N], then mask [nW][N][N], into the accumulator layout [query tile][key tile][lane][e], key 16 a + 4 e + (lane >> 4): padded keys -inf in the bias and 0 in the mask,
+// bias [heads][N][N], then mask [nW][N][N], into the accumulator layout [query tile][key tile][lane][e]: padded keys -inf in the bias and 0 in the mask,
 // padded queries 0; any[w] = the mask of window w has a nonzero entry
 template <int NA>
 __global__ __launch_bounds__(256) void window_tables(const float *__restrict__ bias, const float *__restrict__ mask, float *__restrict__ packed, int *__restrict__ any,
@@ -314,7 +344,7 @@ __global__ __launch_bounds__(256) void window_tables(const float *__restrict__ b
     int nonzero = 0;
     for (int at = threadIdx.x; at < NA * NA * 256; at += 256) {
         const int e = at & 3, lane = (at >> 2) & 63, ab = at >> 8, a = ab % NA, b = ab / NA;
-        const int j = 16 * a + 4 * e + (lane >> 4), i = 16 * b + (lane & 15);
+        const int j = 16 * a + token_of(lane >> 4, e, spread_tile(a, (N + 3) / 4)), i = 16 * b + (lane & 15);
         const float v = j >= N ? pad : (i < N ? src[(size_t)i * N + j] : 0.f);
         packed[(size_t)t * (NA * NA * 256) + at] = v;
         nonzero |= v != 0.f;
@@ -329,10 +359,11 @@ __device__ __forceinline__ int logical_block() {
     return (x < rem ? x * (q + 1) : rem * (q + 1) + (x - rem) * q) + id / 8;
 }
 
-// waves per SIMD that the registers leave room for
+// waves per SIMD that the registers leave room for (7 x 7 windows, stage 1: forward fp32 5 without the bias in registers level, bf16 4 and 6 without it 24
+// and 27 against 23 us; backward 4, then with P and dS crossing one after the other, level, 2: 143 against 130 us, bf16 59 against 54)
 template <typename T>
-constexpr int kFwdWaves = sizeof(T) == 4 ? 5 : 6;
-constexpr int kBwdWaves = 4;
+constexpr int kFwdWaves = sizeof(T) == 4 ? 4 : 5;
+constexpr int kBwdWaves = 3;
 
 template <typename T, int NS, int NA = tiles_of(NS)>
 __global__ __launch_bounds__(64 * NA, kFwdWaves<T>) void window_train_fwd(const T *__restrict__ qkv, const float *__restrict__ packed, const int *__restrict__ any,
@@ -351,21 +382,23 @@ __global__ __launch_bounds__(64 * NA, kFwdWaves<T>) void window_train_fwd(const 
         sq.load(q, stride, N), sk.load(q + C, stride, N), sv.load(q + 2 * C, stride, N);
     };
     auto none = [&]() { sq.clear(), sk.clear(), sv.clear(); };          // a value on both ways: else the old one would stay live through the loop
+    f32x4 bias[NA];
+    load_bias<NA>(bias, packed, head, w, lane);
     fetch(slab);
     zero_tail<T, NA>(Q, N), zero_tail<T, NA>(K, N), zero_tail<T, NA>(V, N);
     for (int win = slab; win < windows; win += nslab) {
         __syncthreads();                               // the previous window's images are read
         sq.store(Q, N), sk.store(K, N), sv.store(V, N);
         f32x4 added[NA];
-        int table = head;
-        asm volatile("" : "+s"(table));                // loaded anew: kept over the loop it would not fit the registers
-        load_added<NA>(added, packed, table, nW && any[win % nW] ? heads + win % nW : -1, w, lane);
-        win + nslab < windows ? fetch(win + nslab) : none();          // behind the tables: what is asked for first arrives first
+#pragma unroll
+        for (int a = 0; a < NA; ++a) added[a] = bias[a];
+        add_mask<NA>(added, packed, any, heads, win, nW, w, lane);
+        win + nslab < windows ? fetch(win + nslab) : none();          // behind the mask: what is asked for first arrives first
         __syncthreads();
         f32x4 p[NA], o[2] = {kZero4, kZero4};
 #pragma unroll
         for (int a = 0; a < NA; ++a) p[a] = kZero4;
-        Lds<T>::template rows_product<NA>(p, K, Q, w, lane);
+        Lds<T>::template rows_product<NS>(p, K, Q, w, lane);
         const float inv = softmax_tile<NS>(p, added, scale);
         Lds<T>::template columns_product<NS>(o, V, Lds<T>::template operand<NA>(p), lane);
         store_tile(out + (size_t)win * N * C + (size_t)head * D, C, i, N, lane, o, inv);
@@ -378,8 +411,9 @@ __global__ __launch_bounds__(64 * NA, kBwdWaves) void window_train_bwd(const T *
                                                                        int heads, int N, float scale) {
     extern __shared__ __attribute__((aligned(16))) unsigned char lds[];
     constexpr size_t img = image_elems<T>(NA);
-    T *Q = reinterpret_cast<T *>(lds), *G = Q + img, *K = G + img, *V = K + img, *X = K;          // P and dS cross where K and V were
-    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, i = 16 * w + (lane & 15), j = 16 * w + key_of_row(lane & 15);
+    T *Q = reinterpret_cast<T *>(lds), *G = Q + img, *K = G + img, *V = K + img;
+    T *X = K, *Y = X + Lds<T>::cross_bytes(NA) / sizeof(T);            // P and dS cross where K and V were
+    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, i = 16 * w + (lane & 15), j = 16 * w + token_of_row(lane & 15, spread_tile(w, NS));
     const int job = logical_block(), slab = job / heads, head = job - slab * heads;
     const int C = heads * D, stride = 3 * C;
     const long wstride = (long)N * stride;
@@ -403,15 +437,16 @@ __global__ __launch_bounds__(64 * NA, kBwdWaves) void window_train_bwd(const T *
         f32x4 added[NA];
         int table = head;
         asm volatile("" : "+s"(table));                // loaded anew: kept over the loop it would not fit the registers
-        load_added<NA>(added, packed, table, nW && any[win % nW] ? heads + win % nW : -1, w, lane);
+        load_bias<NA>(added, packed, table, w, lane);
+        add_mask<NA>(added, packed, any, heads, win, nW, w, lane);
         __syncthreads();
         T *dq = dqkv + (size_t)win * wstride + (size_t)head * D;
         f32x4 p[NA], ds[NA];
 #pragma unroll
         for (int a = 0; a < NA; ++a) p[a] = ds[a] = kZero4;
-        Lds<T>::template rows_product<NA>(p, K, Q, w, lane);
+        Lds<T>::template rows_product<NS>(p, K, Q, w, lane);
         const float inv = softmax_tile<NS>(p, added, scale);
-        Lds<T>::template rows_product<NA>(ds, V, G, w, lane);
+        Lds<T>::template rows_product<NS>(ds, V, G, w, lane);
         float dot = 0.f;
 #pragma unroll
         for (int s = 0; s < NS; ++s) {
@@ -432,19 +467,17 @@ __global__ __launch_bounds__(64 * NA, kBwdWaves) void window_train_bwd(const T *
         }
         __syncthreads();                               // K and V are read
         Lds<T>::template cross_write<NA>(X, po, w, lane);
-        __syncthreads();                               // every query row of P is there
-        win + nslab < windows ? fetch(win + nslab) : none();          // (not before: the registers are the scores' and P's until here)
+        Lds<T>::template cross_write<NA>(Y, so, w, lane);
+        __syncthreads();                               // every query row of P and dS is there
+        win + nslab < windows ? fetch(win + nslab) : none();          // (not before: the registers are the scores' until here)
         {
             f32x4 o[2] = {kZero4, kZero4};
             Lds<T>::template cross_product<NS>(o, G, X, w, lane);
             store_tile(dq + 2 * C, stride, j, N, lane, o, 1.f);
         }
-        __syncthreads();                               // P is read
-        Lds<T>::template cross_write<NA>(X, so, w, lane);
-        __syncthreads();
         {
             f32x4 o[2] = {kZero4, kZero4};
-            Lds<T>::template cross_product<NS>(o, Q, X, w, lane);
+            Lds<T>::template cross_product<NS>(o, Q, Y, w, lane);
             store_tile(dq + C, stride, j, N, lane, o, scale);
         }
     }
@@ -473,13 +506,14 @@ __global__ __launch_bounds__(1024) void window_train_dbias(const float *__restri
         const float4 v = part[k][lane];
         s.x += v.x, s.y += v.y, s.z += v.z, s.w += v.w;
     }
-    const int j = 16 * (ab % NA) + (lane >> 4), i = 16 * (ab / NA) + (lane & 15);
+    const bool spread = spread_tile(ab % NA, (N + 3) / 4);
+    const int j = 16 * (ab % NA) + token_of(lane >> 4, 0, spread), step = spread ? 4 : 1, i = 16 * (ab / NA) + (lane & 15);
     if (i >= N) return;
     float *to = dbias + ((size_t)head * N + i) * N + j;
     if (j < N) to[0] = s.x;
-    if (j + 4 < N) to[4] = s.y;
-    if (j + 8 < N) to[8] = s.z;
-    if (j + 12 < N) to[12] = s.w;
+    if (j + step < N) to[step] = s.y;
+    if (j + 2 * step < N) to[2 * step] = s.z;
+    if (j + 3 * step < N) to[3 * step] = s.w;
 }
 
 // ---- launches ---------------------------------------------------------------------------------------------------------------------------------
@@ -494,7 +528,7 @@ template <typename T>
 size_t fwd_lds(int NA) { return 3 * image_elems<T>(NA) * sizeof(T); }
 template <typename T>
 size_t bwd_lds(int NA) {
-    const size_t two = 2 * image_elems<T>(NA) * sizeof(T), cross = Lds<T>::cross_bytes(NA);
+    const size_t two = 2 * image_elems<T>(NA) * sizeof(T), cross = 2 * Lds<T>::cross_bytes(NA);
     return two + (two > cross ? two : cross);
 }
 int per_cu(size_t lds, int waves_per_simd, int NA) {
