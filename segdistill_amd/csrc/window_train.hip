@@ -307,7 +307,7 @@ __device__ __forceinline__ void load_bias(f32x4 (&t)[NA], const float *__restric
 }
 template <int NA>
 __device__ __forceinline__ void add_mask(f32x4 (&t)[NA], const float *__restrict__ packed, const int *__restrict__ any, int heads, int win, int nW, int w, int lane) {
-    if (nW == 0 || !any[win % nW]) return;
+    if (nW == 0 || !any[(win % nW) * NA + w]) return;
     const f32x4 *from = table_tiles<NA>(packed, heads + win % nW, w, lane);
 #pragma unroll
     for (int a = 0; a < NA; ++a) t[a] += from[a * 64];
@@ -334,23 +334,29 @@ __device__ __forceinline__ float softmax_tile(f32x4 (&p)[NA], const f32x4 (&adde
 
 // ---- tables --------------------------------------------------------------------------------------------------------------------------------------
 // bias [heads][N][N], then mask [nW][N][N], into the accumulator layout [query tile][key tile][lane][e]: padded keys -inf in the bias and 0 in the mask,
-// padded queries 0; any[w] = the mask of window w has a nonzero entry
+// padded queries 0; any[NA m + b] = query tile b of mask m has a nonzero entry.  A workgroup per table and query tile, all of a thread's loads at once (361
+// masks of 49 x 49: 8.6 us with a workgroup per table)
 template <int NA>
 __global__ __launch_bounds__(256) void window_tables(const float *__restrict__ bias, const float *__restrict__ mask, float *__restrict__ packed, int *__restrict__ any,
                                                      int heads, int N) {
-    const int t = blockIdx.x;
+    const int t = blockIdx.x, b = blockIdx.y, e = threadIdx.x & 3, lane = threadIdx.x >> 2, i = 16 * b + (lane & 15);
     const float *src = t < heads ? bias + (size_t)t * N * N : mask + (size_t)(t - heads) * N * N;
     const float pad = t < heads ? -INFINITY : 0.f;
+    float v[NA];
+#pragma unroll
+    for (int a = 0; a < NA; ++a) {
+        const int j = 16 * a + token_of(lane >> 4, e, spread_tile(a, (N + 3) / 4));
+        v[a] = src[min(i, N - 1) * N + min(j, N - 1)];
+        v[a] = j >= N ? pad : (i < N ? v[a] : 0.f);
+    }
     int nonzero = 0;
-    for (int at = threadIdx.x; at < NA * NA * 256; at += 256) {
-        const int e = at & 3, lane = (at >> 2) & 63, ab = at >> 8, a = ab % NA, b = ab / NA;
-        const int j = 16 * a + token_of(lane >> 4, e, spread_tile(a, (N + 3) / 4)), i = 16 * b + (lane & 15);
-        const float v = j >= N ? pad : (i < N ? src[(size_t)i * N + j] : 0.f);
-        packed[(size_t)t * (NA * NA * 256) + at] = v;
-        nonzero |= v != 0.f;
+#pragma unroll
+    for (int a = 0; a < NA; ++a) {
+        packed[((size_t)t * NA + b) * (NA * 256) + a * 256 + threadIdx.x] = v[a];
+        nonzero |= v[a] != 0.f;
     }
     nonzero = __syncthreads_or(nonzero);
-    if (t >= heads && threadIdx.x == 0) any[t - heads] = nonzero;
+    if (t >= heads && threadIdx.x == 0) any[(t - heads) * NA + b] = nonzero;
 }
 
 // Workgroups that share windows -- neighbouring heads, whose rows share cache lines -- sit on one of the eight chiplets: consecutive logical ids do.
@@ -371,7 +377,7 @@ __global__ __launch_bounds__(64 * NA, kFwdWaves<T>) void window_train_fwd(const 
     extern __shared__ __attribute__((aligned(16))) unsigned char lds[];
     constexpr size_t img = image_elems<T>(NA);
     T *Q = reinterpret_cast<T *>(lds), *K = Q + img, *V = K + img;
-    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, i = 16 * w + (lane & 15);
+    const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), i = 16 * w + (lane & 15);
     const int job = logical_block(), slab = job / heads, head = job - slab * heads;
     const int C = heads * D, stride = 3 * C;
     const long wstride = (long)N * stride;
@@ -413,7 +419,7 @@ __global__ __launch_bounds__(64 * NA, kBwdWaves) void window_train_bwd(const T *
     constexpr size_t img = image_elems<T>(NA);
     T *Q = reinterpret_cast<T *>(lds), *G = Q + img, *K = G + img, *V = K + img;
     T *X = K, *Y = X + Lds<T>::cross_bytes(NA) / sizeof(T);            // P and dS cross where K and V were
-    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, i = 16 * w + (lane & 15), j = 16 * w + token_of_row(lane & 15, spread_tile(w, NS));
+    const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), i = 16 * w + (lane & 15), j = 16 * w + token_of_row(lane & 15, spread_tile(w, NS));
     const int job = logical_block(), slab = job / heads, head = job - slab * heads;
     const int C = heads * D, stride = 3 * C;
     const long wstride = (long)N * stride;
@@ -555,7 +561,7 @@ int check_args(const void *qkv, const float *packed, size_t packed_floats, int d
 template <typename T, int NS, int NA = tiles_of(NS)>
 int fwd_launch(const void *qkv, const float *bias, const float *mask, float *packed, void *out, long windows, int nW, int heads, int N, float scale, hipStream_t st) {
     int *any = reinterpret_cast<int *>(packed + table_floats(heads, nW, N));
-    hipLaunchKernelGGL((window_tables<NA>), dim3((unsigned)(heads + nW)), dim3(256), 0, st, bias, mask, packed, any, heads, N);
+    hipLaunchKernelGGL((window_tables<NA>), dim3((unsigned)(heads + nW), NA), dim3(256), 0, st, bias, mask, packed, any, heads, N);
     const size_t lds = fwd_lds<T>(NA);
     const int ns = slabs_for(windows, heads, per_cu(lds, kFwdWaves<T>, NA));
     hipLaunchKernelGGL((window_train_fwd<T, NS>), dim3((unsigned)(ns * heads)), dim3(64 * NA), lds, st, static_cast<const T *>(qkv), packed, any, static_cast<T *>(out),
@@ -591,7 +597,7 @@ int sd_window_attn_train_supported(int tokens_per_window, int head_dim) { return
 
 size_t sd_window_attn_train_packed_floats(int heads, int mask_windows, int tokens_per_window) {
     if (heads <= 0 || mask_windows < 0 || tokens_per_window < 1 || tokens_per_window > 64) return 0;
-    return sd::table_floats(heads, mask_windows, tokens_per_window) + (size_t)mask_windows;
+    return sd::table_floats(heads, mask_windows, tokens_per_window) + (size_t)mask_windows * sd::tiles(tokens_per_window);
 }
 
 int sd_window_attn_train_fwd(const void *qkv, const float *bias, const float *mask, float *packed, size_t packed_floats, void *out, int dtype, long windows,
