@@ -7,6 +7,9 @@
 // A row is a pixel's classes (stride P: class planes [B, C, P]) or contiguous (P == 1).  Both forms read the logits once from memory and write
 // k entries; the sums of the rest are taken over the unchosen terms only -- total minus chosen would cancel exactly where a confident teacher
 // needs the digits -- and relative to the largest of them, so they neither overflow nor vanish.
+//
+// Memory bound where nothing else were: N e bytes.  Measured: [8, 150, 128, 128] fp32, k = 10: 34 us (2.3 TB/s; the rounds of the search in LDS and VALU).
+// 2048 rows of 65536 bf16, k = 64: 72 us (3.7 TB/s; the read alone with the group maxima 40).  One row of 32003 fp32: 7.5 us, a chain of latencies.
 #include <hip/hip_runtime.h>
 #include <math.h>
 
@@ -27,7 +30,7 @@ __device__ __forceinline__ float of_key(int k) { return __int_as_float(k ^ ((k >
 // ---- class planes -----------------------------------------------------------------------------------------------------------------------------
 // One thread per pixel: neighbouring lanes read neighbouring pixels of a class plane.  The list of the best K so far sits in registers, sorted;
 // a new element moves through it as a bubble: slot j becomes the median of (x, slot j - 1, slot j), so the sequence has no branch and no
-// dynamic index.  What falls out of the list feeds the rest's running sum.  k > 32: several passes of 32, each bounded by the last entry of
+// dynamic index.  For more classes than the columns below hold.  What falls out of the list feeds the rest's running sum.  k > 32: several passes of 32, each bounded by the last entry of
 // the one before (rare, and the map's second read comes from cache where it fits).
 template <typename T, int K>
 __global__ __launch_bounds__(256) void topk_planes(const T *__restrict__ x, T *__restrict__ values, int *__restrict__ index, float *__restrict__ rest,
@@ -85,7 +88,7 @@ __global__ __launch_bounds__(256) void topk_planes(const T *__restrict__ x, T *_
 // The same with the pixels' classes parked in LDS when they fit: the register list costs K steps per class; here the maxima of groups of eight classes sit in
 // registers, and each of the k rounds takes the largest of them and scans its group again -- NG + 8 steps per entry instead of K per class.  Two lanes
 // share a pixel, each with half of its classes in a column of its own, and exchange their best: 64 pixels per column pair leave one wave per SIMD at 150
-// classes, 32 leave two (45 -> 37 us at [8, 150, 128, 128]; four lanes per pixel: 46 us, each lane scans a group per entry).  A taken class is
+// classes, 32 leave two (45 -> 34 us at [8, 150, 128, 128]; four lanes per pixel: 46 us, each lane scans a group per entry; the register list 84).  A taken class is
 // overwritten by kNoKey, so the sum of the rest is one more pass over the columns with its maximum known.  The scans go up and compare strictly, and the
 // lower half wins a tie: the lowest class does.
 template <typename T, int NG>

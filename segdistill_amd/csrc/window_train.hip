@@ -19,6 +19,11 @@
 //   bf16 storage: v_mfma_f32_16x16x32_bf16 on the operands as stored.  P and dS enter their products as two bf16 terms (the
 //   value and what its rounding left): one term alone would put an error as large as the result's own rounding on every output.
 //   Softmax, dS and the bias gradient are fp32.  Operand columns come from the row images by transposed LDS reads (ds_read_b64_tr_b16).
+//
+// 2888 windows of 49 tokens, 3 heads, 361 masks:  fp32 tables 4.5 us, forward 61 (2.6 TB/s), backward 125 to 138 (2.1 to 2.3 TB/s; 60 % of the matrix
+// pipe: tiles of 16 make 64 x 64 of 49 x 49; without HBM traffic it takes 122, without products 77), join 5.  bf16: forward 24 (3.3 TB/s), backward 54
+// (2.6 TB/s; VALU, LDS and HBM each 40 % busy; without products 43).  Tiles of 32, two waves to a window: 75 + 145 and 26.5 + 66; raised wave priority
+// around the products and LDS reads pinned ahead of them: level.
 #include <math.h>
 
 #include <type_traits>

@@ -76,7 +76,7 @@ def test_window_attention_refusals(L):
     assert ok(1, 32) and ok(49, 32) and ok(64, 32) and not ok(0, 32) and not ok(65, 32) and not ok(49, 64)
     ws, pk = L.sd_window_attn_train_workspace_bytes(0, 6, 3, 49), L.sd_window_attn_train_packed_floats(3, 2, 49)
     assert ws > 0 and L.sd_window_attn_train_workspace_bytes(0, 6, 3, 65) == 0 and L.sd_window_attn_train_workspace_bytes(0, 0, 3, 49) == 0
-    assert L.sd_window_attn_train_workspace_bytes(2, 6, 3, 49) == 0 and pk == 5 * 4096 + 2 and L.sd_window_attn_train_packed_floats(3, -1, 49) == 0
+    assert L.sd_window_attn_train_workspace_bytes(2, 6, 3, 49) == 0 and pk == 5 * 4096 + 2 * 4 and L.sd_window_attn_train_packed_floats(3, -1, 49) == 0
 
     def fwd(q=P, b=P, m=NULL, k=P, kf=pk, o=P, dt=0, w=6, nw=0, h=3, n=49, d=32):
         return L.sd_window_attn_train_fwd(q, b, m, k, kf, o, dt, w, nw, h, n, d, 1.0, NULL)

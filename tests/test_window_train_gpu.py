@@ -74,6 +74,21 @@ def _with(x, heads, scale=32 ** -0.5):
 
 
 @pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize('n', range(1, 65))
+def test_every_window_size(n, dtype):
+    _check(*_with(_inputs(4, n, 2, dtype, 500 + n, 2), 2))
+
+
+@pytest.mark.parametrize('query', [0, 17, 48])
+def test_masks_that_say_something_to_one_query(query):
+    qkv, bias, _, dout = _inputs(6, 49, 2, torch.float32, query)
+    mask = torch.zeros(3, 49, 49, device='cuda')
+    mask[1, query, 5:40] = -math.inf
+    mask[2, query, 48] = 3.0
+    _check(qkv, bias, mask, 2, 32 ** -0.5, dout)
+
+
+@pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16])
 @pytest.mark.parametrize('n', [5, 49, 64])
 def test_masks_that_leave_nothing(n, dtype):
     """rows, then whole windows, at -inf: output 0, no gradient; a mask at the type's lowest value is a mask, not an empty row"""
