@@ -341,11 +341,14 @@ __device__ __forceinline__ RowEntries load_entries(const Entries &e, size_t row,
 
 __host__ __device__ inline int row_words(int C) { return (C + 7 + 31) / 32; }      // up to 7 bits of shift in front
 
-template <typename T, int NT>
-__global__ __launch_bounds__(NT == 64 ? 256 : NT) void topk_kl_rows_fwd(const T *__restrict__ S, Entries e, float4 *__restrict__ stats, double *__restrict__ part,
+// ONE: the grid holds every row, no workgroup takes a second one.  Without the loop the constants of the 64-bit logarithms are not kept in registers around it:
+// 64 instead of 103, twice the waves (2048 rows of 65536 bf16: 62 -> 54 us; the loop under a bound of 80 or 64 registers spills, 78 and 84 us).  Three vectors
+// in flight per lane: four spill at that bound (66 us) or leave six waves (58 us), two: 58 us.
+template <typename T, int NT, bool ONE>
+__global__ __launch_bounds__(NT == 64 ? 256 : NT, ONE && NT == 256 ? 8 : 1) void topk_kl_rows_fwd(const T *__restrict__ S, Entries e, float4 *__restrict__ stats, double *__restrict__ part,
                                                                         long rows, int C, float c2) {
     extern __shared__ __attribute__((aligned(16))) unsigned char lds[];
-    constexpr int G = NT == 64 ? 4 : 1, N = VecIO<T>::N, V = 4;
+    constexpr int G = NT == 64 ? 4 : 1, N = VecIO<T>::N, V = 3;
     __shared__ Online tmp[NT / 64 + 1];
     const int nwords = row_words(C);
     const int grp = NT == 64 ? threadIdx.x >> 6 : 0, tid = NT == 64 ? threadIdx.x & 63 : threadIdx.x;
@@ -353,9 +356,20 @@ __global__ __launch_bounds__(NT == 64 ? 256 : NT) void topk_kl_rows_fwd(const T 
     double kl = 0, counted = 0;
     for (int w = tid; w < nwords; w += NT) bits[w] = 0;
     for (long row = (long)blockIdx.x * G + grp; row < rows; row += (long)gridDim.x * G) {
-        if (e.valid && !e.valid[row]) continue;                       // the same answer in all threads of the group
+        if (e.valid && !e.valid[row]) {                               // the same answer in all threads of the group
+            if constexpr (ONE) break;
+            else continue;
+        }
         const T *z = S + (size_t)row * C;
         const int head = row_head(z, C), shift = (8 - (head & 7)) & 7, nvec = (C - head) / N;
+        const typename VecIO<T>::raw_t *vec = reinterpret_cast<const typename VecIO<T>::raw_t *>(z + head);
+        typename VecIO<T>::raw_t raw[V];
+        auto fetch = [&](int i) {
+#pragma unroll
+            for (int u = 0; u < V; ++u) raw[u] = __builtin_nontemporal_load(vec + i + u * NT);
+        };
+        int i = tid;
+        if (i + (V - 1) * NT < nvec) fetch(i);                         // on their way while the entries are taken
         const RowEntries x = load_entries(e, row, C, c2);
         group_sync<NT>();                                              // the mask is clear
         if (tid < 64) {
@@ -370,7 +384,8 @@ __global__ __launch_bounds__(NT == 64 ? 256 : NT) void topk_kl_rows_fwd(const T 
             const float one[1] = {VecIO<T>::load1(z + tid)};
             online_fold(low, one, c2);
         }
-        auto fold = [&](float (&a)[N], int i) {
+        // the elements of one vector that are in A leave as -inf
+        auto drop = [&](float *a, int i) {
             const int at = head + shift + i * N;
             const unsigned m = bits[at >> 5] >> (at & 31);
             if (m & ((1u << N) - 1)) {
@@ -378,25 +393,26 @@ __global__ __launch_bounds__(NT == 64 ? 256 : NT) void topk_kl_rows_fwd(const T 
                 for (int q = 0; q < N; ++q)
                     if ((m >> q) & 1) a[q] = -INFINITY;
             }
-            online_fold(low, a, c2);
         };
-        const typename VecIO<T>::raw_t *vec = reinterpret_cast<const typename VecIO<T>::raw_t *>(z + head);
-        int i = tid;
-        for (; i + (V - 1) * NT < nvec; i += V * NT) {                 // V vectors on their way at a time
-            typename VecIO<T>::raw_t raw[V];
-#pragma unroll
-            for (int u = 0; u < V; ++u) raw[u] = __builtin_nontemporal_load(vec + i + u * NT);
+        while (i + (V - 1) * NT < nvec) {                              // V vectors on their way at a time
+            float a[V * N];
 #pragma unroll
             for (int u = 0; u < V; ++u) {
-                float a[N];
-                unpack_vec<T>(raw[u], a);
-                fold(a, i + u * NT);
+                float v[N];
+                unpack_vec<T>(raw[u], v);
+                drop(v, i + u * NT);
+#pragma unroll
+                for (int q = 0; q < N; ++q) a[u * N + q] = v[q];
             }
+            i += V * NT;
+            if (i + (V - 1) * NT < nvec) fetch(i);
+            online_fold(low, a, c2);
         }
         for (; i < nvec; i += NT) {
             float a[N];
             VecIO<T>::load(z + head + (size_t)i * N, a);
-            fold(a, i);
+            drop(a, i);
+            online_fold(low, a, c2);
         }
         const int t = head + nvec * N + tid;
         if (t < C && outside(t)) {
@@ -430,9 +446,11 @@ __global__ __launch_bounds__(NT == 64 ? 256 : NT) void topk_kl_rows_fwd(const T 
             s += qr_num;
             const bool says = x.ts > 0.f || x.ts != x.ts;
             const float er = e.rest ? ex2((e.rest[row] - x.tr) * c2) : 0.f;
-            const double ts = weights + er, log_ratio = log(s) - log(ts), inv_t = 1.0 / ts, pr = er * inv_t;
-            double k = terms * inv_t + kl_term(weights * inv_t, log_ratio);
-            if (e.rest) k += kl_term(pr, (((double)e.rest[row] - (double)x.tr) - ((double)low.m - (double)r)) * ti - log((double)low.s) + log_ratio);
+            const double ts = weights + er, inv_t = 1.0 / ts, pr = er * inv_t;
+            // two logarithms by one instruction stream: the even lanes' is that of s / ts, the odd ones' that of s / (ts low.s)
+            const double lg = log((tid & 1 ? s / (double)low.s : s) * inv_t), lg_rest = __shfl_xor(lg, 1, 64);
+            double k = terms * inv_t + kl_term(weights * inv_t, lg);
+            if (e.rest) k += kl_term(pr, (((double)e.rest[row] - (double)x.tr) - ((double)low.m - (double)r)) * ti + lg_rest);
             if (tid == 0) {
                 const float w = low.s > 0.f || low.s != low.s ? (float)((qr_num / s - pr) / low.s) : 0.f;
                 stats[row] = says ? make_float4(finite_ref(low.m), w, r, (float)(1.0 / s)) : make_float4(0.f, 0.f, r, 0.f);
@@ -443,6 +461,7 @@ __global__ __launch_bounds__(NT == 64 ? 256 : NT) void topk_kl_rows_fwd(const T 
             for (int h = 0; h < 2; ++h)                                // every vector of this row has been read (online_group waits for all)
                 if (x.first[h]) bits[(x.c[h] + shift) >> 5] = 0;
         }
+        if constexpr (ONE) break;
     }
     write_partial<NT == 64 ? 256 : NT>(kl, counted, part);
 }
@@ -535,9 +554,14 @@ int fwd_launch(const void *S, const Entries &e, long B, int C, long P, const Pla
     const T *s = static_cast<const T *>(S);
     const dim3 grid((unsigned)pl.blocks);
     if (P == 1) {
-        if (pl.threads == 64) hipLaunchKernelGGL((topk_kl_rows_fwd<T, 64>), grid, dim3(256), pl.lds, st, s, e, stats, part, B, C, c2);
-        else if (pl.threads == 256) hipLaunchKernelGGL((topk_kl_rows_fwd<T, 256>), grid, dim3(256), pl.lds, st, s, e, stats, part, B, C, c2);
-        else hipLaunchKernelGGL((topk_kl_rows_fwd<T, 1024>), grid, dim3(1024), pl.lds, st, s, e, stats, part, B, C, c2);
+#define SD_ROWS(NT, ONE) hipLaunchKernelGGL((topk_kl_rows_fwd<T, NT, ONE>), grid, dim3(NT == 64 ? 256 : NT), pl.lds, st, s, e, stats, part, B, C, c2)
+        const bool one = pl.blocks == pl.per;
+        if (pl.threads == 64 && one) SD_ROWS(64, true);
+        else if (pl.threads == 64) SD_ROWS(64, false);
+        else if (pl.threads == 256 && one) SD_ROWS(256, true);
+        else if (pl.threads == 256) SD_ROWS(256, false);
+        else SD_ROWS(1024, true);                      // fewer than 1024 rows
+#undef SD_ROWS
     } else {
         hipLaunchKernelGGL((topk_kl_planes_fwd<T>), grid, dim3(BT * kWaves), pl.lds, st, s, e, stats, part, C, P, (int)pl.per, pl.nwords, c2);
     }

@@ -250,6 +250,16 @@ def test_criterion_and_gradient(shape, k, tau, alpha, drop, with_rest, dtype):
     _check_kl(S, v, i, r if with_rest else None, tau, alpha, valid)
 
 
+@pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize('shape', [(16384, 30), (16501, 30), (4096, 2052), (4111, 2052), (1023, 2052)])
+def test_more_rows_than_the_grid_holds(shape, dtype):
+    """four short rows per workgroup, one long one; 4096 workgroups"""
+    g = torch.Generator(device='cuda').manual_seed(shape[0])
+    S = (torch.randn(shape, device='cuda', generator=g) * 2).to(dtype)
+    v, i, r = _teacher(S, 6, 1.0, g, dtype)
+    _check_kl(S, v, i, r, 1.0, 1.0, torch.rand(shape[0], device='cuda', generator=g) >= 0.3)
+
+
 @pytest.mark.parametrize('shape', [(9, 40), (4, 3001), (2, 40, 3, 5)])
 @pytest.mark.parametrize('with_rest', [True, False])
 def test_entries_absent_doubled_and_without_weight(shape, with_rest):
