@@ -9,8 +9,8 @@
 //
 // Each row keeps (m_r, w, m, 1/s): its gradient is w 2^{(z_c - m_r) c2} outside A, with w = (q_r - p_r) / s_r.
 // Memory bound: the forward reads z, the backward reads z and writes dz; nothing of the size of z is kept between them.
-// Measured: [8, 150, 128, 128] fp32, k = 10: forward 29 us (2.7 TB/s), backward 40 us (4.0 TB/s); 2048 rows of 65536 bf16, k = 64: forward 62 us
-// (4.3 TB/s), backward 98 us (5.5 TB/s); the join of the row losses 4 us.
+// Measured: [8, 150, 128, 128] fp32, k = 10: forward 29 us (2.7 TB/s), backward 40 us (4.0 TB/s); 2048 rows of 65536 bf16, k = 64: forward 55 us
+// (4.9 TB/s), backward 98 us (5.5 TB/s); the join of the row losses 4 us.
 #include <hip/hip_runtime.h>
 #include <math.h>
 
