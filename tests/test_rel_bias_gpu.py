@@ -122,3 +122,22 @@ def test_the_plan_may_move_between_forward_and_backward():
     assert torch.equal(torch.autograd.grad(out, table, torch.ones_like(out), retain_graph=True)[0], want)
     with pytest.raises(RuntimeError, match='second derivative'):
         torch.autograd.grad(out, table, torch.ones_like(out), create_graph=True)
+
+
+def test_offsets_past_32_bits():
+    """a bias of 2.2e9 elements: every head against a call on that head alone"""
+    from segdistill_amd import rel_bias
+    n, heads = 8192, 33
+    d = (torch.arange(n, device='cuda').unsqueeze(1) - torch.arange(n, device='cuda')).abs()
+    plan = rel_bias.BucketPlan(torch.minimum(d, torch.full_like(d, 31)), 32)
+    g = torch.Generator(device='cuda').manual_seed(4)
+    table = torch.randn(32, heads, device='cuda', generator=g).to(torch.bfloat16).requires_grad_()
+    grad = torch.empty(heads, n, n, device='cuda', dtype=torch.bfloat16).normal_(generator=g)
+    assert grad.numel() > 2 ** 31
+    out = rel_bias.bucket_bias(table, plan)
+    dtable = torch.autograd.grad(out, table, grad)[0]
+    for h in (0, 31, 32):
+        t = table.detach()[:, h:h + 1].contiguous().requires_grad_()
+        one = rel_bias.bucket_bias(t, plan)
+        assert torch.equal(one[0], out[h]) and torch.equal(one[0, 5], t.detach()[plan.index[5].long(), 0])
+        assert torch.equal(torch.autograd.grad(one, t, grad[h:h + 1])[0][:, 0], dtable[:, h])

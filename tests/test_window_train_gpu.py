@@ -199,3 +199,20 @@ def test_refusals():
             call(**kw)
     with pytest.raises(TypeError):
         call(q=qkv.half())
+
+
+def test_offsets_past_32_bits():
+    """qkv of 2.3e9 elements: the last windows against a call on them alone (their operands are the same, and so is every operation)"""
+    from segdistill_amd import window_attn
+    windows, n, heads = 160000, 49, 3
+    g = torch.Generator(device='cuda').manual_seed(9)
+    qkv = torch.empty(windows, n, 3 * heads * 32, device='cuda', dtype=torch.bfloat16).normal_(generator=g).requires_grad_()
+    dout = torch.empty(windows, n, heads * 32, device='cuda', dtype=torch.bfloat16).normal_(generator=g)
+    bias = torch.randn(heads, n, n, device='cuda', generator=g)
+    assert qkv.numel() > 2 ** 31
+    out = window_attn.attention(qkv, bias, None, heads, 32 ** -0.5)
+    dqkv = torch.autograd.grad(out, qkv, dout)[0]
+    for at in (slice(0, 5), slice(windows - 7, windows)):
+        q = qkv.detach()[at].clone().requires_grad_()
+        o = window_attn.attention(q, bias, None, heads, 32 ** -0.5)
+        assert torch.equal(o, out[at]) and torch.equal(torch.autograd.grad(o, q, dout[at])[0], dqkv[at])
