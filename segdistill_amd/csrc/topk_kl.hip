@@ -521,27 +521,33 @@ __global__ __launch_bounds__(NT == 64 ? 256 : NT) void topk_kl_rows_bwd(const T 
 
 // ---- launches ---------------------------------------------------------------------------------------------------------------------------------
 struct Plan {
-    int threads, blocks, nwords, lds;      // threads per row (P == 1) or per workgroup (planes: one per pixel)
-    long per;                              // workgroups per image (planes)
+    int fwd, bwd, blocks, nwords, lds;     // threads per row of the two passes (P == 1); the forward's workgroups
+    long per;                              // workgroups that one pass over the rows needs: the forward's (P == 1), an image's (planes)
 };
 // false: not a shape these kernels launch
-bool plan(long B, int C, long P, int k, Plan *pl) {
+bool plan(long B, int C, long P, int k, int element_bytes, Plan *pl) {
     if (P == 1) {
         pl->nwords = row_words(C);
-        // a wave per short row; a long one by four waves, or by sixteen where there are too few rows to fill the 256 CUs with fours
-        pl->threads = C <= 2048 ? 64 : B >= 1024 ? 256 : 1024;
-        const long wgs = pl->threads == 64 ? (B + 3) / 4 : B;
-        if (wgs > kMaxBlocks) return false;
+        // Forward: a wave per row costs least where rows are short or many (16384 rows of 2048 fp32: 41 us, by four waves 74; of 8192: 93 against 115; 2048 of
+        // 8192: 19 and 21), four waves per row are faster where they are not (1024 rows of 8192: 15, one wave 17; 1024 of 32768: 27 against 40), sixteen only for
+        // few and very long ones (256 rows of 83419: 23 against 30; 512: 41 against 36; 256 of 32768: 14 both).
+        // Backward, one pass without a reduction: a wave per short row (16384 rows of 1025 fp32: 40 and 44 us, bf16 29 and 42; of 4096 fp32: 105 against 93),
+        // sixteen for long rows that are few (512 rows of 16384 fp32: 18 against 23; 256 of 83419: 36 against 71; 1024 of 16384: 30 both) or very long (4096 of
+        // 83419: 589 against 658; 2048 of 65536 bf16: 104 against 98; 4096 of 8192: 58 against 48).
+        const long bytes = (long)C * element_bytes;
+        pl->fwd = C <= 2048 || (bytes <= 32768 && B >= 2048) ? 64 : B <= 256 && bytes > 131072 ? 1024 : 256;
+        pl->bwd = C <= 2048 ? 64 : bytes >= 16384 && (B < 1024 || bytes > 131072) ? 1024 : 256;
+        const long wgs = pl->fwd == 64 ? (B + 3) / 4 : B;
+        if ((pl->bwd == 64 ? wgs : B) > kMaxBlocks) return false;
         // (16384 rows of 4000 fp32: 97 us, with at most 4096 workgroups, each with a loop, 121)
         pl->blocks = (int)(wgs < 16384 ? wgs : 16384);
-        pl->lds = pl->nwords * 4 * (pl->threads == 64 ? 4 : 1);
+        pl->lds = pl->nwords * 4 * (pl->fwd == 64 ? 4 : 1);
         pl->per = wgs;
         return true;
     }
     pl->nwords = (C + 31) / 32;
     const long column = 4L * (2 * pl->nwords + k + 1);                  // bytes of LDS per pixel
     if (column * BT > 62464) return false;                              // 64 KB less what the kernels hold besides
-    pl->threads = BT;
     pl->lds = (int)column * BT;
     pl->per = (P + BT - 1) / BT;
     if (pl->per > kMaxBlocks / B) return false;
@@ -557,11 +563,11 @@ int fwd_launch(const void *S, const Entries &e, long B, int C, long P, const Pla
     if (P == 1) {
 #define SD_ROWS(NT, ONE) hipLaunchKernelGGL((topk_kl_rows_fwd<T, NT, ONE>), grid, dim3(NT == 64 ? 256 : NT), pl.lds, st, s, e, stats, part, B, C, c2)
         const bool one = pl.blocks == pl.per;
-        if (pl.threads == 64 && one) SD_ROWS(64, true);
-        else if (pl.threads == 64) SD_ROWS(64, false);
-        else if (pl.threads == 256 && one) SD_ROWS(256, true);
-        else if (pl.threads == 256) SD_ROWS(256, false);
-        else SD_ROWS(1024, true);                      // fewer than 1024 rows
+        if (pl.fwd == 64 && one) SD_ROWS(64, true);
+        else if (pl.fwd == 64) SD_ROWS(64, false);
+        else if (pl.fwd == 256 && one) SD_ROWS(256, true);
+        else if (pl.fwd == 256) SD_ROWS(256, false);
+        else SD_ROWS(1024, true);                      // at most 256 rows
 #undef SD_ROWS
     } else {
         hipLaunchKernelGGL((topk_kl_planes_fwd<T>), grid, dim3(BT * kWaves), pl.lds, st, s, e, stats, part, C, P, (int)pl.per, pl.nwords, c2);
@@ -576,9 +582,9 @@ int bwd_launch(const void *S, const Entries &e, long B, int C, long P, const Pla
     const T *s = static_cast<const T *>(S);
     T *d = static_cast<T *>(dS);
     if (P == 1) {
-        const dim3 grid((unsigned)pl.per);
-        if (pl.threads == 64) hipLaunchKernelGGL((topk_kl_rows_bwd<T, 64>), grid, dim3(256), 0, st, s, e, stats, inv_n, upstream, d, B, C, c2, coef);
-        else if (pl.threads == 256) hipLaunchKernelGGL((topk_kl_rows_bwd<T, 256>), grid, dim3(256), 0, st, s, e, stats, inv_n, upstream, d, B, C, c2, coef);
+        const dim3 grid((unsigned)(pl.bwd == 64 ? (B + 3) / 4 : B));
+        if (pl.bwd == 64) hipLaunchKernelGGL((topk_kl_rows_bwd<T, 64>), grid, dim3(256), 0, st, s, e, stats, inv_n, upstream, d, B, C, c2, coef);
+        else if (pl.bwd == 256) hipLaunchKernelGGL((topk_kl_rows_bwd<T, 256>), grid, dim3(256), 0, st, s, e, stats, inv_n, upstream, d, B, C, c2, coef);
         else hipLaunchKernelGGL((topk_kl_rows_bwd<T, 1024>), grid, dim3(1024), 0, st, s, e, stats, inv_n, upstream, d, B, C, c2, coef);
     } else {
         const dim3 grid((unsigned)pl.blocks);
@@ -592,7 +598,7 @@ int check_args(const void *S, const void *values, const int32_t *index, const fl
     if (!S || !values || !index) return SD_E_NULL;
     if ((dtype != SD_F32 && dtype != SD_BF16) || (values_dtype != SD_F32 && values_dtype != SD_BF16)) return SD_E_DTYPE;
     if (B <= 0 || C <= 0 || P <= 0 || k <= 0 || B > 0x7fffffffL || P > 0x7fffffffL || !(tau >= kTauMin && tau <= kTauMax)) return SD_E_SHAPE;
-    if (k > kTopkMax || C > kTopkMaxClasses || !plan(B, C, P, k, pl)) return SD_E_UNSUPPORTED;
+    if (k > kTopkMax || C > kTopkMaxClasses || !plan(B, C, P, k, dtype == SD_F32 ? 4 : 2, pl)) return SD_E_UNSUPPORTED;
     const uintptr_t es = dtype == SD_F32 ? 3 : 1, ev = values_dtype == SD_F32 ? 3 : 1;
     if ((reinterpret_cast<uintptr_t>(S) & es) || (reinterpret_cast<uintptr_t>(values) & ev) ||
         ((reinterpret_cast<uintptr_t>(index) | reinterpret_cast<uintptr_t>(rest)) & 3))
@@ -607,12 +613,13 @@ extern "C" {
 
 int sd_topk_kl_supported(long B, int C, long P, int k) {
     sd::Plan pl;
-    return B > 0 && C > 0 && P > 0 && k > 0 && B <= 0x7fffffffL && P <= 0x7fffffffL && k <= sd::kTopkMax && C <= sd::kTopkMaxClasses && sd::plan(B, C, P, k, &pl);
+    return B > 0 && C > 0 && P > 0 && k > 0 && B <= 0x7fffffffL && P <= 0x7fffffffL && k <= sd::kTopkMax && C <= sd::kTopkMaxClasses && sd::plan(B, C, P, k, 4, &pl);
 }
 
 size_t sd_topk_kl_workspace_bytes(long B, int C, long P, int k) {
-    sd::Plan pl;
-    return sd_topk_kl_supported(B, C, P, k) && sd::plan(B, C, P, k, &pl) ? 2 * sizeof(double) * (size_t)pl.blocks : 0;
+    sd::Plan f32, bf16;                    // for logits of either type
+    if (!sd_topk_kl_supported(B, C, P, k) || !sd::plan(B, C, P, k, 4, &f32) || !sd::plan(B, C, P, k, 2, &bf16)) return 0;
+    return 2 * sizeof(double) * (size_t)(f32.blocks > bf16.blocks ? f32.blocks : bf16.blocks);
 }
 
 int sd_topk_kl_fwd(const void *S, const void *values, const int32_t *index, const float *rest, const uint8_t *valid, int dtype, int values_dtype, long B, int C,

@@ -251,9 +251,9 @@ def test_criterion_and_gradient(shape, k, tau, alpha, drop, with_rest, dtype):
 
 
 @pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16])
-@pytest.mark.parametrize('shape', [(16384, 30), (65536, 12), (66001, 12), (4111, 2052), (16411, 2052), (1023, 2052)])
-def test_more_rows_than_the_grid_holds(shape, dtype):
-    """four short rows per workgroup, one long one; 16384 workgroups"""
+@pytest.mark.parametrize('shape', [(16384, 30), (65536, 12), (66001, 12), (2047, 2052), (2049, 2052), (16411, 2052), (2050, 8193), (1023, 8200), (256, 33001), (257, 33001), (255, 66001), (1025, 33001)])
+def test_waves_per_row_and_rows_per_workgroup(shape, dtype):
+    """either side of the sizes where a row goes to more waves, or a workgroup to a second row"""
     g = torch.Generator(device='cuda').manual_seed(shape[0])
     S = (torch.randn(shape, device='cuda', generator=g) * 2).to(dtype)
     v, i, r = _teacher(S, 6, 1.0, g, dtype)
