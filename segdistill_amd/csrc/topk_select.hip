@@ -433,7 +433,8 @@ __global__ __launch_bounds__(NT == 64 ? 256 : NT, WAVES) void topk_rows(const T 
     } else {
         row.stream(tid, take);
     }
-    if (sum != sum) sh.odd = 1;                   // also where bound * c2 leaves the range
+    // NaN, or +inf: bound * c2 is below the range (every term of the sum is at most 1 otherwise)
+    if (!(sum <= FLT_MAX)) sh.odd = 1;
 #pragma unroll
     for (int d = 32; d > 0; d >>= 1) sum += __shfl_xor(sum, d, 64);
     if ((tid & 63) == 0) sh.sum[tid >> 6] = sum;

@@ -131,6 +131,23 @@ def test_infinities_and_nan_that_are_left_over(shape, count, dtype):
     assert v.isnan().all() and bool(rest.isnan().all()) == (count > k)
 
 
+@pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize('V', [40, 700, 2049, 5003, 30001, 40000, 140001])
+@pytest.mark.parametrize('kind', ['tiny tau', 'huge logits', 'huge positive logits'])
+def test_rest_where_a_logit_over_tau_leaves_fp32(V, kind, dtype):
+    """logits whose quotient by tau is beyond 2^128: 2^((x - bound) / tau) is 0 or 1 all the same, and the rest is the largest logit left over"""
+    g = torch.Generator(device='cuda').manual_seed(V)
+    rand = torch.rand(3, V, device='cuda', generator=g)
+    if kind == 'tiny tau':
+        tau, x = 1e-37, -30.0 - torch.floor(rand * 60) / 4                          # levels of a quarter, each many times over in a long row
+    else:
+        tau, x = 1.0, torch.where(rand < 24 / V, -2.5e38, -3e38)
+        if kind == 'huge positive logits':
+            x = -x
+    for k in (1, 7, 30):
+        _check_select(x.to(dtype), k, tau)
+
+
 def test_more_rows_than_one_launch_holds():
     from segdistill_amd import ops
     rows = 4 * 0xffffff + 37                                                         # four rows per workgroup, 2^24 - 1 workgroups
