@@ -103,9 +103,14 @@ class WindowAttention(nn.Module):
 
     @staticmethod
     def _plan_of_loaded_index(self, _keys):
-        """a checkpoint brings its own relative_position_index, and the only one to a module that was built on the meta device"""
-        if not self.relative_position_index.is_meta:
-            self.bias_plan = rel_bias.BucketPlan(self.relative_position_index, self.relative_position_bias_table.shape[0])
+        """a checkpoint brings its own relative_position_index, and the only one to a module that was built on the meta device.  The plan is written in place,
+        as the index is: a captured step has its addresses.  One that cannot be (an index whose buckets are cut otherwise) is replaced and stays alive."""
+        index, plan = self.relative_position_index, self.bias_plan
+        if index.is_meta or (plan is not None and plan.update(index)):
+            return
+        if plan is not None:
+            self.__dict__.setdefault('_former_plans', []).append(plan)
+        self.bias_plan = rel_bias.BucketPlan(index, self.relative_position_bias_table.shape[0])
 
     def _bias_packed(self, n, h):
         """relative position bias [h, N, N] in the attention kernel's accumulator layout (padded keys = -inf); cached for a frozen table."""
@@ -179,6 +184,11 @@ class WindowAttention(nn.Module):
         drop = self.attn_drop.p if self.training else 0.
         out = F.scaled_dot_product_attention(q, k, v, attn_mask=add, dropout_p=drop, scale=self.scale)
         return self.proj_drop(self.proj(out.transpose(1, 2).reshape(bw, n, c)))
+
+
+def bias_plans(model):
+    """the bucket plans that `model`'s window attentions read now (a captured step holds the addresses of those it was captured with)"""
+    return [m.bias_plan for m in model.modules() if isinstance(m, WindowAttention)]
 
 
 class SwinTransformerBlock(nn.Module):

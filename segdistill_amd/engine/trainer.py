@@ -8,6 +8,7 @@ import contextlib
 import torch
 
 from .. import deferred
+from ..backbones.swin import bias_plans
 from . import segments
 from .dp import DataParallelReducer
 from .optim import PolyLR, build_optimizer, sync_derived_weights
@@ -395,6 +396,7 @@ class KDTrainer:
     def load_state_dict(self, sd):
         m = self.model
         weights = sd['state_dict'] if 'state_dict' in sd else sd.get('student', sd.get('model'))   # 'student' / 'model': round-1 files
+        plans = bias_plans(m)
         if hasattr(m, 'student'):
             m.student.load_state_dict(weights)
             m.distillation_loss.load_state_dict(sd.get('distillation_loss', {}), strict=False)
@@ -402,10 +404,19 @@ class KDTrainer:
             m.load_state_dict(weights)
         self.optimizer.load_state_dict(sd['optimizer'])
         self._sync_derived_weights()
+        if bias_plans(m) != plans and self._captured():
+            import warnings
+            warnings.warn('the loaded relative_position_index cuts its buckets otherwise: the captured step reads the former one; continuing in eager mode')
+            self.disable_graph()
         meta = sd.get('meta', sd)
         self.iter = int(meta['iter'])
         if hasattr(m, 'cnt'):
             m.cnt = int(meta['cnt'])
+
+    def _captured(self):
+        m = self.model
+        return (getattr(self, '_graph', None) is not None or getattr(m, '_graphed_teacher', None) is not None
+                or getattr(getattr(m, 'student', None), '_graphed_backbone', None) is not None)
 
     def _sync_derived_weights(self):
         """Copies of the weights that kernels read instead of the fp32 parameter are rewritten IN PLACE now (engine/optim.py::

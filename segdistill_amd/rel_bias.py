@@ -15,7 +15,8 @@ CHUNK = 512          # sd_bucket_bias_chunk(): the pairs of one bucket that one 
 
 class BucketPlan(nn.Module):
     """The (query, key) pairs of `index` [Nq, Nk] (integers in [0, num_buckets)) in the order the gradient sums them.  Built once per index: it reads the
-    index on the host.  A module without parameters or state-dict entries, so that a model that holds one moves it along."""
+    index on the host.  A module without parameters or state-dict entries, so that a model that holds one moves it along.  A captured graph reads the plan's
+    memory: `update` gives it another index, and the plan has to live as long as the graph."""
 
     def __init__(self, index, num_buckets):
         super().__init__()
@@ -24,6 +25,10 @@ class BucketPlan(nn.Module):
         nb = int(num_buckets)
         if index.numel() > 2 ** 31 - 1:
             raise ValueError('BucketPlan: more than 2^31 - 1 pairs')
+        with torch.inference_mode(False):                                    # buffers that a backward may keep, wherever the plan is built
+            self._order(index, nb)
+
+    def _order(self, index, nb):
         flat = index.detach().reshape(-1).long()
         lo, hi = torch.stack(torch.aminmax(flat)).tolist()
         if lo < 0 or hi >= nb:
@@ -44,6 +49,17 @@ class BucketPlan(nn.Module):
         first_pair = order[start.clamp(max=flat.numel() - 1)]
         self.register_buffer('chunk_order', torch.sort(first_pair, stable=True).indices.int(), persistent=False)
 
+    def update(self, index):
+        """Take another index of the same shape and number of buckets, written where the old one is: a captured graph that reads this plan reads the new
+        one.  False, and nothing written, if the new index needs another number of chunks or lies on another device (then: a new plan)."""
+        new = BucketPlan(index, self.num_buckets)
+        if new.shape != self.shape or new.num_chunks != self.num_chunks or new.index.device != self.index.device:
+            return False
+        with torch.no_grad():
+            for name, b in self.named_buffers():
+                b.copy_(getattr(new, name))
+        return True
+
     def extra_repr(self):
         return f'{self.shape[0]} x {self.shape[1]} pairs in {self.num_buckets} buckets'
 
@@ -56,14 +72,15 @@ class _BucketBiasFunction(torch.autograd.Function):
         rc = _launch(table.device, _lib.lib().sd_bucket_bias_fwd, table.data_ptr(), plan._buffers['index'].data_ptr(), out.data_ptr(), _DT[table.dtype], nb, heads,
                      plan.num_pairs)
         _lib.check(rc, 'sd_bucket_bias_fwd')
-        ctx.plan, ctx.held = plan, tuple(plan._buffers[n] for n in ('order', 'chunk_start', 'chunk_order', 'bucket_chunk'))      # (the plan may move meanwhile)
+        ctx.plan = plan
+        ctx.save_for_backward(*(plan._buffers[n] for n in ('order', 'chunk_start', 'chunk_order', 'bucket_chunk')))      # (the plan may move meanwhile, or be updated: an error)
         return out
 
     @staticmethod
     def backward(ctx, grad_out):
         _no_double_backward('bucket_bias')
         plan = ctx.plan
-        order, start, by_pair, bucket = ctx.held
+        order, start, by_pair, bucket = ctx.saved_tensors
         nb, chunks = plan.num_buckets, plan.num_chunks
         d = grad_out.contiguous()
         heads = d.shape[0]

@@ -160,3 +160,57 @@ def test_kd_step_of_a_swin_student_against_top_logits_eager_and_replayed():
                 assert vg[k] == pytest.approx(ve[k], abs=3e-4 * max(1.0, abs(ve[k]))), (it, k)
     tables = [b.attn.relative_position_bias_table for l in ref.student.backbone.layers for b in l.blocks]
     assert all(p.grad is not None and float(p.grad.abs().sum()) > 0 for p in tables)
+
+
+def test_a_captured_step_reads_the_index_that_was_loaded_after_its_capture():
+    """the capture has the plan's addresses: a checkpoint (with another index, and bias tables large enough to show it) loaded into a replaying trainer and an
+    eager one, then equal losses and table gradients"""
+    from segdistill_amd.engine import KDTrainer, SyntheticADE
+    opt, sched = dict(type='AdamW', lr=6e-5, betas=(0.9, 0.999), weight_decay=0.01), dict(policy='poly', power=1.0, min_lr=0.0, by_epoch=False)
+    ref = _model()
+    gra = copy.deepcopy(ref)
+    te, tg = KDTrainer(ref, opt, sched), KDTrainer(gra, opt, sched)
+    de, dg = (SyntheticADE(2, size=(112, 120), num_classes=19, device='cuda:0', pool=3, seed=1) for _ in range(2))
+    assert tg.enable_graph(dict(img=dg._pool[0][0], img_metas=None, gt_semantic_seg=dg._pool[0][1])), getattr(tg, 'graph_error', None)
+    graph = tg._graph
+
+    def steps(n):
+        for _ in range(n):
+            te.step(de.next())
+            torch.cuda.synchronize()
+            tg.step(dg.next())
+            ve, vg = te.log_values(), tg.log_values()
+            for k in ve:
+                if 'acc' not in k:
+                    assert vg[k] == pytest.approx(ve[k], abs=3e-4 * max(1.0, abs(ve[k]))), k
+    steps(2)
+    sd = te.state_dict()
+    sd['state_dict'] = {k: v.clone() for k, v in sd['state_dict'].items()}
+    torch.manual_seed(4)
+    for k, v in sd['state_dict'].items():
+        if k.endswith('relative_position_bias_table'):
+            v.normal_(std=3.0)
+    plain = copy.deepcopy(sd)
+    for k, v in sd['state_dict'].items():
+        if k.endswith('relative_position_index'):
+            sd['state_dict'][k] = v.flip(0)
+    for state in (plain, sd):
+        te.load_state_dict(copy.deepcopy(state)), tg.load_state_dict(copy.deepcopy(state))
+        junk = [torch.full((n,), -1, dtype=torch.int32, device='cuda') for n in (49, 169, 170, 2401) * 40]          # over whatever a load may have freed
+        assert tg._graph is graph
+        steps(2)
+        del junk
+    # a stale index would give unrelated gradients of the tables (a relative difference of 1 and more); two trainers differ by the order of the sums in library
+    # kernels and by what two optimizer steps of 6e-5 make of it
+    for m in (ref, gra):
+        for blk in (b for l in m.student.backbone.layers for b in l.blocks):
+            assert torch.equal(blk.attn.bias_plan.index.long(), blk.attn.relative_position_index)
+            assert torch.equal(blk.attn.relative_position_index[0], blk.attn.relative_position_index.new_tensor(_first_row_flipped()))
+    tables = [[b.attn.relative_position_bias_table for l in m.student.backbone.layers for b in l.blocks] for m in (ref, gra)]
+    for a, b in zip(*tables):
+        assert float((a.grad - b.grad).norm()) <= 2e-2 * float(a.grad.norm()) and float(a.grad.norm()) > 0
+
+
+def _first_row_flipped():
+    """the last token's row of a 7 x 7 window's index: (dy + 6) * 13 + dx + 6 from (6, 6)"""
+    return [(6 - y + 6) * 13 + 6 - x + 6 for y in range(7) for x in range(7)]
