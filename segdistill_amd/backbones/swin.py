@@ -91,9 +91,7 @@ class WindowAttention(nn.Module):
         rel = (coords[:, :, None] - coords[:, None, :]).permute(1, 2, 0)   # [N, N, 2]
         index = (rel[..., 0] + wh - 1) * (2 * ww - 1) + (rel[..., 1] + ww - 1)
         self.register_buffer('relative_position_index', index)
-        self.bias_plan = None
-        self._plan_of_loaded_index(self, None)
-        self.register_load_state_dict_post_hook(WindowAttention._plan_of_loaded_index)
+        self.register_load_state_dict_post_hook(WindowAttention._update_plan)
         self.qkv = nn.Linear(dim, dim * 3, bias=qkv_bias)
         self.attn_drop = nn.Dropout(attn_drop)
         self.proj = nn.Linear(dim, dim)
@@ -101,16 +99,35 @@ class WindowAttention(nn.Module):
         trunc_normal_(self.relative_position_bias_table, std=.02)
         self.softmax = nn.Softmax(dim=-1)
 
+    # The plan by which the trainable table is gathered and its gradient summed (a frozen block needs none): built from relative_position_index when it is first
+    # asked for, held beside the tensor and the version it was built from.  A buffer that was changed or replaced since -- by a load, a copy, an assignment --
+    # is compared and, if it says something else, planned anew.  A buffer changed in place has its plan changed in place: a captured step has the addresses of
+    # both.  A plan that cannot be (its buckets are cut into another number of chunks) is replaced and stays alive.
+    @property
+    def bias_plan(self):
+        """the rel_bias.BucketPlan of relative_position_index as it is now; None where it cannot be read: on the meta device, or changed and being captured"""
+        index, held = self.relative_position_index, self.__dict__.get('_plan')
+        version = None if index.is_inference() else index._version
+        if held is not None and held[1] is index and held[2] == version is not None:
+            return held[0]
+        if index.is_meta or (index.is_cuda and torch.cuda.is_current_stream_capturing()):
+            return None
+        plan = held[0] if held is not None and held[0].index.device == index.device and held[0].shape == tuple(index.shape) else None
+        if plan is None or not bool((plan.index == index).all()):
+            if plan is None or held[1] is not index or not plan.update(index):
+                if plan is not None and held[1] is index:
+                    self.__dict__.setdefault('_former_plans', []).append(plan)
+                plan = rel_bias.BucketPlan(index, self.relative_position_bias_table.shape[0])
+            if index.is_cuda:
+                torch.cuda.current_stream(index.device).synchronize()          # whichever stream asks next
+        self.__dict__['_plan'] = (plan, index, version)
+        return plan
+
     @staticmethod
-    def _plan_of_loaded_index(self, _keys):
-        """a checkpoint brings its own relative_position_index, and the only one to a module that was built on the meta device.  The plan is written in place,
-        as the index is: a captured step has its addresses.  One that cannot be (an index whose buckets are cut otherwise) is replaced and stays alive."""
-        index, plan = self.relative_position_index, self.bias_plan
-        if index.is_meta or (plan is not None and plan.update(index)):
-            return
-        if plan is not None:
-            self.__dict__.setdefault('_former_plans', []).append(plan)
-        self.bias_plan = rel_bias.BucketPlan(index, self.relative_position_bias_table.shape[0])
+    def _update_plan(self, _keys):
+        """a checkpoint brought its own index: a captured step that reads the plan does not come by here again"""
+        if '_plan' in self.__dict__:
+            self.bias_plan
 
     def _bias_packed(self, n, h):
         """relative position bias [h, N, N] in the attention kernel's accumulator layout (padded keys = -inf); cached for a frozen table."""
@@ -124,6 +141,14 @@ class WindowAttention(nn.Module):
         if not tbl.requires_grad and not (tbl.is_cuda and torch.cuda.is_current_stream_capturing()):
             object.__setattr__(self, '_bias_p_cache', (sig, bp))
         return bp
+
+    def _bias(self, n, h):
+        """relative position bias [h, N, N]: where a graph may be built by the bucket plan"""
+        tbl = self.relative_position_bias_table
+        plan = self.bias_plan if (tbl.requires_grad or torch.is_grad_enabled()) and rel_bias.supported(tbl) else None
+        if plan is None:
+            return tbl[self.relative_position_index.view(-1)].view(n, n, h).permute(2, 0, 1)
+        return rel_bias.bucket_bias(tbl, plan)
 
     def _mask_packed(self, mask):
         if mask is None:
@@ -153,14 +178,10 @@ class WindowAttention(nn.Module):
         if (torch.is_grad_enabled() and (qkv.requires_grad or tbl.requires_grad) and not (self.training and self.attn_drop.p > 0)
                 and window_attn.train_supported(qkv, n, c // h) and rel_bias.supported(tbl) and (mask is None or bw % mask.shape[0] == 0)):
             # a graph to build (a Swin student): the same product with its gradients, one kernel each way (csrc/window_train.hip)
-            return self.proj_drop(self.proj(window_attn.attention(qkv, rel_bias.bucket_bias(tbl, self.bias_plan), mask, h, self.scale)))
+            return self.proj_drop(self.proj(window_attn.attention(qkv, self._bias(n, h), mask, h, self.scale)))
         q, k, v = qkv.reshape(bw, n, 3, h, c // h).permute(2, 0, 3, 1, 4)
         def additive():
-            if tbl.requires_grad and rel_bias.supported(tbl):
-                bias = rel_bias.bucket_bias(tbl, self.bias_plan)                                        # [h,N,N]
-            else:
-                bias = tbl[self.relative_position_index.view(-1)].view(n, n, h).permute(2, 0, 1)
-            add = bias.unsqueeze(0)
+            add = self._bias(n, h).unsqueeze(0)
             if mask is not None:
                 nw = mask.shape[0]
                 add = (add + mask.unsqueeze(1)).repeat(bw // nw, 1, 1, 1)  # windows of one image are contiguous
@@ -187,8 +208,8 @@ class WindowAttention(nn.Module):
 
 
 def bias_plans(model):
-    """the bucket plans that `model`'s window attentions read now (a captured step holds the addresses of those it was captured with)"""
-    return [m.bias_plan for m in model.modules() if isinstance(m, WindowAttention)]
+    """the bucket plans that `model`'s window attentions have built (a captured step holds the addresses of those it was captured with)"""
+    return [m.__dict__['_plan'][0] for m in model.modules() if isinstance(m, WindowAttention) and '_plan' in m.__dict__]
 
 
 class SwinTransformerBlock(nn.Module):

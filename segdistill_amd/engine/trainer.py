@@ -268,7 +268,8 @@ class KDTrainer:
     def _restore_buffers(self, saved):
         with torch.no_grad():
             for b, b0 in zip(self._trainable_net().buffers(), saved):
-                b.copy_(b0)
+                if not torch.equal(b, b0):      # (a constant one stays untouched, and what was derived from it stays valid)
+                    b.copy_(b0)
 
     def _autocast(self, cache_enabled=True):
         if self.bf16 and torch.cuda.is_available():

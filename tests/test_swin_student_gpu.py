@@ -162,7 +162,7 @@ def test_kd_step_of_a_swin_student_against_top_logits_eager_and_replayed():
     assert all(p.grad is not None and float(p.grad.abs().sum()) > 0 for p in tables)
 
 
-def test_a_captured_step_reads_the_index_that_was_loaded_after_its_capture():
+def test_a_captured_step_reads_the_index_that_was_loaded_after_its_capture(monkeypatch):
     """the capture has the plan's addresses: a checkpoint (with another index, and bias tables large enough to show it) loaded into a replaying trainer and an
     eager one, then equal losses and table gradients"""
     from segdistill_amd.engine import KDTrainer, SyntheticADE
@@ -171,7 +171,11 @@ def test_a_captured_step_reads_the_index_that_was_loaded_after_its_capture():
     gra = copy.deepcopy(ref)
     te, tg = KDTrainer(ref, opt, sched), KDTrainer(gra, opt, sched)
     de, dg = (SyntheticADE(2, size=(112, 120), num_classes=19, device='cuda:0', pool=3, seed=1) for _ in range(2))
+    from segdistill_amd import rel_bias
+    gathers, bias = [], rel_bias.bucket_bias
+    monkeypatch.setattr(rel_bias, 'bucket_bias', lambda *a: (gathers.append(torch.cuda.is_current_stream_capturing()), bias(*a))[1])
     assert tg.enable_graph(dict(img=dg._pool[0][0], img_metas=None, gt_semantic_seg=dg._pool[0][1])), getattr(tg, 'graph_error', None)
+    assert gathers == [False] * 8 + [True] * 4                             # two warm-up steps and the capture of four blocks
     graph = tg._graph
 
     def steps(n):
@@ -214,3 +218,36 @@ def test_a_captured_step_reads_the_index_that_was_loaded_after_its_capture():
 def _first_row_flipped():
     """the last token's row of a 7 x 7 window's index: (dy + 6) * 13 + dx + 6 from (6, 6)"""
     return [(6 - y + 6) * 13 + 6 - x + 6 for y in range(7) for x in range(7)]
+
+
+def test_the_bias_follows_an_index_that_was_changed_by_hand():
+    """the plan of the step before: an index written in place, replaced, and changed while it cannot be read (in a capture)"""
+    from segdistill_amd.backbones.swin import WindowAttention
+    torch.manual_seed(5)
+    att = WindowAttention(64, (4, 5), 2).cuda()
+    torch.nn.init.normal_(att.relative_position_bias_table)
+    table = att.relative_position_bias_table
+
+    def check(index):
+        out = att._bias(20, 2)
+        assert torch.equal(out, table.detach()[index.reshape(-1)].view(20, 20, 2).permute(2, 0, 1))
+        d = torch.randn_like(out)
+        want, size = (torch.zeros(63, 2, dtype=torch.float64).index_add_(0, index.reshape(-1).cpu(), x.double().cpu().reshape(2, -1).t()) for x in (d, d.abs()))
+        # at most 20 pairs of a bucket, a tree of six levels: within 15 steps of 2^-24 of the sum of magnitudes, as every bucket of one chunk
+        assert ((torch.autograd.grad(out, table, d)[0].double().cpu() - want).abs() <= 15 * 2.0 ** -24 * size).all()
+    index = att.relative_position_index
+    check(index)
+    index.copy_(index.flip(0).clone())
+    check(index)
+    att.relative_position_index = index.roll(1, 0)
+    check(index.roll(1, 0))
+    now = att.relative_position_index
+    now.copy_(index)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph), torch.no_grad():
+        att.relative_position_index.copy_(index.roll(3, 1))
+        out = att._bias(20, 2)
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(out, table.detach()[index.roll(3, 1).reshape(-1)].view(20, 20, 2).permute(2, 0, 1))
+    check(index.roll(3, 1))

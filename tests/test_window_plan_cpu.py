@@ -1,5 +1,6 @@
 """The bucket plan of a Swin block's window attention (rel_bias.BucketPlan): a captured step holds the addresses of its tensors, so a checkpoint load writes
 it in place.  Host logic: no GPU."""
+import copy
 import types
 import weakref
 
@@ -74,6 +75,7 @@ def _trainer(att):
 def test_the_trainer_keeps_its_captured_step_over_a_load_unless_a_plan_was_replaced():
     from segdistill_amd.backbones.swin import WindowAttention
     t = _trainer(WindowAttention(32, (24, 24), 1))
+    assert t.model[0].bias_plan.num_chunks > 47 * 47                              # built: a captured step has used it
     graph = t._graph
     sd = {'state_dict': {n: v.clone() for n, v in t.model.state_dict().items()}, 'optimizer': t.optimizer.state_dict(), 'meta': {'iter': 3}}
     t.load_state_dict(sd)
@@ -90,3 +92,43 @@ def test_a_plan_built_in_inference_mode_serves_a_backward():
         index = torch.arange(12).view(3, 4) % 5
         plan = BucketPlan(index, 5)
     assert not any(b.is_inference() for b in plan.buffers()) and _same(plan, index, 5)
+
+
+def test_the_plan_follows_its_buffer():
+    """changed in place (the plan too, at its address), replaced, filled by hand after to_empty or on the meta device, copied with its module"""
+    from segdistill_amd.backbones.swin import WindowAttention
+    att = WindowAttention(64, (4, 5), 2)
+    index, plan, at = att.relative_position_index, att.bias_plan, _at(att.bias_plan)
+    assert att.bias_plan is plan
+    index.copy_(index.flip(0).clone())
+    assert att.bias_plan is plan and _at(plan) == at and _same(plan, index, 63)
+    index.copy_(index.clone())                                             # (the same again)
+    assert att.bias_plan is plan and att.bias_plan is plan
+    other = copy.deepcopy(att)
+    assert other.bias_plan is not plan and _same(other.bias_plan, index, 63)
+    att.relative_position_index = index.roll(1, 0)
+    assert att.bias_plan is not plan and _same(att.bias_plan, index.roll(1, 0), 63) and _same(plan, index, 63)
+    keep = att.bias_plan
+    att.relative_position_index = att.relative_position_index.clone()
+    assert att.bias_plan is keep                                           # another tensor that says the same
+    with torch.device('meta'):
+        empty = WindowAttention(64, (4, 5), 2)
+    assert empty.bias_plan is None
+    for a in (empty, other):
+        a.to_empty(device='cpu')
+        a.relative_position_index.copy_(index)
+        assert _same(a.bias_plan, index, 63)
+    with torch.inference_mode():
+        att.relative_position_index = index.clone()
+    assert _same(att.bias_plan, index, 63) and _same(att.bias_plan, index, 63)
+
+
+def test_a_block_that_never_trains_has_no_plan():
+    from segdistill_amd.backbones.swin import WindowAttention, bias_plans
+    att = WindowAttention(64, (4, 4), 2)
+    att.load_state_dict(att.state_dict())
+    with torch.no_grad():
+        att(torch.randn(3, 16, 64))
+    assert bias_plans(att) == []
+    assert bias_plans(torch.nn.Sequential(att, WindowAttention(64, (4, 4), 2))) == [] and len(list(att.modules())) == 6
+    assert att.bias_plan is bias_plans(att)[0]
