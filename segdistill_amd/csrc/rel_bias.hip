@@ -40,8 +40,8 @@ template <typename T, bool DIRECT>
 __global__ __launch_bounds__(256) void bucket_bias_chunks(const T *__restrict__ dbias, const int *__restrict__ order, const int *__restrict__ chunk_start,
                                                           const int *__restrict__ chunk_order, float *__restrict__ part, T *__restrict__ dtable, int chunks, int H, long NP) {
     const int lane = threadIdx.x & 63;
-    const int n = gridDim.x, id = blockIdx.x, rem = n % 8, xcd = id % 8;              // consecutive logical workgroups share a chiplet
-    const int wg = (xcd < rem ? xcd * (n / 8 + 1) : rem * (n / 8 + 1) + (xcd - rem) * (n / 8)) + id / 8;
+    const int wgs = gridDim.x, id = blockIdx.x, rem = wgs % 8, xcd = id % 8;          // consecutive logical workgroups share a chiplet
+    const int wg = (xcd < rem ? xcd * (wgs / 8 + 1) : rem * (wgs / 8 + 1) + (xcd - rem) * (wgs / 8)) + id / 8;
     const int nth = __builtin_amdgcn_readfirstlane(wg * 4 + (int)(threadIdx.x >> 6));
     if (nth >= chunks) return;
     const int c = chunk_order[nth];
@@ -57,10 +57,11 @@ __global__ __launch_bounds__(256) void bucket_bias_chunks(const T *__restrict__ 
     }
     int at[kChunk / 64];
     bool in[kChunk / 64];
+    const int n = hi - lo;                            // (lo + 511 may lie beyond 2^31 - 1)
 #pragma unroll
     for (int u = 0; u < kChunk / 64; ++u) {
-        in[u] = lo + u * 64 + lane < hi;
-        at[u] = order[min(lo + u * 64 + lane, hi - 1)];               // lanes behind the end load the last pair again: no branch around a load
+        in[u] = u * 64 + lane < n;
+        at[u] = order[lo + min(u * 64 + lane, n - 1)];                // lanes behind the end load the last pair again: no branch around a load
     }
     for (int h = h0; h < h1; ++h) {
         const T *d = dbias + (size_t)h * NP;

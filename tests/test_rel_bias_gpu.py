@@ -141,3 +141,28 @@ def test_offsets_past_32_bits():
         one = rel_bias.bucket_bias(t, plan)
         assert torch.equal(one[0], out[h]) and torch.equal(one[0, 5], t.detach()[plan.index[5].long(), 0])
         assert torch.equal(torch.autograd.grad(one, t, grad[h:h + 1])[0][:, 0], dtable[:, h])
+
+
+def test_the_last_chunk_of_as_many_pairs_as_there_may_be():
+    """2^31 - 1 pairs: the last chunk starts 188 pairs before the end, and 512 from there is beyond a 32-bit integer.  The plan as the C entry takes it, the
+    pairs in their own order: all but 700 in one bucket, the rest in the other.  704 and 0 are exact in bf16, and so is every sum on the way."""
+    from segdistill_amd import _lib
+    L, pairs, last = _lib.lib(), 2 ** 31 - 1, 700
+    order = torch.arange(pairs, device='cuda', dtype=torch.int32)
+    first = torch.arange(0, pairs - last, 512, device='cuda')
+    start = torch.cat([first, torch.tensor([pairs - last, pairs - last + 512, pairs], device='cuda')]).int()
+    chunks = start.numel() - 1
+    bucket = torch.tensor([0, first.numel(), chunks], device='cuda', dtype=torch.int32)
+    assert int(start[-1] - start[-2]) == 188
+    dbias = torch.zeros(pairs, device='cuda', dtype=torch.bfloat16)
+    dbias[-last:] = 1
+    dbias[-4:] = 2
+    out = torch.full((2, 1), float('nan'), device='cuda', dtype=torch.bfloat16)
+    size = L.sd_bucket_bias_workspace_bytes(2, chunks, 1)
+    work = torch.empty(size, dtype=torch.uint8, device='cuda')
+    by_pair = torch.arange(chunks, device='cuda', dtype=torch.int32)
+    rc = L.sd_bucket_bias_bwd(dbias.data_ptr(), order.data_ptr(), start.data_ptr(), by_pair.data_ptr(), bucket.data_ptr(), out.data_ptr(), 1, 2, chunks, 1, pairs,
+                              work.data_ptr(), size, torch.cuda.current_stream().cuda_stream)
+    assert rc == 0
+    torch.cuda.synchronize()
+    assert out.flatten().tolist() == [0.0, 704.0]
