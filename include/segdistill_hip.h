@@ -314,7 +314,7 @@ int sd_window_attn_fwd_packed(const void *qkv, const float *bias_packed, const f
  * Softmax, its gradient and the bias gradient are fp32 for both storage types.  A row that bias + mask leave at -inf everywhere has output 0 and no
  * gradient.  The backward recomputes the probabilities: nothing but the operands and `packed` is kept.  dbias sums the windows in a fixed order
  * (slabs in `workspace`, 16-byte aligned, _workspace_bytes; no atomics).
- * _supported(): 1 <= N <= 64, D == 32, else SD_E_UNSUPPORTED.  qkv, out, dout, dqkv 16-byte aligned.
+ * _supported(): 1 <= N <= 64, D == 32, else SD_E_UNSUPPORTED.  heads + mask_windows < 2^24.  qkv, out, dout, dqkv 16-byte aligned.
  */
 int sd_window_attn_train_supported(int tokens_per_window, int head_dim);
 size_t sd_window_attn_train_packed_floats(int heads, int mask_windows, int tokens_per_window);

@@ -549,6 +549,7 @@ int per_cu(size_t lds, int waves_per_simd, int NA) {
 template <typename T>
 int bwd_slabs(long windows, int heads, int N) { return slabs_for(windows, heads, per_cu(bwd_lds<T>(tiles(N)), kBwdWaves, tiles(N))); }
 
+constexpr int kMaxTables = 0xffffff;                                  // a workgroup of 256 threads each: a launch holds fewer than 2^32 threads
 bool shape_ok(long windows, int heads, int N) { return windows > 0 && heads > 0 && heads <= 65535 && windows <= 0x3fffffffL / heads && N >= 1 && N <= 64; }
 size_t table_elems(int N) { return (size_t)tiles(N) * tiles(N) * 256; }
 size_t table_floats(int heads, int nW, int N) { return (size_t)(heads + nW) * table_elems(N); }
@@ -557,7 +558,7 @@ int check_args(const void *qkv, const float *packed, size_t packed_floats, int d
     if (!qkv || !packed) return SD_E_NULL;
     if (dtype != SD_F32 && dtype != SD_BF16) return SD_E_DTYPE;
     if (!sd_window_attn_train_supported(N, d)) return SD_E_UNSUPPORTED;
-    if (!shape_ok(windows, heads, N) || nW < 0 || (nW > 0 && windows % nW != 0)) return SD_E_SHAPE;
+    if (!shape_ok(windows, heads, N) || nW < 0 || (nW > 0 && windows % nW != 0) || nW > kMaxTables - heads) return SD_E_SHAPE;
     if (packed_floats < sd_window_attn_train_packed_floats(heads, nW, N)) return SD_E_WORKSPACE;
     if ((reinterpret_cast<uintptr_t>(qkv) | reinterpret_cast<uintptr_t>(packed)) & 15) return SD_E_ALIGN;
     return SD_OK;

@@ -154,3 +154,9 @@ def test_window_attention_built_on_the_meta_device_gets_its_plan_with_the_loaded
             assert torch.equal(t, dict(att.bias_plan.named_buffers())[name]), name
     x = torch.randn(4, 12, 64)
     assert torch.equal(att(x), real(x))
+
+
+def test_more_masks_than_one_launch_packs_are_refused(L):
+    for w, h, want in ((1 << 24, 1, E_SHAPE), ((1 << 24) - 1, 1, E_SHAPE), ((1 << 24) - 2, 1, E_WS), ((1 << 24) - 2, 2, E_SHAPE)):
+        assert L.sd_window_attn_train_fwd(P, P, P, P, 10, P, 0, w, w, h, 1, 32, 1.0, NULL) == want, (w, h)
+        assert L.sd_window_attn_train_bwd(P, P, 10, P, P, P, 0, w, w, h, 1, 32, 1.0, P, 1 << 40, NULL) == want, (w, h)
