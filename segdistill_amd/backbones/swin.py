@@ -25,6 +25,7 @@ import torch.nn.functional as F
 from ..builder import BACKBONES
 from ..layernorm import HipLayerNorm, layernorm_map, map_supported          # nn.LayerNorm subclass: same keys, HIP kernels on CUDA tokens (ATen's ran 3.9 ms of a config-4 step)
 from .. import rel_bias, window_attn
+from ..ops import _transformed
 from ..layers import DropPath, to_2tuple, trunc_normal_
 
 
@@ -148,7 +149,7 @@ class WindowAttention(nn.Module):
         plan = self.bias_plan if (tbl.requires_grad or torch.is_grad_enabled()) and rel_bias.supported(tbl) else None
         if plan is None:
             return tbl[self.relative_position_index.view(-1)].view(n, n, h).permute(2, 0, 1)
-        return rel_bias.bucket_bias(tbl, plan)
+        return rel_bias.bucket_bias(tbl, plan, True)
 
     def _mask_packed(self, mask):
         if mask is None:
@@ -169,6 +170,8 @@ class WindowAttention(nn.Module):
         h = self.num_heads
         tbl = self.relative_position_bias_table
         qkv = self.qkv(x)
+        if x.is_cuda and _transformed() and not (self.training and self.attn_drop.p > 0):
+            return self.proj_drop(self.proj(window_attn.plain_attention(qkv, self._bias(n, h), mask, h, self.scale)))
         if (not (torch.is_grad_enabled() and (qkv.requires_grad or tbl.requires_grad)) and not (self.training and self.attn_drop.p > 0)
                 and window_attn.supported(qkv, n, h, c // h) and (mask is None or bw % mask.shape[0] == 0)):
             # no graph to build (the frozen teacher): one kernel over the qkv Linear's output, bias and mask read from their tables

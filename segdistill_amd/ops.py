@@ -41,6 +41,20 @@ def _no_double_backward(name):
         raise RuntimeError(f'{name} has no second derivative (backward was called with create_graph=True)')
 
 
+def _transformed():
+    """A torch.func transform or forward-mode differentiation is on: kernels reached by address take no part in those."""
+    return torch._C._functorch.peek_interpreter_stack() is not None or torch.autograd.forward_ad._current_level >= 0
+
+
+def _addressless(t):
+    """A tensor that stands for a batch of others (a gradient under is_grads_batched or vmap)."""
+    try:
+        t.data_ptr()
+    except RuntimeError:
+        return True
+    return False
+
+
 class _CGDKLFunction(torch.autograd.Function):
     """loss = alpha/rows * sum_rows KL(softmax(T_r/tau) || softmax(S_r/tau)); S,T at softmax resolution."""
 

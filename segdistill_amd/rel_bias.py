@@ -7,7 +7,7 @@ import torch
 import torch.nn as nn
 
 from . import _lib
-from .ops import _DT, _launch, _no_double_backward, _ptr, _require_gpu
+from .ops import _DT, _addressless, _launch, _no_double_backward, _ptr, _require_gpu, _transformed
 
 
 CHUNK = 512          # sd_bucket_bias_chunk(): the pairs of one bucket that one wave sums (a plan is built without the library)
@@ -66,21 +66,24 @@ class BucketPlan(nn.Module):
 
 class _BucketBiasFunction(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, table, plan):
+    def forward(ctx, table, plan, create_graph):
         nb, heads = table.shape
+        held = tuple(plan._buffers[n] for n in ('index', 'order', 'chunk_start', 'chunk_order', 'bucket_chunk'))
         out = torch.empty((heads,) + plan.shape, dtype=table.dtype, device=table.device)
-        rc = _launch(table.device, _lib.lib().sd_bucket_bias_fwd, table.data_ptr(), plan._buffers['index'].data_ptr(), out.data_ptr(), _DT[table.dtype], nb, heads,
-                     plan.num_pairs)
+        rc = _launch(table.device, _lib.lib().sd_bucket_bias_fwd, table.data_ptr(), held[0].data_ptr(), out.data_ptr(), _DT[table.dtype], nb, heads, plan.num_pairs)
         _lib.check(rc, 'sd_bucket_bias_fwd')
-        ctx.plan = plan
-        ctx.save_for_backward(*(plan._buffers[n] for n in ('order', 'chunk_start', 'chunk_order', 'bucket_chunk')))      # (the plan may move meanwhile, or be updated: an error)
+        ctx.plan, ctx.create_graph = plan, create_graph
+        ctx.save_for_backward(*held)                   # (the plan may move meanwhile, or be updated: an error)
         return out
 
     @staticmethod
     def backward(ctx, grad_out):
-        _no_double_backward('bucket_bias')
         plan = ctx.plan
-        order, start, by_pair, bucket = ctx.saved_tensors
+        index, order, start, by_pair, bucket = ctx.saved_tensors
+        if ctx.create_graph and (torch.is_grad_enabled() or _addressless(grad_out)):
+            d = grad_out.reshape(grad_out.shape[0], -1).t().float()
+            return d.new_zeros(plan.num_buckets, d.shape[1]).index_add(0, index.reshape(-1), d).to(grad_out.dtype), None, None
+        _no_double_backward('bucket_bias')
         nb, chunks = plan.num_buckets, plan.num_chunks
         d = grad_out.contiguous()
         heads = d.shape[0]
@@ -91,16 +94,18 @@ class _BucketBiasFunction(torch.autograd.Function):
         rc = _launch(d.device, L.sd_bucket_bias_bwd, d.data_ptr(), order.data_ptr(), start.data_ptr(), by_pair.data_ptr(), bucket.data_ptr(),
                      dtable.data_ptr(), _DT[d.dtype], nb, chunks, heads, plan.num_pairs, _ptr(ws), ws_bytes)
         _lib.check(rc, 'sd_bucket_bias_bwd')
-        return dtable, None
+        return dtable, None, None
 
 
 def supported(table):
-    """bucket_bias takes a table of this type on this device."""
-    return table.is_cuda and table.dtype in _DT
+    """bucket_bias takes a table of this type on this device, and no transform (torch.func, forward mode) is on."""
+    return table.is_cuda and table.dtype in _DT and not _transformed()
 
 
-def bucket_bias(table, plan):
-    """table [num_buckets, heads] (fp32 or bf16) -> bias [heads, Nq, Nk] = table[index].permute(2, 0, 1), with a deterministic gradient for the table."""
+def bucket_bias(table, plan, create_graph=False):
+    """table [num_buckets, heads] (fp32 or bf16) -> bias [heads, Nq, Nk] = table[index].permute(2, 0, 1), with a deterministic gradient for the table.
+    create_graph: the gradient may be asked for with a graph of its own, or for a batch of gradients at once (then by torch operators); without, that is an
+    error."""
     _require_gpu(table)
     if table.dtype not in _DT:
         raise TypeError(f'bucket_bias: unsupported dtype {table.dtype}')
@@ -108,4 +113,4 @@ def bucket_bias(table, plan):
         raise ValueError(f'bucket_bias: table {tuple(table.shape)} does not fit a plan of {plan.num_buckets} buckets')
     if plan._buffers['index'].device != table.device:
         raise ValueError(f'bucket_bias: the plan is on {plan.index.device}, the table on {table.device}')
-    return _BucketBiasFunction.apply(table.contiguous(), plan)
+    return _BucketBiasFunction.apply(table.contiguous(), plan, create_graph)

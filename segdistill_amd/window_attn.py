@@ -3,12 +3,13 @@ output (csrc/window_attn.hip; reference mmseg/models/backbones/swin_transformer.
 from small packed tables inside the kernel, q / k / v are not permuted and the output comes out token-major for the projection."""
 from __future__ import annotations
 
+import math
 import os
 
 import torch
 
 from . import _lib
-from .ops import _DT, _launch, _no_double_backward, _ptr, _require_gpu, _stream_ptr
+from .ops import _DT, _addressless, _launch, _ptr, _require_gpu, _stream_ptr, _transformed
 
 ENABLED = os.environ.get('SEGDISTILL_WINDOW_ATTN', '1') == '1'       # A/B: 0 = F.scaled_dot_product_attention with a materialised additive tensor
 
@@ -48,8 +49,46 @@ def forward_packed(qkv, bias_p, mask_p, mask_flags, heads, scale):
 
 
 def train_supported(qkv, n, head_dim):
-    """The training kernels take this qkv Linear output [windows, N, 3*heads*head_dim]: fp32 or bf16, windows of up to 64 tokens, head_dim 32."""
-    return bool(ENABLED and qkv.is_cuda and qkv.dtype in _DT and qkv.dim() == 3 and _lib.lib().sd_window_attn_train_supported(int(n), int(head_dim)))
+    """The training kernels take this qkv Linear output [windows, N, 3*heads*head_dim]: fp32 or bf16, windows of up to 64 tokens, head_dim 32; and no transform
+    (torch.func, forward mode) is on."""
+    return bool(ENABLED and qkv.is_cuda and qkv.dtype in _DT and qkv.dim() == 3 and not _transformed()
+                and _lib.lib().sd_window_attn_train_supported(int(n), int(head_dim)))
+
+
+def _version(t):
+    return None if t is None or t.is_inference() else t._version
+
+
+def _probabilities(qkv, bias, mask, heads, scale):
+    """q, k, v [windows, heads, N, D] and the softmax of their scores, in fp32 (fp64 where qkv is) by torch operators"""
+    bw, n, c3 = qkv.shape
+    wide = torch.promote_types(qkv.dtype, torch.float32)
+    q, k, v = (t.contiguous() for t in qkv.to(wide).reshape(bw, n, 3, heads, c3 // 3 // heads).permute(2, 0, 3, 1, 4))
+    s = q @ k.transpose(-2, -1).contiguous() * scale + bias.to(wide)
+    if mask is not None:
+        s = (s.view(bw // mask.shape[0], mask.shape[0], heads, n, n) + mask.detach().to(wide).unsqueeze(1)).view(bw, heads, n, n)
+    nothing = (s == -math.inf).all(-1, keepdim=True)
+    return q, k, v, torch.softmax(s.masked_fill(nothing, 0.), -1).masked_fill(nothing, 0.)
+
+
+def plain_attention(qkv, bias, mask, heads, scale):
+    """`attention` by torch operators that every transform (torch.func, forward mode) knows.  (The library's fused attention is not one of them: per-sample
+    gradients of its additive tensor are wrong from the second sample on.)"""
+    with torch.autocast(qkv.device.type, enabled=False):
+        _, _, v, p = _probabilities(qkv, bias, mask, heads, scale)
+        return (p @ v).transpose(1, 2).reshape(qkv.shape[0], qkv.shape[1], -1).to(qkv.dtype)
+
+
+def _plain_gradients(qkv, bias, mask, heads, scale, grad_out):
+    """The gradients (csrc/window_train.hip) by torch operators in fp32, which differentiate further and take batches of gradients."""
+    bw, n, c3 = qkv.shape
+    with torch.autocast(qkv.device.type, enabled=False):
+        q, k, v, p = _probabilities(qkv, bias, mask, heads, scale)
+        g = grad_out.float().reshape(bw, n, heads, -1).transpose(1, 2).contiguous()
+        dp = g @ v.transpose(-2, -1).contiguous()
+        ds = p * (dp - (p * dp).sum(-1, keepdim=True))
+        dqkv = torch.stack([ds @ k * scale, ds.transpose(-2, -1).contiguous() @ q * scale, p.transpose(-2, -1).contiguous() @ g])
+        return dqkv.permute(1, 3, 0, 2, 4).reshape(bw, n, c3).to(qkv.dtype), ds.sum(0).to(bias.dtype)
 
 
 class _WindowAttentionFunction(torch.autograd.Function):
@@ -67,13 +106,18 @@ class _WindowAttentionFunction(torch.autograd.Function):
         _lib.check(rc, 'sd_window_attn_train_fwd')
         ctx.save_for_backward(qkv, packed)
         ctx.meta = (nw, heads, scale, bias.dtype)
+        ctx.tables = (bias, mask, _version(bias), _version(mask))          # `packed` has what the kernel needs: these may change, unless a graph is asked for
         return out
 
     @staticmethod
     def backward(ctx, grad_out):
-        _no_double_backward('window_attn.attention')
         qkv, packed = ctx.saved_tensors
         nw, heads, scale, bias_dtype = ctx.meta
+        if torch.is_grad_enabled() or _addressless(grad_out):
+            bias, mask, *versions = ctx.tables
+            if versions != [_version(bias), _version(mask)]:
+                raise RuntimeError('window_attn.attention: bias or mask was modified by an inplace operation between the forward and a backward with a graph of its own')
+            return (*_plain_gradients(qkv, bias, mask, heads, scale, grad_out), None, None, None)
         bw, n, c3 = qkv.shape
         L, dt = _lib.lib(), _DT[qkv.dtype]
         go = grad_out.to(qkv.dtype).contiguous()
@@ -94,7 +138,8 @@ def attention(qkv, bias, mask, heads, scale):
 
     qkv [windows, N, 3*heads*32] (fp32 or bf16) as the qkv Linear leaves it, N <= 64; bias [heads, N, N]; mask [nW, N, N] additive, without a gradient
     (windows of one image are contiguous and nW divides their number), or None -> [windows, N, heads*32].  A query row that bias + mask leave at -inf
-    everywhere has output 0 and no gradient."""
+    everywhere has output 0 and no gradient.  A gradient with a graph of its own (create_graph), or for a batch of gradients at once, is taken by torch
+    operators."""
     _require_gpu(qkv, bias)
     heads = int(heads)
     if qkv.dim() != 3 or heads <= 0 or qkv.shape[2] % (3 * heads):

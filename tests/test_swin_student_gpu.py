@@ -251,3 +251,93 @@ def test_the_bias_follows_an_index_that_was_changed_by_hand():
     torch.cuda.synchronize()
     assert torch.equal(out, table.detach()[index.roll(3, 1).reshape(-1)].view(20, 20, 2).permute(2, 0, 1))
     check(index.roll(3, 1))
+
+
+def _attention_twice(seed=6):
+    """a trainable window attention, and the same in fp64 on the CPU"""
+    from segdistill_amd.backbones.swin import WindowAttention
+    torch.manual_seed(seed)
+    att = WindowAttention(64, (4, 4), 2)
+    torch.nn.init.normal_(att.relative_position_bias_table)
+    ref = copy.deepcopy(att).double()
+    x = torch.randn(6, 16, 64)
+    mask = torch.where(torch.rand(3, 16, 16) < 0.2, -100.0, 0.0)
+    mask[1, 3] = -100.0
+    return att.cuda(), ref, x, mask
+
+
+def _close(got, want, what=''):
+    """two Linears, a softmax and their derivatives in fp32: 1e-4 of the largest value is two hundred times what their sums of 64 to 192 terms round by"""
+    got = got.detach().double().cpu()
+    assert got.shape == want.shape and float((got - want).abs().max()) <= 1e-4 * float(want.abs().max()), what
+
+
+def test_gradients_with_a_graph_of_their_own():
+    """create_graph through a trainable block: first and second derivatives against fp64"""
+    att, ref, x, mask = _attention_twice()
+    both = []
+    for a, inp, m in ((att, x.cuda(), mask.cuda()), (ref, x.double(), mask.double())):
+        inp.requires_grad_()
+        names = [n for n, _ in a.named_parameters()]
+        params = list(a.parameters())
+        first = torch.autograd.grad(a(inp, m).square().sum(), [inp] + params, create_graph=True)
+        second = torch.autograd.grad(sum(g.square().sum() for g in first), [inp] + params)
+        both.append((first, second))
+    for k, (got, want) in enumerate(zip(both[0], both[1])):
+        for n, g, w in zip(['x'] + names, got, want):
+            _close(g, w.detach(), (k, n))
+    # and a gradient without a graph is the kernel's, as before
+    xg = x.cuda().requires_grad_()
+    plain = torch.autograd.grad(att(xg, mask.cuda()).square().sum(), [xg] + list(att.parameters()))
+    for g, w in zip(plain, both[1][0]):
+        _close(g, w.detach())
+
+
+def test_transforms_take_torch_operators():
+    """torch.func.grad, per-sample gradients, vmap, a batch of gradients at once; the forward mode against the backward: w . J v = J^T w . v"""
+    att, ref, x, mask = _attention_twice(7)
+    out = []
+    for a, inp, m in ((att, x.cuda(), mask.cuda()), (ref, x.double(), mask.double())):
+        params = {n: p.detach() for n, p in a.named_parameters()}
+
+        def loss(p, y):
+            return torch.func.functional_call(a, p, (y, m)).square().sum()
+        pair = torch.stack([inp, inp.flip(0)])
+        one = torch.func.grad(loss)(params, inp)
+        per = torch.func.vmap(torch.func.grad(loss), in_dims=(None, 0))(params, pair)
+        mapped = torch.func.vmap(lambda y: a(y, m))(pair)
+        leaf = inp.clone().requires_grad_()
+        y = a(leaf, m)
+        ds = torch.stack([torch.ones_like(y), y.detach(), y.detach().flip(0)])
+        batch = torch.autograd.grad(y, [leaf] + list(a.parameters()), ds, is_grads_batched=True)
+        if a is att:
+            tangent = torch.func.jvp(lambda z: a(z, m), (inp,), (pair[1],))[1]
+            assert tangent.shape == y.shape
+            along = (tangent.double() * ds[1].double()).sum().view(1)
+        else:
+            along = (batch[0][1] * pair[1]).sum().view(1)
+        out.append((list(one.values()), list(per.values()), [mapped], list(batch), [along]))
+    wide = copy.deepcopy(ref).cuda()
+    got = torch.func.vmap(lambda y: wide(y, mask.double().cuda()))(pair.cuda())
+    assert float((got.cpu() - mapped).abs().max()) <= 1e-13 * float(mapped.abs().max())
+    for got, want in zip(*out):
+        for g, w in zip(got, want):
+            _close(g, w.detach())
+
+
+def test_tables_may_change_behind_a_forward_unless_a_graph_is_asked_for():
+    from segdistill_amd import window_attn
+    g = torch.Generator(device='cuda').manual_seed(8)
+    qkv = torch.randn(4, 9, 192, device='cuda', generator=g, requires_grad=True)
+    bias, mask = torch.randn(2, 9, 9, device='cuda', generator=g), torch.zeros(2, 9, 9, device='cuda')
+    with torch.inference_mode():
+        cached = mask.clone()                                               # as one that an evaluation left behind
+    out = window_attn.attention(qkv, bias, mask, 2, 0.2)
+    want = torch.autograd.grad(out, qkv, torch.ones_like(out), retain_graph=True)[0]
+    with_graph = torch.autograd.grad(window_attn.attention(qkv, bias, cached, 2, 0.2), qkv, torch.ones_like(out), create_graph=True)[0]
+    assert float((with_graph - want).abs().max()) <= 1e-5 * float(want.abs().max())
+    mask.fill_(3.0)
+    bias.zero_()
+    assert torch.equal(torch.autograd.grad(out, qkv, torch.ones_like(out), retain_graph=True)[0], want)
+    with pytest.raises(RuntimeError, match='modified'):
+        torch.autograd.grad(out, qkv, torch.ones_like(out), create_graph=True)
