@@ -450,6 +450,69 @@ def test_offsets_past_32_bits():
     assert abs(float(loss)) < 1e-6 and float(d[-1].abs().max()) < 1e-8 and float(d[0].abs().max()) < 1e-8
 
 
+def _poisoned(like):
+    """the address of memory that holds NaN, free again: the next tensor of that size"""
+    torch.cuda.synchronize()
+    t = torch.full_like(like, math.nan)
+    return t.data_ptr()
+
+
+def _parts_agree(S, v, i, r, valid, tau, parts):
+    """topk_kl of all of S against the same on `parts`, equal pieces of it: the loss is their mean; the gradient of a piece alone is as many times larger, up to
+    the rounding of the two results (half a step of bf16 each) and of the 32-bit factors before it.  The gradient is written where NaN was."""
+    from segdistill_amd import ops
+    S.requires_grad_()
+    loss = ops.topk_kl(S, v, i, r, tau=tau, alpha=1.0, valid=valid)
+    at = _poisoned(S.detach())
+    (d,) = torch.autograd.grad(loss, S)
+    assert d.data_ptr() == at
+    mean = 0.0
+    for p in parts:
+        s = S.detach()[p].clone().requires_grad_()
+        one = ops.topk_kl(s, v[p], i[p], r[p], tau=tau, alpha=1.0, valid=None if valid is None else valid[p])
+        (g,) = torch.autograd.grad(one, s)
+        mean += float(one.detach()) / len(parts)
+        a, b = d[p].float() * len(parts), g.float()
+        assert bool(((a - b).abs() <= (2 ** -7 + 16 * U) * b.abs()).all()), p
+        assert float(b.abs().amax()) > 0
+    assert abs(float(loss.detach()) - mean) <= 4 * U * mean and mean > 0.1
+
+
+def test_rows_past_32_bits_against_their_parts():
+    """2.3e9 logits in rows (bf16): selection and criterion, every row of the gradient, against calls on eighths"""
+    from segdistill_amd import ops
+    R, V = 17600, 131072
+    g = torch.Generator(device='cuda').manual_seed(21)
+    S = torch.empty(R, V, device='cuda', dtype=torch.bfloat16).normal_(std=2.0, generator=g)
+    parts = [slice(a, a + R // 8) for a in range(0, R, R // 8)]
+    top = ops.topk_logits(S, 5, tau=2.0)
+    for p in (parts[0], parts[-1]):
+        assert all(torch.equal(a[p], b) for a, b in zip(top, ops.topk_logits(S[p].clone(), 5, tau=2.0)))
+    assert int(top[1][-1].long().unique().numel()) == 5 and torch.equal(top[0][-1], S[-1][top[1][-1].long()])
+    i = torch.randint(0, V, (R, 6), device='cuda', generator=g, dtype=torch.int32)
+    v = torch.randn(R, 6, device='cuda', generator=g) * 3
+    _parts_agree(S, v, i, torch.randn(R, device='cuda', generator=g) + 9.0, None, 2.0, parts)
+
+
+def test_planes_past_32_bits_against_their_images():
+    """2.9e9 logits in class planes (bf16), the last image wholly beyond 2^31"""
+    from segdistill_amd import ops
+    B, C, H = 4, 150, 2200
+    g = torch.Generator(device='cuda').manual_seed(22)
+    S = torch.empty(B, C, H, H, device='cuda', dtype=torch.bfloat16).normal_(std=2.0, generator=g)
+    T = torch.empty(B, C, H, H, device='cuda', dtype=torch.bfloat16).normal_(std=3.0, generator=g)
+    assert 3 * C * H * H > 2 ** 31
+    v, i, r = ops.topk_logits(T, 5, tau=2.0)
+    images = [slice(b, b + 1) for b in range(B)]
+    for p in images:
+        assert all(torch.equal(a[p], b) for a, b in zip((v, i, r), ops.topk_logits(T[p].clone(), 5, tau=2.0)))
+    del T
+    # as many valid pixels in every image, so that a part's mean is over exactly a quarter of them
+    keep = torch.rand(1, H, H, device='cuda', generator=g) < 0.8
+    valid = torch.cat([keep.roll(n, 2) for n in range(B)])
+    _parts_agree(S, v, i, r, valid, 2.0, images)
+
+
 def test_criterion_module_in_the_distillation_loss():
     """TopKLoss by its registered name: selection on the teacher tap, criterion on the student tap, ignored labels left out, a teacher of another size"""
     from segdistill_amd.distillation.opts import DistillationLoss
