@@ -786,7 +786,7 @@ def topk_kl(S, values, index, rest=None, *, tau, alpha, valid=None):
         return S.float().sum() * 0.0
     if not _lib.lib().sd_topk_kl_supported(B, Cc, P, k):
         raise ValueError(f'topk_kl: {k} entries of {Cc} classes are not supported (at most {_lib.lib().sd_topk_max_entries()} entries; class planes hold a '
-                         'bit per class and pixel in LDS)')
+                         f'bit per class and pixel in LDS), or {B * P} rows are more than a launch takes')
     if index.dtype == torch.int64:
         index = index.clamp(-1, 2 ** 31 - 1).to(torch.int32)
     return _TopKKLFunction.apply(S.contiguous(), values.detach().contiguous(), index.contiguous(), None if rest is None else rest.detach().contiguous(),

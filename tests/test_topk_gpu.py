@@ -620,3 +620,13 @@ def test_module_resizes_both_taps_to_the_label_size():
     assert float(loss) == pytest.approx(float(want), rel=1e-4)
     a, b = torch.autograd.grad(loss, s)[0], torch.autograd.grad(want, s)[0]
     assert float((a - b).norm() / b.norm()) < 1e-4
+
+
+def test_more_rows_than_the_criterion_launches_are_named():
+    from segdistill_amd import ops
+    rows = 4 * 0xffffff + 1
+    S = torch.zeros(rows, 2, device='cuda')
+    with pytest.raises(ValueError, match=f'{rows} rows'):
+        ops.topk_kl(S, S[:, :1], torch.zeros(rows, 1, device='cuda', dtype=torch.int32), tau=1.0, alpha=1.0)
+    loss = ops.topk_kl(S[1:], S[1:, :1], torch.zeros(rows - 1, 1, device='cuda', dtype=torch.int32), torch.zeros(rows - 1, device='cuda'), tau=1.0, alpha=1.0)
+    assert float(loss) == 0.0
