@@ -333,7 +333,7 @@ int sd_window_attn_train_bwd(const void *qkv, const float *packed, size_t packed
  *   backward  dtable[b][h] = sum_{index[p] = b} dbias[h][p]: `order` lists the pairs bucket by bucket; chunk i is order[chunk_start[i] ..
  *             chunk_start[i + 1]) with at most sd_bucket_bias_chunk() pairs of ONE bucket; bucket b owns the chunks [bucket_chunk[b],
  *             bucket_chunk[b + 1]), at least one (an empty bucket: an empty one).  chunk_order: the chunks in the order they are taken (any permutation; by first pair
- *             they share cache lines).  fp32 sums in a fixed order, the chunks of a bucket in fp64.
+ *             they share cache lines).  Sums in fp64, in a fixed order; the chunk sums of a bucket of several are kept in fp32 in between.
  *             workspace: sd_bucket_bias_workspace_bytes (0 when every bucket is one chunk).
  */
 int sd_bucket_bias_chunk(void);

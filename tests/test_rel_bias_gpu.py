@@ -166,3 +166,22 @@ def test_the_last_chunk_of_as_many_pairs_as_there_may_be():
     assert rc == 0
     torch.cuda.synchronize()
     assert out.flatten().tolist() == [0.0, 704.0]
+
+
+@pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize('ws,heads', [(4, 3), (7, 4), (12, 6), (22, 2)])
+def test_a_bucket_of_one_chunk_is_rounded_once(ws, heads, dtype):
+    """up to 512 pairs are summed in 64 bits: nothing but the result's half step is left (and 2^-44 of the magnitudes, 512 additions of 2^-53)"""
+    from segdistill_amd import rel_bias
+    index, nb = _window_index(ws, ws), (2 * ws - 1) ** 2
+    plan = rel_bias.BucketPlan(index.cuda(), nb)
+    assert plan.num_chunks == nb
+    g = torch.Generator(device='cuda').manual_seed(ws)
+    table = torch.zeros(nb, heads, device='cuda', dtype=dtype, requires_grad=True)
+    d = torch.randn(heads, ws * ws, ws * ws, device='cuda', generator=g).to(dtype)
+    got = torch.autograd.grad(rel_bias.bucket_bias(table, plan), table, d)[0].double().cpu()
+    dd = d.double().cpu().reshape(heads, -1).t()
+    ref, mag = (torch.zeros(nb, heads, dtype=torch.float64).index_add_(0, index.reshape(-1), x) for x in (dd, dd.abs()))
+    # to bf16 by way of fp32: its half step besides
+    lim = (torch.finfo(dtype).eps / 2 + (0 if dtype == torch.float32 else U)) * ref.abs() + 2.0 ** -44 * mag
+    assert ((got - ref).abs() <= lim).all()
