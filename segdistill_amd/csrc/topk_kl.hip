@@ -9,8 +9,8 @@
 //
 // Each row keeps (m_r, w, m, 1/s): its gradient is w 2^{(z_c - m_r) c2} outside A, with w = (q_r - p_r) / s_r.
 // Memory bound: the forward reads z, the backward reads z and writes dz; nothing of the size of z is kept between them.
-// Measured: [8, 150, 128, 128] fp32, k = 10: forward 29 us (2.7 TB/s), backward 40 us (4.0 TB/s); 2048 rows of 65536 bf16, k = 64: forward 55 us
-// (4.9 TB/s), backward 98 us (5.5 TB/s); the join of the row losses 4 us.
+// Measured: [8, 150, 128, 128] fp32, k = 10: forward 29 us (2.7 TB/s), backward 40 us (4.0 TB/s); in bf16 50 and 63 us
+// (1.6 and 2.5 TB/s); 2048 rows of 65536 bf16, k = 64: forward 54 us (5.0 TB/s), backward 98 us (5.5 TB/s); the join of the row losses 2 to 5 us.
 #include <hip/hip_runtime.h>
 #include <math.h>
 
@@ -301,7 +301,7 @@ __global__ __launch_bounds__(BT *kWaves) void topk_kl_planes_bwd(const T *__rest
 // ---- contiguous rows [B, C]: NT threads per row ----------------------------------------------------------------------------------------------------
 // A is a bit mask of the row in LDS, shifted so that an aligned 16-byte vector of logits has its bits in one byte (bf16) or half a byte (fp32).
 // Every wave takes the entries by itself, two per lane: their statistics need no exchange.  Short rows are bound by what a row costs a wave whatever its length --
-// the reductions over 64 lanes, the 64-bit end: 1.3 ns (65536 rows of 150 fp32: 89 us; as class planes the same logits take 15).
+// the reductions over 64 lanes, the 64-bit end: 1.3 ns (65536 rows of 150 fp32: 87 us, VALU 98 % busy, backward 57; as class planes the same logits take 15).
 struct RowEntries {
     int c[2];
     float v[2];

@@ -8,8 +8,8 @@
 // k entries; the sums of the rest are taken over the unchosen terms only -- total minus chosen would cancel exactly where a confident teacher
 // needs the digits -- and relative to the largest of them, so they neither overflow nor vanish.
 //
-// Memory bound where nothing else were: N e bytes.  Measured: [8, 150, 128, 128] fp32, k = 10: 34 us (2.3 TB/s; the rounds of the search in LDS and VALU).
-// 2048 rows of 65536 bf16, k = 64: 72 us (3.7 TB/s; the read alone with the group maxima 40).  One row of 32003 fp32: 7.5 us, a chain of latencies.
+// Memory bound where nothing else were: N e bytes.  Measured: [8, 150, 128, 128] fp32, k = 10: 34 us (2.3 TB/s; the rounds of the search in LDS and VALU, 41 % busy), in
+// bf16 36 us.  2048 rows of 65536 bf16, k = 64: 71 to 75 us (3.7 TB/s; the read alone with the group maxima 40).  One row of 32003 fp32: 8 us, a chain of latencies.
 #include <hip/hip_runtime.h>
 #include <math.h>
 

@@ -20,10 +20,11 @@
 //   value and what its rounding left): one term alone would put an error as large as the result's own rounding on every output.
 //   Softmax, dS and the bias gradient are fp32.  Operand columns come from the row images by transposed LDS reads (ds_read_b64_tr_b16).
 //
-// 2888 windows of 49 tokens, 3 heads, 361 masks:  fp32 tables 4.5 us, forward 61 (2.6 TB/s), backward 125 to 138 (2.1 to 2.3 TB/s; 60 % of the matrix
-// pipe: tiles of 16 make 64 x 64 of 49 x 49; without HBM traffic it takes 122, without products 77), join 5.  bf16: forward 24 (3.3 TB/s), backward 54
-// (2.6 TB/s; VALU, LDS and HBM each 40 % busy; without products 43).  Tiles of 32, two waves to a window: 75 + 145 and 26.5 + 66; raised wave priority
-// around the products and LDS reads pinned ahead of them: level.
+// 2888 windows of 49 tokens, 3 heads, 361 masks (217 MB forward, 380 MB backward in fp32):  fp32 tables 4.7 us, forward 59 (3.7 TB/s; matrix pipe 45 % busy),
+// backward 126 to 138 (2.8 to 3.0 TB/s; matrix pipe 52 % busy, tiles of 16 make 64 x 64 of 49 x 49; without HBM traffic it takes 122, without products 77),
+// join 5.  bf16: forward 24 (4.6 TB/s), backward 54 (3.5 TB/s; VALU 37 %, LDS 36 % busy and 12 % more in conflicts; without products 43).  Tiles of 32, two waves
+// to a window: 75 + 145 and 26.5 + 66; raised wave priority around the products and LDS reads pinned ahead of them: level.
+// 2048 windows of 64 tokens, 3 heads, 256 masks (201 and 352 MB in fp32): fp32 53 + 96 us (3.8 and 3.7 TB/s), bf16 30 + 41 (3.4 and 4.3 TB/s).
 #include <math.h>
 
 #include <type_traits>
@@ -371,7 +372,8 @@ __device__ __forceinline__ int logical_block() {
 }
 
 // waves per SIMD that the registers leave room for (7 x 7 windows, stage 1: forward fp32 5 without the bias in registers level, bf16 4 and 6 without it 24
-// and 27 against 23 us; backward 4, then with P and dS crossing one after the other, level, 2: 143 against 130 us, bf16 59 against 54)
+// and 27 against 23 us; backward 4, then with P and dS crossing one after the other, level, 2: 143 against 130 us, bf16 59 against 54).  At 61 to 64 tokens the
+// bf16 forward's 5 leave 17 registers in scratch (40 bytes a lane); no other bound was measured there.
 template <typename T>
 constexpr int kFwdWaves = sizeof(T) == 4 ? 4 : 5;
 constexpr int kBwdWaves = 3;
