@@ -126,9 +126,35 @@ class WindowAttention(nn.Module):
 
     @staticmethod
     def _update_plan(self, _keys):
-        """a checkpoint brought its own index: a captured step that reads the plan does not come by here again"""
+        """a checkpoint brought its own index and table: a captured step that reads what was derived from them does not come by here again"""
         if '_plan' in self.__dict__:
             self.bias_plan
+        with torch.no_grad():
+            for kind, held, *how in self.__dict__.get('_in_graphs', ()):
+                if kind == 'bias':
+                    held.copy_(self._pack_bias(*how))
+                elif kind == 'additive':
+                    held.copy_(self._additive(*how))
+
+    def _keep_for_replays(self, kind, held, *how):
+        """A cached tensor that is read in a capture: the graph has its address, so it lives on when the cache moves to another geometry or table."""
+        first = held[0] if isinstance(held, tuple) else held
+        if first.is_cuda and torch.cuda.is_current_stream_capturing():
+            kept = self.__dict__.setdefault('_in_graphs', [])
+            if not any(k[1] is held for k in kept):
+                kept.append((kind, held, *how))
+
+    def _pack_bias(self, n, h):
+        tbl = self.relative_position_bias_table
+        return window_attn.pack_tables(tbl[self.relative_position_index.view(-1)].view(n, n, h).permute(2, 0, 1), float('-inf'))[0]
+
+    def _additive(self, n, h, bw, mask, dtype):
+        """bias + mask [windows or 1, h, n, n] in the attention's type"""
+        add = self._bias(n, h).unsqueeze(0)
+        if mask is not None:
+            nw = mask.shape[0]
+            add = (add + mask.unsqueeze(1)).repeat(bw // nw, 1, 1, 1)  # windows of one image are contiguous
+        return add.to(dtype)
 
     def _bias_packed(self, n, h):
         """relative position bias [h, N, N] in the attention kernel's accumulator layout (padded keys = -inf); cached for a frozen table."""
@@ -136,9 +162,10 @@ class WindowAttention(nn.Module):
         sig = (tbl._version, tbl.data_ptr(), n)
         hit = None if tbl.requires_grad else getattr(self, '_bias_p_cache', None)     # a trainable table is gathered every call: fused
         if hit is not None and hit[0] == sig:                                          # optimizers do not bump _version
+            self._keep_for_replays('bias', hit[1], n, h)
             return hit[1]
         with torch.no_grad():
-            bp = window_attn.pack_tables(tbl[self.relative_position_index.view(-1)].view(n, n, h).permute(2, 0, 1), float('-inf'))[0]
+            bp = self._pack_bias(n, h)
         if not tbl.requires_grad and not (tbl.is_cuda and torch.cuda.is_current_stream_capturing()):
             object.__setattr__(self, '_bias_p_cache', (sig, bp))
         return bp
@@ -157,6 +184,7 @@ class WindowAttention(nn.Module):
         sig = (mask.data_ptr(), mask._version, tuple(mask.shape))
         hit = getattr(self, '_mask_p_cache', None)
         if hit is not None and hit[0] == sig:
+            self._keep_for_replays('mask', hit[1])
             return hit[1]
         with torch.no_grad():
             mp = window_attn.pack_tables(mask, 0.0, True)
@@ -183,14 +211,8 @@ class WindowAttention(nn.Module):
             # a graph to build (a Swin student): the same product with its gradients, one kernel each way (csrc/window_train.hip)
             return self.proj_drop(self.proj(window_attn.attention(qkv, self._bias(n, h), mask, h, self.scale)))
         q, k, v = qkv.reshape(bw, n, 3, h, c // h).permute(2, 0, 3, 1, 4)
-        def additive():
-            add = self._bias(n, h).unsqueeze(0)
-            if mask is not None:
-                nw = mask.shape[0]
-                add = (add + mask.unsqueeze(1)).repeat(bw // nw, 1, 1, 1)  # windows of one image are contiguous
-            return add.to(q.dtype)
         if tbl.requires_grad:
-            add = additive()
+            add = self._additive(n, h, bw, mask, q.dtype)
         else:
             # frozen network (the config-4 teacher): bias gather + mask add + the repeat over the batch -- a 111 MB copy per stage-1 block --
             # are the same tensor every step.  ONE entry per module, the most recent geometry (keyed entries were never evicted, so
@@ -200,9 +222,10 @@ class WindowAttention(nn.Module):
             hit = getattr(self, '_add_cache', None)
             if hit is not None and hit[0] == sig:
                 add = hit[1]
+                self._keep_for_replays('additive', add, n, h, bw, mask, q.dtype)
             else:
                 with torch.no_grad():
-                    add = additive()
+                    add = self._additive(n, h, bw, mask, q.dtype)
                 if not (q.is_cuda and torch.cuda.is_current_stream_capturing()):
                     object.__setattr__(self, '_add_cache', (sig, add))
         drop = self.attn_drop.p if self.training else 0.

@@ -102,3 +102,44 @@ def test_partially_frozen_swin_keeps_the_gradients_of_its_trainable_parts():
         a, b = grads[True][n], grads[False][n]
         assert a is not None and float(b.abs().max()) > 0, n
         assert float((a - b).abs().max()) <= 2e-4 * float(b.abs().max()) + 1e-9, n
+
+
+@pytest.mark.parametrize('ws', [(7, 7), (5, 5)])
+def test_a_captured_frozen_block_keeps_its_tables(ws):
+    """what a frozen window attention caches -- packed bias and mask (7 x 7), the additive tensor (other windows) -- is read by a captured forward: it outlives a
+    forward with another mask, and follows a checkpoint that is loaded after the capture"""
+    from segdistill_amd.backbones.swin import WindowAttention
+    torch.manual_seed(11)
+    att = WindowAttention(64, ws, 2).cuda().eval().requires_grad_(False)
+    torch.nn.init.normal_(att.relative_position_bias_table)
+    n = ws[0] * ws[1]
+    x = torch.randn(8, n, 64, device='cuda')
+    masks = [torch.where(torch.rand(4, n, n, device='cuda') < 0.3, -100.0, 0.0) for _ in range(2)]
+    sd = {k: v.clone() for k, v in att.state_dict().items()}
+    sd['relative_position_bias_table'] = sd['relative_position_bias_table'].normal_(std=3.0)
+    other = WindowAttention(64, ws, 2).cuda().eval().requires_grad_(False)
+    other.load_state_dict(sd)
+    with torch.no_grad():
+        want, loaded = att(x, masks[0]).clone(), other(x, masks[0]).clone()
+        assert float((want - loaded).abs().max()) > 0.01
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            att(x, masks[0])
+        torch.cuda.current_stream().wait_stream(side)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = att(x, masks[0])
+
+        def replay():
+            junk = [torch.full((k,), float('nan'), device='cuda') for k in (4 * 4096, 2 * 4096, 8 * 2 * n * n, 2 * n * n) * 20]
+            graph.replay()
+            torch.cuda.synchronize()
+            del junk
+            return out
+        assert torch.equal(replay(), want)
+        att(x, masks[1])
+        assert torch.equal(replay(), want)
+        att.load_state_dict(sd)
+        assert torch.equal(replay(), loaded)
+        assert torch.equal(att(x, masks[0]), loaded) and torch.equal(replay(), loaded)
