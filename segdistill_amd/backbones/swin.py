@@ -26,6 +26,7 @@ from ..builder import BACKBONES
 from ..layernorm import HipLayerNorm, layernorm_map, map_supported          # nn.LayerNorm subclass: same keys, HIP kernels on CUDA tokens (ATen's ran 3.9 ms of a config-4 step)
 from .. import rel_bias, window_attn
 from ..ops import _transformed
+from ..window_attn import _version
 from ..layers import DropPath, to_2tuple, trunc_normal_
 
 
@@ -108,7 +109,7 @@ class WindowAttention(nn.Module):
     def bias_plan(self):
         """the rel_bias.BucketPlan of relative_position_index as it is now; None where it cannot be read: on the meta device, or changed and being captured"""
         index, held = self.relative_position_index, self.__dict__.get('_plan')
-        version = None if index.is_inference() else index._version
+        version = _version(index)
         if held is not None and held[1] is index and held[2] == version is not None:
             return held[0]
         if index.is_meta or (index.is_cuda and torch.cuda.is_current_stream_capturing()):
@@ -159,7 +160,7 @@ class WindowAttention(nn.Module):
     def _bias_packed(self, n, h):
         """relative position bias [h, N, N] in the attention kernel's accumulator layout (padded keys = -inf); cached for a frozen table."""
         tbl = self.relative_position_bias_table
-        sig = (tbl._version, tbl.data_ptr(), n)
+        sig = (_version(tbl), tbl.data_ptr(), n)
         hit = None if tbl.requires_grad else getattr(self, '_bias_p_cache', None)     # a trainable table is gathered every call: fused
         if hit is not None and hit[0] == sig:                                          # optimizers do not bump _version
             self._keep_for_replays('bias', hit[1], n, h)
@@ -167,7 +168,7 @@ class WindowAttention(nn.Module):
         with torch.no_grad():
             bp = self._pack_bias(n, h)
         if not tbl.requires_grad and not (tbl.is_cuda and torch.cuda.is_current_stream_capturing()):
-            object.__setattr__(self, '_bias_p_cache', (sig, bp))
+            object.__setattr__(self, '_bias_p_cache', (sig, bp, tbl.detach()))          # (held: its address stays its own)
         return bp
 
     def _bias(self, n, h):
@@ -181,7 +182,7 @@ class WindowAttention(nn.Module):
     def _mask_packed(self, mask):
         if mask is None:
             return None, None
-        sig = (mask.data_ptr(), mask._version, tuple(mask.shape))
+        sig = (mask.data_ptr(), _version(mask), tuple(mask.shape), mask.stride())
         hit = getattr(self, '_mask_p_cache', None)
         if hit is not None and hit[0] == sig:
             self._keep_for_replays('mask', hit[1])
@@ -189,7 +190,7 @@ class WindowAttention(nn.Module):
         with torch.no_grad():
             mp = window_attn.pack_tables(mask, 0.0, True)
         if not (mask.is_cuda and torch.cuda.is_current_stream_capturing()):
-            object.__setattr__(self, '_mask_p_cache', (sig, mp))
+            object.__setattr__(self, '_mask_p_cache', (sig, mp, mask))
         return mp
 
     def forward(self, x, mask=None):
@@ -218,7 +219,7 @@ class WindowAttention(nn.Module):
             # are the same tensor every step.  ONE entry per module, the most recent geometry (keyed entries were never evicted, so
             # an eval run over variable-size images grew by one [B*nW, h, N, N] tensor per distinct size and shifted block); a checkpoint load
             # bumps the table's version and invalidates it; nothing is stored while a hipGraph is being captured
-            sig = (tbl._version, tbl.data_ptr(), None if mask is None else (mask.data_ptr(), mask._version), bw, q.dtype)
+            sig = (_version(tbl), tbl.data_ptr(), None if mask is None else (mask.data_ptr(), _version(mask), tuple(mask.shape), mask.stride()), bw, q.dtype)
             hit = getattr(self, '_add_cache', None)
             if hit is not None and hit[0] == sig:
                 add = hit[1]
@@ -227,7 +228,7 @@ class WindowAttention(nn.Module):
                 with torch.no_grad():
                     add = self._additive(n, h, bw, mask, q.dtype)
                 if not (q.is_cuda and torch.cuda.is_current_stream_capturing()):
-                    object.__setattr__(self, '_add_cache', (sig, add))
+                    object.__setattr__(self, '_add_cache', (sig, add, tbl.detach(), mask))
         drop = self.attn_drop.p if self.training else 0.
         out = F.scaled_dot_product_attention(q, k, v, attn_mask=add, dropout_p=drop, scale=self.scale)
         return self.proj_drop(self.proj(out.transpose(1, 2).reshape(bw, n, c)))

@@ -56,6 +56,7 @@ def train_supported(qkv, n, head_dim):
 
 
 def _version(t):
+    """the counter of writes in place; None where there is none (no tensor, or one made in inference mode)"""
     return None if t is None or t.is_inference() else t._version
 
 

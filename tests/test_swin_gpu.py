@@ -143,3 +143,24 @@ def test_a_captured_frozen_block_keeps_its_tables(ws):
         att.load_state_dict(sd)
         assert torch.equal(replay(), loaded)
         assert torch.equal(att(x, masks[0]), loaded) and torch.equal(replay(), loaded)
+
+
+@pytest.mark.parametrize('ws', [(7, 7), (5, 5)])
+def test_a_frozen_block_tells_masks_apart_that_share_an_address(ws):
+    """each mask goes before the next one comes, to the same memory; and masks made in inference mode, as an evaluation leaves them.  (Sums of at most 64 terms
+    in fp32, two Linears and a softmax: within 1e-5 of the largest value.)"""
+    from segdistill_amd.backbones.swin import WindowAttention
+    torch.manual_seed(12)
+    att = WindowAttention(64, ws, 2).cuda().eval().requires_grad_(False)
+    n = ws[0] * ws[1]
+    x = torch.randn(8, n, 64, device='cuda')
+    ref = WindowAttention(64, ws, 2).double().eval()
+    ref.load_state_dict({k: v.cpu() for k, v in att.state_dict().items()})
+    with torch.no_grad():
+        for turn in range(6):
+            with torch.inference_mode(turn >= 4):
+                mask = torch.where(torch.rand(4, n, n, device='cuda') < 0.5, -100.0, 0.0)
+            got = att(x, mask).double().cpu()
+            want = ref(x.double().cpu(), mask.double().cpu())
+            assert float((got - want).abs().max()) <= 1e-5 * float(want.abs().max()), turn
+            del mask
